@@ -21,7 +21,9 @@ from .ops import (
     fused_recurrent_gated_delta_rule_fwd,
     gated_delta_rule_chunk_layer,
     gated_delta_rule_decode_layer,
+    gated_linear_unit,
     gated_rms_norm,
+    selective_scan,
     short_convolution,
 )
 
@@ -40,6 +42,8 @@ __all__ = [
     "delta_rule",
     "gated_delta_rule_chunk_layer",
     "gated_delta_rule_decode_layer",
+    "gated_linear_unit",
     "gated_rms_norm",
+    "selective_scan",
     "short_convolution",
 ]

@@ -48,6 +48,16 @@ EXPORTED_SYMBOLS = (
     "gdn_fold_states",
     "gdn_short_conv_fwd",
     "gdn_gated_rmsnorm_fwd",
+    "gdn_short_conv_fwd_bias",
+    "gdn_short_conv_bwd",
+    "gdn_short_conv_bwd_workspace_bytes",
+    "gdn_glu_fwd",
+    "gdn_glu_bwd",
+    "gdn_glu_bwd_workspace_bytes",
+    "gdn_selective_scan_fwd",
+    "gdn_selective_scan_bwd",
+    "gdn_selective_scan_checkpoint_bytes",
+    "gdn_selective_scan_bwd_workspace_bytes",
     "gdn_last_error",
     "gdn_reload_kernel_overrides",
     "gdn_device_error",
@@ -122,6 +132,26 @@ def _declare(lib):
     lib.gdn_gated_rmsnorm_fwd.argtypes = [_vp] * 3 + [ctypes.c_float, _vp, ctypes.c_longlong,
                                                       _i, _i, _vp]
     lib.gdn_gated_rmsnorm_fwd.restype = _i
+    lib.gdn_short_conv_fwd_bias.argtypes = [_vp] * 6 + [_i] * 6 + [_vp]
+    lib.gdn_short_conv_fwd_bias.restype = _i
+    lib.gdn_short_conv_bwd.argtypes = [_vp] * 10 + [_i] * 6 + [_vp, _sz, _vp]
+    lib.gdn_short_conv_bwd.restype = _i
+    lib.gdn_short_conv_bwd_workspace_bytes.argtypes = [_i] * 4
+    lib.gdn_short_conv_bwd_workspace_bytes.restype = _sz
+    lib.gdn_glu_fwd.argtypes = [_vp] * 6 + [_i] * 4 + [_vp]
+    lib.gdn_glu_fwd.restype = _i
+    lib.gdn_glu_bwd.argtypes = [_vp] * 9 + [_i] * 4 + [_vp, _sz, _vp]
+    lib.gdn_glu_bwd.restype = _i
+    lib.gdn_glu_bwd_workspace_bytes.argtypes = [_i] * 3
+    lib.gdn_glu_bwd_workspace_bytes.restype = _sz
+    lib.gdn_selective_scan_fwd.argtypes = [_vp] * 12 + [_i] * 7 + [_vp]
+    lib.gdn_selective_scan_fwd.restype = _i
+    lib.gdn_selective_scan_bwd.argtypes = [_vp] * 20 + [_i] * 7 + [_vp, _sz, _vp]
+    lib.gdn_selective_scan_bwd.restype = _i
+    lib.gdn_selective_scan_checkpoint_bytes.argtypes = [_i] * 4
+    lib.gdn_selective_scan_checkpoint_bytes.restype = _sz
+    lib.gdn_selective_scan_bwd_workspace_bytes.argtypes = [_i] * 5
+    lib.gdn_selective_scan_bwd_workspace_bytes.restype = _sz
     lib.gdn_last_error.argtypes = []
     lib.gdn_last_error.restype = ctypes.c_char_p
     lib.gdn_reload_kernel_overrides.argtypes = []

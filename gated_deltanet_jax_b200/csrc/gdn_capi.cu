@@ -117,6 +117,130 @@ int cuda_status(cudaError_t e, const char* what) {
   return fail(GDN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+// dst from src, or zeros (src NULL), on the stream.
+int carry(void* dst, const void* src, size_t bytes, void* stream, const char* what) {
+  cudaError_t e = src ? cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToDevice,
+                                        (cudaStream_t)stream)
+                      : cudaMemsetAsync(dst, 0, bytes, (cudaStream_t)stream);
+  return cuda_status(e, what);
+}
+
+int check_workspace(const void* ws, size_t have, size_t need, const char* query) {
+  if (need == 0) return GDN_OK;
+  if (!ws || have < need)
+    return fail(GDN_ERR_INVALID, "needs %zu workspace bytes (%s), got %zu", need, query,
+                ws ? have : (size_t)0);
+  if (!aligned16(ws)) return fail(GDN_ERR_INVALID, "the workspace must be 16-byte aligned");
+  return GDN_OK;
+}
+
+int check_dtype(int dtype) {
+  if (dtype != GDN_DTYPE_FP32 && dtype != GDN_DTYPE_BF16)
+    return fail(GDN_ERR_INVALID, "dtype %d is neither GDN_DTYPE_FP32 nor GDN_DTYPE_BF16", dtype);
+  return GDN_OK;
+}
+
+// The arguments that the short convolution's forward and backward share
+// (state_out: the final state, or its gradient).
+int check_short_conv(const float* weight, const float* bias, const void* state_in,
+                     const void* state_out, int B, int T, int C, int K, int activation,
+                     int dtype) {
+  g_err[0] = '\0';
+  if (B < 0 || T < 0 || C < 0) return fail(GDN_ERR_INVALID, "negative size B=%d T=%d C=%d", B, T, C);
+  if (int rc = check_dtype(dtype)) return rc;
+  if (activation != 0 && activation != 1)
+    return fail(GDN_ERR_INVALID, "activation %d is neither 0 (none) nor 1 (silu)", activation);
+  if (K < 1 || K > gdn::kShortConvMaxK)
+    return fail(GDN_ERR_UNSUPPORTED, "kernel size K=%d not supported (1 .. %d)", K,
+                gdn::kShortConvMaxK);
+  if (B > 65535) return fail(GDN_ERR_UNSUPPORTED, "B=%d exceeds 65535", B);
+  if (B == 0 || C == 0) return GDN_OK;
+  if (!gdn::short_conv_supported(C, K, dtype))
+    return fail(GDN_ERR_UNSUPPORTED, "C=%d channels must be a multiple of %d for this dtype", C,
+                dtype == GDN_DTYPE_BF16 ? 8 : 4);
+  if (T > (1 << 30) || (long long)B * ((long long)T + K) * C > (1LL << 40))
+    return fail(GDN_ERR_INVALID, "tensor too large (T > 2^30 or B*T*C > 2^40)");
+  if (!weight || !aligned16(weight))
+    return fail(GDN_ERR_INVALID, "weight must be non-NULL and 16-byte aligned");
+  if (!aligned16(bias)) return fail(GDN_ERR_INVALID, "bias must be 16-byte aligned");
+  if (!aligned16(state_in) || !aligned16(state_out))
+    return fail(GDN_ERR_INVALID, "the conv states must be 16-byte aligned");
+  return GDN_OK;
+}
+
+size_t glu_half_bytes(int M, int I, int dtype) {
+  const size_t e = dtype == GDN_DTYPE_BF16 ? 2 : 4;
+  return ((size_t)M * I * e + 255) / 256 * 256;
+}
+
+int check_glu(const void* x, const void* wg, const void* wu, int M, int D, int I, int dtype) {
+  g_err[0] = '\0';
+  if (M < 0 || D < 0 || I < 0) return fail(GDN_ERR_INVALID, "negative size M=%d D=%d I=%d", M, D, I);
+  if (int rc = check_dtype(dtype)) return rc;
+  // (the CUDA-core form's grid: 65535 row tiles of 64)
+  if (M > 65535 * 64 || I > 65535 * 64 || D > 65535 * 64)
+    return fail(GDN_ERR_UNSUPPORTED, "M=%d, D=%d or I=%d exceeds %d", M, D, I, 65535 * 64);
+  if ((long long)M * (D > I ? D : I) > (1LL << 40) || (long long)I * D > (1LL << 40))
+    return fail(GDN_ERR_INVALID, "tensor too large (more than 2^40 elements)");
+  if (D > 0 && ((M > 0 && !x) || (I > 0 && (!wg || !wu))))
+    return fail(GDN_ERR_INVALID, "x, w_gate and w_up must be non-NULL");
+  if (!aligned16(x) || !aligned16(wg) || !aligned16(wu))
+    return fail(GDN_ERR_INVALID, "x, w_gate and w_up must be 16-byte aligned");
+  return GDN_OK;
+}
+
+int check_scan(const void* x, const void* dt, const float* A, const void* Bm, const void* Cm,
+               const float* D, const void* z, const float* dt_bias, const float* h0, int B, int T,
+               int C, int N, int G, int softplus, int dtype) {
+  g_err[0] = '\0';
+  if (B < 0 || T < 0 || C < 0) return fail(GDN_ERR_INVALID, "negative size B=%d T=%d C=%d", B, T, C);
+  if (int rc = check_dtype(dtype)) return rc;
+  if (softplus != 0 && softplus != 1)
+    return fail(GDN_ERR_INVALID, "softplus must be 0 or 1 (got %d)", softplus);
+  if (N < 1 || N > gdn::kScanMaxStates)
+    return fail(GDN_ERR_UNSUPPORTED, "N=%d states not supported (1 .. %d)", N,
+                gdn::kScanMaxStates);
+  if (G < 1 || C % G)
+    return fail(GDN_ERR_INVALID, "C=%d channels must be a multiple of G=%d groups", C, G);
+  if (B > 65535) return fail(GDN_ERR_UNSUPPORTED, "B=%d exceeds 65535", B);
+  if (T > (1 << 30) || (long long)B * T * C > (1LL << 40) || (long long)B * C * N > (1LL << 40))
+    return fail(GDN_ERR_INVALID, "tensor too large (T > 2^30 or more than 2^40 elements)");
+  if (B == 0 || C == 0) return GDN_OK;
+  if (!A || (T > 0 && (!x || !dt || !Bm || !Cm)))
+    return fail(GDN_ERR_INVALID, "x, dt, A, B and C must be non-NULL");
+  const void* ptrs[9] = {x, dt, A, Bm, Cm, D, z, dt_bias, h0};
+  const char* names[9] = {"x", "dt", "A", "B", "C", "D", "z", "dt_bias", "h0"};
+  for (int i = 0; i < 9; ++i)
+    if (!aligned16(ptrs[i])) return fail(GDN_ERR_INVALID, "%s is not 16-byte aligned", names[i]);
+  return GDN_OK;
+}
+
+gdn::ScanArgs scan_args(const void* x, const void* dt, const float* A, const void* Bm,
+                        const void* Cm, const float* D, const void* z, const float* dt_bias,
+                        const float* h0, int B, int T, int C, int N, int G, int softplus,
+                        int dtype) {
+  gdn::ScanArgs a{};
+  a.x = x;
+  a.dt = dt;
+  a.A = A;
+  a.Bm = Bm;
+  a.Cm = Cm;
+  a.D = D;
+  a.z = z;
+  a.dt_bias = dt_bias;
+  a.h0 = h0;
+  a.B = B;
+  a.T = T;
+  a.C = C;
+  a.N = N;
+  a.G = G;
+  a.softplus = softplus;
+  a.dtype = dtype;
+  const int k = gdn::scan_checkpoint_tokens(N);
+  a.nck = (T + k - 1) / k;
+  return a;
+}
+
 // Grouped heads: q and k carry Hk heads, v / g / beta / state H, with H % Hk == 0.
 int check_groups(int H, int Hk) {
   if (Hk < 0) return fail(GDN_ERR_INVALID, "negative Hk=%d", Hk);
@@ -640,47 +764,196 @@ int gdn_device_error(int clear) {
   return a ? a : (b ? b : (c ? c : (d ? d : e)));
 }
 
-int gdn_abi_version(void) { return (1 << 16) | 10; }
+int gdn_abi_version(void) { return (1 << 16) | 11; }
 
 int gdn_binary_version(void) { return gdn::chunk_scan_binary_version(); }
 
 int gdn_short_conv_fwd(const void* x, const float* weight, const void* state_in, void* state_out,
                        void* y, int B, int T, int C, int K, int activation, int dtype,
                        void* stream) {
-  g_err[0] = '\0';
-  if (B < 0 || T < 0 || C < 0) return fail(GDN_ERR_INVALID, "negative size B=%d T=%d C=%d", B, T, C);
-  if (dtype != GDN_DTYPE_FP32 && dtype != GDN_DTYPE_BF16)
-    return fail(GDN_ERR_INVALID, "dtype %d is neither GDN_DTYPE_FP32 nor GDN_DTYPE_BF16", dtype);
-  if (activation != 0 && activation != 1)
-    return fail(GDN_ERR_INVALID, "activation %d is neither 0 (none) nor 1 (silu)", activation);
-  if (K < 1 || K > gdn::kShortConvMaxK)
-    return fail(GDN_ERR_UNSUPPORTED, "kernel size K=%d not supported (1 .. %d)", K,
-                gdn::kShortConvMaxK);
-  if (B > 65535) return fail(GDN_ERR_UNSUPPORTED, "B=%d exceeds 65535", B);
-  if (B == 0 || C == 0) return GDN_OK;
-  if (!gdn::short_conv_supported(C, K, dtype))
-    return fail(GDN_ERR_UNSUPPORTED, "C=%d channels must be a multiple of %d for this dtype", C,
-                dtype == GDN_DTYPE_BF16 ? 8 : 4);
-  if ((long long)B * ((long long)T + K) * C > (1LL << 40))
-    return fail(GDN_ERR_INVALID, "tensor too large (B*T*C > 2^40)");
-  if (!weight || !aligned16(weight))
-    return fail(GDN_ERR_INVALID, "weight must be non-NULL and 16-byte aligned");
+  return gdn_short_conv_fwd_bias(x, weight, nullptr, state_in, state_out, y, B, T, C, K,
+                                 activation, dtype, stream);
+}
+
+int gdn_short_conv_fwd_bias(const void* x, const float* weight, const float* bias,
+                            const void* state_in, void* state_out, void* y, int B, int T, int C,
+                            int K, int activation, int dtype, void* stream) {
+  int rc = check_short_conv(weight, bias, state_in, state_out, B, T, C, K, activation, dtype);
+  if (rc || B == 0 || C == 0) return rc;
   if (T > 0 && (!x || !y || !aligned16(x) || !aligned16(y)))
     return fail(GDN_ERR_INVALID, "x and y must be non-NULL and 16-byte aligned");
-  if ((state_in && !aligned16(state_in)) || (state_out && !aligned16(state_out)))
-    return fail(GDN_ERR_INVALID, "the conv states must be 16-byte aligned");
   if (T == 0) {
     // nothing to convolve; the state still carries through
     if (!state_out || state_out == state_in || K == 1) return GDN_OK;
-    const size_t bytes = (size_t)B * (K - 1) * C * (dtype == GDN_DTYPE_BF16 ? 2 : 4);
-    cudaError_t e = state_in ? cudaMemcpyAsync(state_out, state_in, bytes,
-                                               cudaMemcpyDeviceToDevice, (cudaStream_t)stream)
-                             : cudaMemsetAsync(state_out, 0, bytes, (cudaStream_t)stream);
-    return cuda_status(e, "gdn_short_conv_fwd (T=0 state copy)");
+    return carry(state_out, state_in, (size_t)B * (K - 1) * C * (dtype == GDN_DTYPE_BF16 ? 2 : 4),
+                 stream, "gdn_short_conv_fwd (T=0 state copy)");
   }
-  return cuda_status(gdn::launch_short_conv(x, weight, state_in, state_out, y, B, T, C, K,
+  return cuda_status(gdn::launch_short_conv(x, weight, bias, state_in, state_out, y, B, T, C, K,
                                             activation, dtype, (cudaStream_t)stream),
                      "gdn_short_conv_fwd");
+}
+
+size_t gdn_short_conv_bwd_workspace_bytes(int B, int T, int C, int K) {
+  if (K < 1 || K > gdn::kShortConvMaxK) return 0;
+  return gdn::short_conv_bwd_workspace_bytes(B, T, C, K);
+}
+
+int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
+                       const void* state_in, const void* dy, const void* dstate_out, void* dx,
+                       float* dweight, float* dbias, void* dstate_in, int B, int T, int C, int K,
+                       int activation, int dtype, void* workspace, size_t ws_bytes,
+                       void* stream) {
+  int rc = check_short_conv(weight, bias, state_in, dstate_out, B, T, C, K, activation, dtype);
+  if (rc || C == 0) return rc;
+  if (!dweight || !aligned16(dweight))
+    return fail(GDN_ERR_INVALID, "dweight must be non-NULL and 16-byte aligned");
+  if (dbias && !aligned16(dbias)) return fail(GDN_ERR_INVALID, "dbias is not 16-byte aligned");
+  if (dstate_in && !aligned16(dstate_in))
+    return fail(GDN_ERR_INVALID, "dstate_in is not 16-byte aligned");
+  if (B == 0 || T == 0) {
+    // no output depends on the weights; the final state is the initial one
+    rc = carry(dweight, nullptr, sizeof(float) * (size_t)K * C, stream, "gdn_short_conv_bwd");
+    if (!rc && dbias)
+      rc = carry(dbias, nullptr, sizeof(float) * (size_t)C, stream, "gdn_short_conv_bwd");
+    if (!rc && dstate_in && B > 0 && K > 1)
+      rc = carry(dstate_in, dstate_out,
+                 (size_t)B * (K - 1) * C * (dtype == GDN_DTYPE_BF16 ? 2 : 4), stream,
+                 "gdn_short_conv_bwd");
+    return rc;
+  }
+  if (!x || !dy || !dx || !aligned16(x) || !aligned16(dy) || !aligned16(dx))
+    return fail(GDN_ERR_INVALID, "x, dy and dx must be non-NULL and 16-byte aligned");
+  if (dx == x || dx == dy)
+    return fail(GDN_ERR_INVALID, "dx may not be x or dy: a token's gradient reads its neighbours");
+  rc = check_workspace(workspace, ws_bytes, gdn::short_conv_bwd_workspace_bytes(B, T, C, K),
+                       "gdn_short_conv_bwd_workspace_bytes");
+  if (rc) return rc;
+  gdn::ShortConvBwdArgs a{x, weight, bias, state_in, dy, dstate_out, dx, dweight, dbias,
+                          dstate_in, static_cast<float*>(workspace), B, T, C, K, activation,
+                          dtype};
+  return cuda_status(gdn::launch_short_conv_bwd(a, (cudaStream_t)stream), "gdn_short_conv_bwd");
+}
+
+int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, void* g, void* u,
+                int M, int D, int I, int dtype, void* stream) {
+  int rc = check_glu(x, w_gate, w_up, M, D, I, dtype);
+  if (rc) return rc;
+  if (M == 0 || I == 0) return GDN_OK;
+  if (!h || !aligned16(h)) return fail(GDN_ERR_INVALID, "h must be non-NULL and 16-byte aligned");
+  if ((g == nullptr) != (u == nullptr))
+    return fail(GDN_ERR_INVALID, "g and u are kept together: both or neither");
+  if (g && (!aligned16(g) || !aligned16(u)))
+    return fail(GDN_ERR_INVALID, "g and u must be 16-byte aligned");
+  gdn::GluArgs a{x, w_gate, w_up, h, g, u, M, D, I, dtype};
+  return cuda_status(gdn::launch_glu_fwd(a, (cudaStream_t)stream), "gdn_glu_fwd");
+}
+
+size_t gdn_glu_bwd_workspace_bytes(int M, int I, int dtype) {
+  if (M <= 0 || I <= 0) return 0;
+  return 2 * glu_half_bytes(M, I, dtype);
+}
+
+int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void* g, const void* u,
+                const void* dh, void* dx, void* dw_gate, void* dw_up, int M, int D, int I,
+                int dtype, void* workspace, size_t ws_bytes, void* stream) {
+  int rc = check_glu(x, w_gate, w_up, M, D, I, dtype);
+  if (rc) return rc;
+  if ((dw_gate == nullptr) != (dw_up == nullptr))
+    return fail(GDN_ERR_INVALID, "dw_gate and dw_up are formed together: both or neither");
+  const void* outs[3] = {dx, dw_gate, dw_up};
+  for (const void* p : outs)
+    if (p && !aligned16(p)) return fail(GDN_ERR_INVALID, "the gradients must be 16-byte aligned");
+  if (M > 0 && I > 0) {
+    const void* ptrs[3] = {g, u, dh};
+    for (const void* p : ptrs)
+      if (!p || !aligned16(p))
+        return fail(GDN_ERR_INVALID, "g, u and dh must be non-NULL and 16-byte aligned");
+    rc = check_workspace(workspace, ws_bytes, gdn_glu_bwd_workspace_bytes(M, I, dtype),
+                         "gdn_glu_bwd_workspace_bytes");
+    if (rc) return rc;
+  }
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  gdn::GluBwdArgs a{x, w_gate, w_up, g, u, dh, ws, ws ? ws + glu_half_bytes(M, I, dtype) : nullptr,
+                    dx, dw_gate, dw_up, M, D, I, dtype};
+  return cuda_status(gdn::launch_glu_bwd(a, (cudaStream_t)stream), "gdn_glu_bwd");
+}
+
+size_t gdn_selective_scan_checkpoint_bytes(int B, int T, int C, int N) {
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > gdn::kScanMaxStates) return 0;
+  return gdn::scan_checkpoint_bytes(B, T, C, N);
+}
+
+int gdn_selective_scan_fwd(const void* x, const void* dt, const float* A, const void* Bm,
+                           const void* Cm, const float* D, const void* z, const float* dt_bias,
+                           const float* h0, void* y, float* hT, float* checkpoints, int B, int T,
+                           int C, int N, int G, int softplus, int dtype, void* stream) {
+  int rc = check_scan(x, dt, A, Bm, Cm, D, z, dt_bias, h0, B, T, C, N, G, softplus, dtype);
+  if (rc || B == 0 || C == 0) return rc;
+  if ((T > 0 && !y) || !aligned16(y) || !aligned16(hT) || !aligned16(checkpoints))
+    return fail(GDN_ERR_INVALID, "y must be non-NULL; y, hT and checkpoints 16-byte aligned");
+  if (T == 0) {
+    if (!hT || hT == h0) return GDN_OK;
+    return carry(hT, h0, sizeof(float) * (size_t)B * C * N, stream,
+                 "gdn_selective_scan_fwd (T=0 state copy)");
+  }
+  gdn::ScanArgs a = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, B, T, C, N, G, softplus, dtype);
+  a.y = y;
+  a.hT = hT;
+  a.ckpt = checkpoints;
+  return cuda_status(gdn::launch_selective_scan(a, (cudaStream_t)stream),
+                     "gdn_selective_scan_fwd");
+}
+
+size_t gdn_selective_scan_bwd_workspace_bytes(int B, int T, int C, int N, int G) {
+  if (B <= 0 || T < 0 || C <= 0 || N <= 0 || N > gdn::kScanMaxStates || G <= 0 || C % G) return 0;
+  return gdn::selective_scan_bwd_workspace_bytes(B, T, C, N, G);
+}
+
+int gdn_selective_scan_bwd(const void* x, const void* dt, const float* A, const void* Bm,
+                           const void* Cm, const float* D, const void* z, const float* dt_bias,
+                           const float* checkpoints, const void* dy, const float* dhT, void* dx,
+                           void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz,
+                           float* ddt_bias, float* dh0, int B, int T, int C, int N, int G,
+                           int softplus, int dtype, void* workspace, size_t ws_bytes,
+                           void* stream) {
+  int rc = check_scan(x, dt, A, Bm, Cm, D, z, dt_bias, nullptr, B, T, C, N, G, softplus, dtype);
+  if (rc || C == 0) return rc;
+  const void* ptrs[11] = {checkpoints, dy, dhT, dx, ddt, dA, dB, dC, dD, dz, ddt_bias};
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return fail(GDN_ERR_INVALID, "the gradients must be 16-byte aligned");
+  if (!aligned16(dh0)) return fail(GDN_ERR_INVALID, "dh0 is not 16-byte aligned");
+  if (!dA) return fail(GDN_ERR_INVALID, "dA must be non-NULL");
+  if ((D == nullptr) != (dD == nullptr) || (z == nullptr) != (dz == nullptr) ||
+      (dt_bias == nullptr) != (ddt_bias == nullptr))
+    return fail(GDN_ERR_INVALID, "dD, dz and ddt_bias are given exactly when D, z and dt_bias are");
+  if (B > 0 && T > 0 && (!checkpoints || !dy || !dx || !ddt || !dB || !dC))
+    return fail(GDN_ERR_INVALID, "checkpoints, dy, dx, ddt, dB and dC must be non-NULL");
+  if (B == 0) {
+    rc = carry(dA, nullptr, sizeof(float) * (size_t)C * N, stream, "gdn_selective_scan_bwd");
+    if (!rc && dD) rc = carry(dD, nullptr, sizeof(float) * (size_t)C, stream, "dD");
+    if (!rc && ddt_bias) rc = carry(ddt_bias, nullptr, sizeof(float) * (size_t)C, stream, "ddt_bias");
+    return rc;
+  }
+  rc = check_workspace(workspace, ws_bytes, gdn::selective_scan_bwd_workspace_bytes(B, T, C, N, G),
+                       "gdn_selective_scan_bwd_workspace_bytes");
+  if (rc) return rc;
+  gdn::ScanBwdArgs a{};
+  a.fwd = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, nullptr, B, T, C, N, G, softplus, dtype);
+  a.fwd.ckpt = const_cast<float*>(checkpoints);
+  a.dy = dy;
+  a.dhT = dhT;
+  a.dx = dx;
+  a.ddt = ddt;
+  a.dA = dA;
+  a.dB = dB;
+  a.dC = dC;
+  a.dD = dD;
+  a.dz = dz;
+  a.ddt_bias = ddt_bias;
+  a.dh0 = dh0;
+  a.part = static_cast<float*>(workspace);
+  return cuda_status(gdn::launch_selective_scan_bwd(a, (cudaStream_t)stream),
+                     "gdn_selective_scan_bwd");
 }
 
 int gdn_gated_rmsnorm_fwd(const void* o, const void* gate, const float* weight, float eps,

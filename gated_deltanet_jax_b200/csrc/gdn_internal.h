@@ -279,17 +279,115 @@ cudaError_t launch_bwd_grads_tc(const BwdGradsArgs& a, cudaStream_t st);
 int device_error_bwd_grads(bool clear);
 
 // The layer's elementwise work (layer_ops.cu).  Short convolution + SiLU
-// (model.py:15-40): x, y [B,T,C], w [K,C] fp32, states [B,K-1,C] in x's dtype;
+// (model.py:15-40): x, y [B,T,C], w [K,C] fp32, bias [C] fp32 or NULL, states
+// [B,K-1,C] in x's dtype;
 // C a multiple of 8 (bf16) or 4 (fp32), K <= kShortConvMaxK.
 constexpr int kShortConvMaxK = 8;
 bool short_conv_supported(int C, int K, int dtype);
-cudaError_t launch_short_conv(const void* x, const float* w, const void* state_in,
-                              void* state_out, void* y, int B, int T, int C, int K, int act,
+cudaError_t launch_short_conv(const void* x, const float* w, const float* bias,
+                              const void* state_in, void* state_out, void* y, int B, int T, int C, int K, int act,
                               int dtype, cudaStream_t st);
+// Its gradients (short_conv_bwd.cu).  part: short_conv_bwd_workspace_bytes() of
+// scratch; dbias, dstate_in NULL: not wanted; dstate_out NULL: zero.
+struct ShortConvBwdArgs {
+  const void* x;
+  const float* w;
+  const float* bias;
+  const void* state_in;
+  const void* dy;
+  const void* dstate_out;
+  void* dx;
+  float* dw;
+  float* dbias;
+  void* dstate_in;
+  float* part;
+  int B, T, C, K, act, dtype;
+};
+size_t short_conv_bwd_workspace_bytes(int B, int T, int C, int K);
+cudaError_t launch_short_conv_bwd(const ShortConvBwdArgs& a, cudaStream_t st);
+// out[i] = sum over p < parts of part[p stride + i], i < n, in a fixed order.
+cudaError_t launch_sum_partials(const float* part, float* out, long long parts, long long stride,
+                                long long n, cudaStream_t st);
 // Gated RMSNorm (model.py:41-53) over `rows` rows of dv; o and y may alias.
 bool gated_norm_supported(int dv, int dtype);
 cudaError_t launch_gated_norm(const void* o, const void* gate, const float* w, void* y,
                               long long rows, int dv, float eps, int dtype, cudaStream_t st);
+
+// The gated linear unit h = silu(x Wg^T) * (x Wu^T) (glu.cu): x [M,D], wg, wu
+// [I,D], h [M,I], all in one dtype; g, u [M,I] (the two projections, kept for
+// the backward) or both NULL.
+struct GluArgs {
+  const void* x;
+  const void* wg;
+  const void* wu;
+  void* h;
+  void* g;
+  void* u;
+  int M, D, I, dtype;
+};
+cudaError_t launch_glu_fwd(const GluArgs& a, cudaStream_t st);
+// Its gradients from g, u and dh [M,I]; dg, du [M,I] are scratch.  dx [M,D] or
+// NULL; dwg, dwu [I,D] or both NULL.
+struct GluBwdArgs {
+  const void* x;
+  const void* wg;
+  const void* wu;
+  const void* g;
+  const void* u;
+  const void* dh;
+  void* dg;
+  void* du;
+  void* dx;
+  void* dwg;
+  void* dwu;
+  int M, D, I, dtype;
+};
+cudaError_t launch_glu_bwd(const GluBwdArgs& a, cudaStream_t st);
+
+// Selective state-space scan (selective_scan.cu): x, dt, z, y [B,T,C], B, C
+// [B,T,G,N] in one dtype (z NULL: no gate); A [C,N], D, dt_bias [C] fp32 (D,
+// dt_bias may be NULL); h0, hT [B,C,N] fp32 (may be NULL, may alias).  ckpt
+// (NULL: not wanted): the state entering every scan_checkpoint_tokens(N)-th
+// token, [B][nck][C][scan_padded_states(N)] fp32, for the backward.
+constexpr int kScanMaxStates = 64;
+struct ScanArgs {
+  const void* x;
+  const void* dt;
+  const float* A;
+  const void* Bm;
+  const void* Cm;
+  const float* D;
+  const void* z;
+  const float* dt_bias;
+  const float* h0;
+  void* y;
+  float* hT;
+  float* ckpt;
+  int B, T, C, N, G, softplus, dtype, nck;
+};
+int scan_padded_states(int N);
+int scan_checkpoint_tokens(int N);
+size_t scan_checkpoint_bytes(int B, int T, int C, int N);
+cudaError_t launch_selective_scan(const ScanArgs& a, cudaStream_t st);
+// Its gradients (selective_scan_bwd.cu).  fwd: the forward's arguments with its
+// ckpt (y and hT not read); part: selective_scan_bwd_workspace_bytes() of scratch.
+struct ScanBwdArgs {
+  ScanArgs fwd;
+  const void* dy;
+  const float* dhT;   // NULL: zero
+  void* dx;
+  void* ddt;
+  float* dA;
+  void* dB;
+  void* dC;
+  float* dD;          // NULL when D is
+  void* dz;           // NULL when z is
+  float* ddt_bias;    // NULL when dt_bias is
+  float* dh0;         // NULL: not wanted
+  float* part;
+};
+size_t selective_scan_bwd_workspace_bytes(int B, int T, int C, int N, int G);
+cudaError_t launch_selective_scan_bwd(const ScanBwdArgs& a, cudaStream_t st);
 
 // The sequence split's hand-off: out[0] = h0, out[p + 1] = M_p out[p] + S_p for
 // P segments of BH heads (dk = 128, dv % 32 == 0; S, M rows of `ld` floats).

@@ -2,7 +2,7 @@
 // op kernels do not fuse it (model.py:15-53, 119-153):
 //
 //   short_conv_kernel   ShortConvolution (model.py:15-40): a causal depthwise
-//                       convolution over time, kernel K, no bias, then SiLU,
+//                       convolution over time, kernel K, optional bias, then SiLU,
 //                       with an optional state of the K - 1 inputs before the
 //                       first token (decode) and the K - 1 last inputs out;
 //   gated_norm_kernel   FusedRMSNormGated (model.py:41-53) over the op's output:
@@ -57,7 +57,8 @@ __device__ __forceinline__ float silu_acc(float x) { return x / (1.f + expf(-x))
 
 constexpr int kConvThreads = 128;
 
-// x, y [B, T, C]; w [K, C] fp32 (the flax kernel (K, 1, C) as stored);
+// x, y [B, T, C]; w [K, C] fp32 (the flax kernel (K, 1, C) as stored); bias [C]
+// fp32 or NULL;
 // state_in / state_out [B, K - 1, C] in x's dtype (NULL: zeros / not wanted).
 // Block (channel vectors, b, token tile of TT).  The K - 1 inputs before the
 // tile are read as its halo (from the state before token 0); the tile then
@@ -65,7 +66,7 @@ constexpr int kConvThreads = 128;
 template <typename Tin, int K>
 __global__ void __launch_bounds__(kConvThreads)
 short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
-                  const Tin* state_in, Tin* state_out, Tin* __restrict__ y, int T, int C,
+                  const float* __restrict__ bias, const Tin* state_in, Tin* state_out, Tin* __restrict__ y, int T, int C,
                   int TT, int act) {
   using V = Vec16<Tin>;
   constexpr int N = V::N;
@@ -82,6 +83,9 @@ short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
       const float4 q = *reinterpret_cast<const float4*>(w + (size_t)j * C + c + e);
       wk[j][e] = q.x; wk[j][e + 1] = q.y; wk[j][e + 2] = q.z; wk[j][e + 3] = q.w;
     }
+  float bs[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) bs[e] = bias ? bias[c + e] : 0.f;
   const Tin* xb = x + (size_t)b * T * C + c;
   // win[j] = input at token t - (K - 1) + j for the next output t
   float win[K > 1 ? K - 1 : 1][N];
@@ -105,6 +109,7 @@ short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
       float acc = wk[K - 1][e] * cur[e];
 #pragma unroll
       for (int j = 0; j < K - 1; ++j) acc = fmaf(wk[j][e], win[j][e], acc);
+      if (bias) acc += bs[e];
       out[e] = act ? silu_acc(acc) : acc;
     }
     V::store(y + ((size_t)b * T + t) * C + c, out);
@@ -170,8 +175,8 @@ gated_norm_kernel(const Tin* o, const Tin* __restrict__ gate, const float* __res
 }
 
 template <typename Tin>
-cudaError_t conv_dispatch(const void* x, const float* w, const void* si, void* so, void* y,
-                          int B, int T, int C, int K, int TT, int act, cudaStream_t st) {
+cudaError_t conv_dispatch(const void* x, const float* w, const float* bias, const void* si,
+                          void* so, void* y, int B, int T, int C, int K, int TT, int act, cudaStream_t st) {
   constexpr int N = Vec16<Tin>::N;
   const dim3 grid((C / N + kConvThreads - 1) / kConvThreads, B, (T + TT - 1) / TT);
   const Tin* xi = static_cast<const Tin*>(x);
@@ -180,8 +185,8 @@ cudaError_t conv_dispatch(const void* x, const float* w, const void* si, void* s
   Tin* yo = static_cast<Tin*>(y);
 #define GDN_CONV_CASE(KK)                                                                   \
   case KK:                                                                                  \
-    short_conv_kernel<Tin, KK><<<grid, kConvThreads, 0, st>>>(xi, w, s_in, sout, yo, T, C, TT, \
-                                                              act);                         \
+    short_conv_kernel<Tin, KK><<<grid, kConvThreads, 0, st>>>(xi, w, bias, s_in, sout, yo, T, C, \
+                                                              TT, act);                     \
     break;
   switch (K) {
     GDN_CONV_CASE(1)
@@ -205,8 +210,8 @@ bool short_conv_supported(int C, int K, int dtype) {
   return K >= 1 && K <= kShortConvMaxK && C > 0 && C % n == 0;
 }
 
-cudaError_t launch_short_conv(const void* x, const float* w, const void* state_in,
-                              void* state_out, void* y, int B, int T, int C, int K, int act,
+cudaError_t launch_short_conv(const void* x, const float* w, const float* bias,
+                              const void* state_in, void* state_out, void* y, int B, int T, int C, int K, int act,
                               int dtype, cudaStream_t st) {
   if (B == 0 || T == 0) return cudaSuccess;
   if (!short_conv_supported(C, K, dtype) || B > 65535) return cudaErrorInvalidValue;
@@ -216,8 +221,9 @@ cudaError_t launch_short_conv(const void* x, const float* w, const void* state_i
   if (state_in && state_in == state_out) TT = T;
   if ((T + TT - 1) / TT > 65535) TT = (T + 65534) / 65535;
   return dtype == kBF16
-             ? conv_dispatch<__nv_bfloat16>(x, w, state_in, state_out, y, B, T, C, K, TT, act, st)
-             : conv_dispatch<float>(x, w, state_in, state_out, y, B, T, C, K, TT, act, st);
+             ? conv_dispatch<__nv_bfloat16>(x, w, bias, state_in, state_out, y, B, T, C, K, TT, act,
+                                            st)
+             : conv_dispatch<float>(x, w, bias, state_in, state_out, y, B, T, C, K, TT, act, st);
 }
 
 bool gated_norm_supported(int dv, int dtype) {

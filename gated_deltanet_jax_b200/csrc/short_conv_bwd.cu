@@ -1,0 +1,263 @@
+// Gradients of the short convolution (layer_ops.cu: a causal depthwise
+// convolution over time, kernel K, optional bias, then SiLU or nothing).
+//
+// With xe the inputs behind the K - 1 rows of the entering window,
+//   pre[t] = bias + sum_j w[j] xe[t + j],   y[t] = act(pre[t]),
+//   dpre[t] = dy[t] act'(pre[t]),
+//   dxe[s]  = sum_j w[j] dpre[s - j]   (+ the final window's gradient on the last K - 1 rows),
+//   dw[j]   = sum_{b,t} dpre[t] xe[t + j],   dbias = sum_{b,t} dpre[t].
+//
+// HBM-bound: x and dy are read once and dx is written once (pre is formed
+// again from x; it is not kept between the passes).  A thread owns four
+// channels and walks a tile of tokens with x and dpre in sliding register
+// windows; a tile reads K - 1 rows before it and K - 1 after it again.  The
+// sums over tokens stay in registers (fp32) and leave as one partial row per
+// tile, which a second kernel adds up in a fixed order: no atomics, the same
+// bits on every run.
+#include "gdn_common.cuh"
+#include "gdn_internal.h"
+
+namespace gdn {
+
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kVec = 4;        // channels of a thread: 8 bytes of bf16, 16 of fp32
+constexpr int kAhead = 4;      // tokens whose loads are in flight together
+
+__device__ __forceinline__ void ld4(const float* p, float (&v)[kVec]) {
+  const float4 q = load4(p);
+  v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+}
+__device__ __forceinline__ void ld4(const __nv_bfloat16* p, float (&v)[kVec]) {
+  const float4 q = load4(p);
+  v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+}
+
+// Block (channel group, token tile, row b).  part [B * tiles][K + 1][C]: this
+// tile's sums for dw[0 .. K - 1] and dbias.
+template <typename Tin, int K>
+__global__ void __launch_bounds__(kThreads)
+short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
+                      const float* __restrict__ bias, const Tin* __restrict__ state_in,
+                      const Tin* __restrict__ dy, const Tin* __restrict__ dstate_out,
+                      Tin* __restrict__ dx, Tin* __restrict__ dstate_in,
+                      float* __restrict__ part, int T, int C, int TT, int act) {
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * kVec;
+  if (c >= C) return;
+  const int b = blockIdx.z;
+  const int t0 = blockIdx.y * TT;
+  const int t1 = min(T, t0 + TT);
+  constexpr int W = K > 1 ? K - 1 : 1;
+  float wk[K][kVec], bs[kVec], win[W][kVec], dwin[W][kVec], dw[K][kVec], db[kVec];
+#pragma unroll
+  for (int j = 0; j < K; ++j) ld4(w + (size_t)j * C + c, wk[j]);
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    bs[e] = bias ? bias[c + e] : 0.f;
+    db[e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < K; ++j) dw[j][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) dwin[j][e] = 0.f;
+  }
+  const size_t row0 = (size_t)b * T;
+  // win[j] = xe[t + j] for the next token t (the K - 1 inputs before it)
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) {
+    const int tt = t0 - (K - 1) + j;
+    if (tt >= 0) {
+      ld4(x + (row0 + tt) * C + c, win[j]);
+    } else if (state_in) {
+      ld4(state_in + ((size_t)b * (K - 1) + (K - 1) + tt) * C + c, win[j]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) win[j][e] = 0.f;
+    }
+  }
+  // Token t closes row s = t - (K - 1) of dxe: dxe[s] takes dpre[s .. t].
+  const int tend = t1 + K - 1;
+  for (int tb = t0; tb < tend; tb += kAhead) {
+    float xv[kAhead][kVec], gv[kAhead][kVec];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int t = tb + i;
+      if (t < T && t < tend) {
+        ld4(x + (row0 + t) * C + c, xv[i]);
+        ld4(dy + (row0 + t) * C + c, gv[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) xv[i][e] = gv[i][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int t = tb + i;
+      if (t >= tend) break;
+      float dpre[kVec], out[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        float pre = fmaf(wk[K - 1][e], xv[i][e], bs[e]);
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) pre = fmaf(wk[j][e], win[j][e], pre);
+        float d = gv[i][e];
+        if (act) {
+          const float sg = 1.f / (1.f + __expf(-pre));
+          d *= sg * fmaf(pre, 1.f - sg, 1.f);
+        }
+        if (t >= T) d = 0.f;
+        dpre[e] = d;
+        if (t < t1) {
+          db[e] += d;
+          dw[K - 1][e] = fmaf(d, xv[i][e], dw[K - 1][e]);
+#pragma unroll
+          for (int j = 0; j < K - 1; ++j) dw[j][e] = fmaf(d, win[j][e], dw[j][e]);
+        }
+        // dxe[s] = w[0] dpre[t] + w[1] dpre[t - 1] + ...
+        float acc = wk[0][e] * d;
+#pragma unroll
+        for (int j = 1; j < K; ++j) acc = fmaf(wk[j][e], dwin[K - 1 - j][e], acc);
+        out[e] = acc;
+#pragma unroll
+        for (int j = 0; j + 1 < K - 1; ++j) {
+          win[j][e] = win[j + 1][e];
+          dwin[j][e] = dwin[j + 1][e];
+        }
+        if constexpr (K > 1) {
+          win[K - 2][e] = xv[i][e];
+          dwin[K - 2][e] = dpre[e];
+        }
+      }
+      const int s = t - (K - 1);
+      if (s < t0 && blockIdx.y != 0) continue;
+      // the final window's rows are the inputs s = T - (K - 1) .. T - 1
+      if (dstate_out && s >= T - (K - 1)) {
+        float g[kVec];
+        ld4(dstate_out + ((size_t)b * (K - 1) + (s - (T - (K - 1)))) * C + c, g);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) out[e] += g[e];
+      }
+      const float4 o4 = make_float4(out[0], out[1], out[2], out[3]);
+      if (s >= 0)
+        store4(dx + (row0 + s) * C + c, o4);
+      else if (dstate_in)
+        store4(dstate_in + ((size_t)b * (K - 1) + (K - 1) + s) * C + c, o4);
+    }
+  }
+  float* pr = part + ((size_t)b * gridDim.y + blockIdx.y) * (K + 1) * C + c;
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    store4(pr + (size_t)j * C, make_float4(dw[j][0], dw[j][1], dw[j][2], dw[j][3]));
+  store4(pr + (size_t)K * C, make_float4(db[0], db[1], db[2], db[3]));
+}
+
+template <typename Tin>
+cudaError_t bwd_dispatch(const ShortConvBwdArgs& a, int TT, int tiles, cudaStream_t st) {
+  const dim3 grid((a.C / kVec + kThreads - 1) / kThreads, tiles, a.B);
+#define GDN_CONV_BWD_CASE(KK)                                                                  \
+  case KK:                                                                                     \
+    short_conv_bwd_kernel<Tin, KK><<<grid, kThreads, 0, st>>>(                                 \
+        static_cast<const Tin*>(a.x), a.w, a.bias, static_cast<const Tin*>(a.state_in),        \
+        static_cast<const Tin*>(a.dy), static_cast<const Tin*>(a.dstate_out),                  \
+        static_cast<Tin*>(a.dx), static_cast<Tin*>(a.dstate_in), a.part, a.T, a.C, TT, a.act); \
+    break;
+  switch (a.K) {
+    GDN_CONV_BWD_CASE(1)
+    GDN_CONV_BWD_CASE(2)
+    GDN_CONV_BWD_CASE(3)
+    GDN_CONV_BWD_CASE(4)
+    GDN_CONV_BWD_CASE(5)
+    GDN_CONV_BWD_CASE(6)
+    GDN_CONV_BWD_CASE(7)
+    GDN_CONV_BWD_CASE(8)
+    default: return cudaErrorInvalidValue;
+  }
+#undef GDN_CONV_BWD_CASE
+  return cudaGetLastError();
+}
+
+// Token tiles: enough warps to keep loads in flight on every SM (24 a SM),
+// tiles of 32 to 512 tokens (a tile reads 2 (K - 1) rows more than it owns).
+int conv_bwd_tile(int B, int T, int C) {
+  const long long warps_per_row = (C + kVec * 32 - 1) / (kVec * 32);
+  const long long want = 24LL * 148;
+  long long tt = (long long)B * T * warps_per_row / want;
+  tt = (tt + 15) / 16 * 16;
+  if (tt < 32) tt = 32;
+  if (tt > 512) tt = 512;
+  if ((T + tt - 1) / tt > 65535) tt = ((long long)T + 65534) / 65535;
+  return (int)tt;
+}
+
+}  // namespace
+
+size_t short_conv_bwd_workspace_bytes(int B, int T, int C, int K) {
+  if (B <= 0 || T <= 0 || C <= 0) return 0;
+  const int TT = conv_bwd_tile(B, T, C);
+  return (size_t)B * ((T + TT - 1) / TT) * (K + 1) * C * sizeof(float);
+}
+
+cudaError_t launch_short_conv_bwd(const ShortConvBwdArgs& a, cudaStream_t st) {
+  if (!short_conv_supported(a.C, a.K, a.dtype) || a.B > 65535) return cudaErrorInvalidValue;
+  const int TT = conv_bwd_tile(a.B, a.T, a.C);
+  const int tiles = (a.T + TT - 1) / TT;
+  cudaError_t e = a.dtype == kBF16 ? bwd_dispatch<__nv_bfloat16>(a, TT, tiles, st)
+                                   : bwd_dispatch<float>(a, TT, tiles, st);
+  if (e != cudaSuccess) return e;
+  // dw rows 0 .. K - 1, dbias row K of every partial
+  const long long stride = (long long)(a.K + 1) * a.C;
+  e = launch_sum_partials(a.part, a.dw, (long long)a.B * tiles, stride, (long long)a.K * a.C, st);
+  if (e != cudaSuccess || !a.dbias) return e;
+  return launch_sum_partials(a.part + (size_t)a.K * a.C, a.dbias, (long long)a.B * tiles, stride,
+                             a.C, st);
+}
+
+// ---------------------------------------------------------------------------
+// out[i] = sum_p part[p * stride + i], p in a fixed order
+// ---------------------------------------------------------------------------
+
+namespace {
+
+constexpr int kSumCols = 32;   // columns of a block
+constexpr int kSumRows = 16;   // rows of threads, each over every 16th partial
+
+__global__ void __launch_bounds__(kSumCols * kSumRows)
+sum_partials_kernel(const float* __restrict__ part, float* __restrict__ out, long long parts,
+                    long long stride, long long n) {
+  __shared__ float red[kSumRows][kSumCols];
+  const int col = threadIdx.x % kSumCols, row = threadIdx.x / kSumCols;
+  const long long i = (long long)blockIdx.x * kSumCols + col;
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+  if (i < n) {
+    long long p = row;
+    for (; p + 3 * kSumRows < parts; p += 4 * kSumRows) {
+      s0 += part[p * stride + i];
+      s1 += part[(p + kSumRows) * stride + i];
+      s2 += part[(p + 2 * kSumRows) * stride + i];
+      s3 += part[(p + 3 * kSumRows) * stride + i];
+    }
+    for (; p < parts; p += kSumRows) s0 += part[p * stride + i];
+  }
+  red[row][col] = (s0 + s1) + (s2 + s3);
+  __syncthreads();
+  if (row == 0 && i < n) {
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < kSumRows; ++r) s += red[r][col];
+    out[i] = s;
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_sum_partials(const float* part, float* out, long long parts, long long stride,
+                                long long n, cudaStream_t st) {
+  if (n <= 0) return cudaSuccess;
+  const long long blocks = (n + kSumCols - 1) / kSumCols;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  sum_partials_kernel<<<(unsigned)blocks, kSumCols * kSumRows, 0, st>>>(part, out, parts, stride,
+                                                                        n);
+  return cudaGetLastError();
+}
+
+}  // namespace gdn

@@ -468,42 +468,127 @@ def _layer_impl(entry, q, k, v, a, b, A_log, dt_bias, gate, norm_weight, eps, in
     return y, hT
 
 
-def short_convolution(x, weight, *, activation: Optional[str] = "silu", conv_state=None,
-                      output_final_state: bool = False,
+_ACTIVATIONS = {"silu": 1, "swish": 1, None: 0}
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and 16-byte aligned, as the kernels read and write."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _float_vec(t, shape, name, dev):
+    """An optional fp32 parameter of the given shape on ``dev``."""
+    if t is None:
+        return None
+    t = torch.as_tensor(t, device=dev).to(torch.float32)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}; got {tuple(t.shape)}")
+    return _aligned(t)
+
+
+def _check_inputs(pairs, dev, dtype):
+    """CUDA tensors of one device and one dtype."""
+    for name, t in pairs:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, not on {dev}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype} like the other inputs; got {t.dtype}")
+
+
+def _cuda_input(name, t):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be bfloat16 or float32; got {t.dtype}")
+
+
+class _ShortConvFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, conv_state, act):
+        x = _aligned(x)
+        w32 = _aligned(w.to(torch.float32))
+        b32 = None if bias is None else _aligned(bias.to(torch.float32))
+        st = None if conv_state is None else _aligned(conv_state)
+        s_out = x.new_empty((x.shape[0], w.shape[0] - 1, x.shape[2]))
+        y = _short_conv_fwd(x, w32, b32, st, s_out, act)
+        ctx.act = act
+        ctx.w_dtype, ctx.b_dtype = w.dtype, None if bias is None else bias.dtype
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, w32, b32, st)
+        return y, s_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, ds):
+        x, w, bias, st = ctx.saved_tensors
+        B, T, C = x.shape
+        K = w.shape[0]
+        dy = torch.zeros_like(x) if dy is None else _aligned(dy)
+        ds = None if ds is None else _aligned(ds)
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        db = None if bias is None else torch.empty_like(bias)
+        dst = None if st is None else torch.empty_like(st)
+        lib = _lib.load()
+        with torch.cuda.device(x.device):
+            n = lib.gdn_short_conv_bwd_workspace_bytes(B, T, C, K)
+            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
+            rc = lib.gdn_short_conv_bwd(
+                _ptr(x), _ptr(w), _ptr(bias), _ptr(st), _ptr(dy), _ptr(ds), _ptr(dx), _ptr(dw),
+                _ptr(db), _ptr(dst), B, T, C, K, ctx.act, _DTYPES[x.dtype], _ptr(ws), n,
+                torch.cuda.current_stream(x.device).cuda_stream)
+        _lib.check(rc, "gdn_short_conv_bwd")
+        return (dx, dw.to(ctx.w_dtype), None if db is None else db.to(ctx.b_dtype), dst, None)
+
+
+def _short_conv_fwd(x, w, bias, s_in, s_out, act):
+    """gdn_short_conv_fwd_bias on checked, contiguous inputs; returns y."""
+    B, T, C = x.shape
+    y = torch.empty_like(x)
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        rc = lib.gdn_short_conv_fwd_bias(_ptr(x), _ptr(w), _ptr(bias), _ptr(s_in), _ptr(s_out),
+                                         _ptr(y), B, T, C, w.shape[0], act, _DTYPES[x.dtype],
+                                         torch.cuda.current_stream(x.device).cuda_stream)
+    _lib.check(rc, "gdn_short_conv_fwd")
+    return y
+
+
+def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu",
+                      conv_state=None, output_final_state: bool = False,
                       final_state_out: Optional[torch.Tensor] = None
                       ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """ShortConvolution (model.py:15-40) on the GPU (gdn_short_conv_fwd): a
-    causal depthwise convolution over time, kernel K, no bias, then SiLU for
+    causal depthwise convolution over time, kernel K, then SiLU for
     ``activation`` ``'silu'`` / ``'swish'`` (None: none).
 
     x ``[B,T,C]`` bfloat16 or float32 on a CUDA device; weight ``[K,C]`` or the
-    flax kernel ``[K,1,C]`` (float32).  ``conv_state`` ``[B,K-1,C]`` in x's
-    dtype replaces the zero padding before token 0 (the inputs a previous call
-    ended with).  Returns ``(y, state)``: state ``[B,K-1,C]`` holds the last
-    K - 1 inputs when ``output_final_state`` or ``final_state_out`` (which may
-    be ``conv_state``, updated in place) is given, else None.  The reference's
-    call is ``short_convolution(x, w)`` (no state).  Inference only.
+    flax kernel ``[K,1,C]``, bias ``[C]`` or None (taken to float32).  ``conv_state``
+    ``[B,K-1,C]`` in x's dtype replaces the zero padding before token 0 (the
+    inputs a previous call ended with).  Returns ``(y, state)``: state
+    ``[B,K-1,C]`` holds the last K - 1 inputs when ``output_final_state`` or
+    ``final_state_out`` (which may be ``conv_state``, updated in place) is
+    given, else None.  The reference's call is ``short_convolution(x, w)`` (no
+    state).  Differentiable in x, weight, bias and conv_state, through y and
+    the returned state (without ``final_state_out``; gdn_short_conv_bwd).
     """
-    if _wants_grad(x, conv_state):
-        raise NotImplementedError("the short convolution has no backward here")
-    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 3):
-        raise ValueError("x must be a [B,T,C] CUDA tensor")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"x must be bfloat16 or float32; got {x.dtype}")
+    _cuda_input("x", x)
+    if x.dim() != 3:
+        raise ValueError(f"x must be [B,T,C]; got {tuple(x.shape)}")
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be 'silu', 'swish' or None; got {activation!r}")
     B, T, C = x.shape
-    w = torch.as_tensor(weight, device=x.device).to(torch.float32)
+    w = torch.as_tensor(weight, device=x.device)
     if w.dim() == 3:
         w = w.reshape(w.shape[0], w.shape[-1])
     if w.dim() != 2 or w.shape[1] != C:
         raise ValueError(f"weight must be [K,{C}] or [K,1,{C}]; got {tuple(weight.shape)}")
     K = w.shape[0]
-    w = w.contiguous()
-    act = {"silu": 1, "swish": 1, None: 0}.get(activation)
-    if act is None:
-        raise ValueError(f"activation must be 'silu', 'swish' or None; got {activation!r}")
-    x = x.contiguous()
-    if x.data_ptr() % 16:
-        x = x.clone()
     shape = (B, K - 1, C)
 
     def state(t, name):
@@ -517,16 +602,233 @@ def short_convolution(x, weight, *, activation: Optional[str] = "silu", conv_sta
 
     s_in = state(conv_state, "conv_state")
     s_out = state(final_state_out, "final_state_out")
+    if bias is not None:
+        bias = torch.as_tensor(bias, device=x.device)
+        if tuple(bias.shape) != (C,):
+            raise ValueError(f"bias must be [{C}]; got {tuple(bias.shape)}")
+    if _wants_grad(x, w, bias, conv_state):
+        if final_state_out is not None:
+            raise NotImplementedError("the backward does not cover final_state_out")
+        y, s_out = _ShortConvFn.apply(x, w, bias, s_in, act)
+        return y, s_out if output_final_state else None
     if s_out is None and output_final_state:
         s_out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = _short_conv_fwd(_aligned(x), _aligned(w.to(torch.float32)),
+                        None if bias is None else _aligned(bias.to(torch.float32)), s_in, s_out,
+                        act)
+    return y, s_out
+
+
+def _glu_fwd(x, wg, wu, keep):
+    """gdn_glu_fwd on x [M,D], wg, wu [I,D]; returns h [M,I] and, with ``keep``,
+    the two projections."""
+    (M, D), I = x.shape, wg.shape[0]
+    h = x.new_empty((M, I))
+    g, u = (x.new_empty((M, I)), x.new_empty((M, I))) if keep else (None, None)
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        rc = lib.gdn_glu_fwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(h), _ptr(g), _ptr(u), M, D, I,
+                             _DTYPES[x.dtype], torch.cuda.current_stream(x.device).cuda_stream)
+    _lib.check(rc, "gdn_glu_fwd")
+    return h, g, u
+
+
+class _GluFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu):
+        x, wg, wu = _aligned(x), _aligned(wg), _aligned(wu)
+        h, g, u = _glu_fwd(x, wg, wu, True)
+        ctx.save_for_backward(x, wg, wu, g, u)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, wg, wu, g, u = ctx.saved_tensors
+        (M, D), I = x.shape, wg.shape[0]
+        need_x, need_w = ctx.needs_input_grad[0], any(ctx.needs_input_grad[1:])
+        dh = _aligned(dh)
+        dx = torch.empty_like(x) if need_x else None
+        dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_w else (None, None)
+        lib = _lib.load()
+        with torch.cuda.device(x.device):
+            n = lib.gdn_glu_bwd_workspace_bytes(M, I, _DTYPES[x.dtype])
+            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
+            rc = lib.gdn_glu_bwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(g), _ptr(u), _ptr(dh),
+                                 _ptr(dx), _ptr(dwg), _ptr(dwu), M, D, I, _DTYPES[x.dtype],
+                                 _ptr(ws), n, torch.cuda.current_stream(x.device).cuda_stream)
+        _lib.check(rc, "gdn_glu_bwd")
+        return dx, dwg, dwu
+
+
+def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") -> torch.Tensor:
+    """The gated linear unit of the feed-forward block (GatedDeltaNetMLP,
+    model.py:162-180, before its down projection) as one kernel (gdn_glu_fwd):
+    ``silu(x @ gate_weight.T) * (x @ up_weight.T)``.
+
+    x ``[...,D]``, gate_weight and up_weight ``[I,D]`` (torch's Linear layout)
+    in one dtype, bfloat16 or float32, on a CUDA device; returns ``[...,I]``.
+    ``activation``: ``'silu'`` / ``'swish'``.  Differentiable in all three
+    (gdn_glu_bwd, from the two projections kept in x's dtype).
+    """
+    _cuda_input("x", x)
+    if activation not in ("silu", "swish"):
+        raise ValueError(f"activation must be 'silu' or 'swish'; got {activation!r}")
+    if x.dim() < 1:
+        raise ValueError("x must be [...,D]")
+    D = x.shape[-1]
+    _check_inputs((("gate_weight", gate_weight), ("up_weight", up_weight)), x.device, x.dtype)
+    if gate_weight.dim() != 2 or gate_weight.shape[1] != D or up_weight.shape != gate_weight.shape:
+        raise ValueError(f"gate_weight and up_weight must both be [I,{D}]; got "
+                         f"{tuple(gate_weight.shape)}, {tuple(up_weight.shape)}")
+    M = x.numel() // D if D else x.shape[:-1].numel()
+    x2 = x.reshape(M, D)
+    if _wants_grad(x, gate_weight, up_weight):
+        h = _GluFn.apply(x2, gate_weight, up_weight)
+    else:
+        h, _, _ = _glu_fwd(_aligned(x2), _aligned(gate_weight), _aligned(up_weight), False)
+    return h.reshape(*x.shape[:-1], gate_weight.shape[0])
+
+
+def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, keep):
+    """gdn_selective_scan_fwd on checked, contiguous inputs; returns y and, with
+    ``keep``, the checkpoints of the backward."""
+    b, T, ch = x.shape
+    G, N = B.shape[2], A.shape[1]
     y = torch.empty_like(x)
     lib = _lib.load()
     with torch.cuda.device(x.device):
-        rc = lib.gdn_short_conv_fwd(_ptr(x), _ptr(w), _ptr(s_in), _ptr(s_out), _ptr(y), B, T, C,
-                                    K, act, _DTYPES[x.dtype],
-                                    torch.cuda.current_stream(x.device).cuda_stream)
-    _lib.check(rc, "gdn_short_conv_fwd")
-    return y, s_out
+        ck = None
+        if keep:
+            n = lib.gdn_selective_scan_checkpoint_bytes(b, T, ch, N)
+            ck = torch.empty(max(n // 4, 4), dtype=torch.float32, device=x.device)
+        rc = lib.gdn_selective_scan_fwd(
+            _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
+            _ptr(h0), _ptr(y), _ptr(hT), _ptr(ck), b, T, ch, N, G, softplus, _DTYPES[x.dtype],
+            torch.cuda.current_stream(x.device).cuda_stream)
+    _lib.check(rc, "gdn_selective_scan_fwd")
+    return y, ck
+
+
+class _SelectiveScanFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, h0, softplus):
+        f32 = lambda t: None if t is None else _aligned(t.to(torch.float32))  # noqa: E731
+        x, dt, B, C = _aligned(x), _aligned(dt), _aligned(B), _aligned(C)
+        z = None if z is None else _aligned(z)
+        ctx.dtypes = [None if t is None else t.dtype for t in (A, D, dt_bias, h0)]
+        A, D, dt_bias, h0 = f32(A), f32(D), f32(dt_bias), f32(h0)
+        hT = torch.empty((x.shape[0], x.shape[2], A.shape[1]), dtype=torch.float32,
+                         device=x.device)
+        y, ck = _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, True)
+        ctx.softplus, ctx.has_h0 = softplus, h0 is not None
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, ck)
+        return y, hT
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dhT):
+        x, dt, A, B, C, D, z, dt_bias, ck = ctx.saved_tensors
+        b, T, ch = x.shape
+        G, N = B.shape[2], A.shape[1]
+        dev = x.device
+        dy = torch.zeros_like(x) if dy is None else _aligned(dy)
+        dhT = None if dhT is None else _aligned(dhT.to(torch.float32))
+        like = lambda t: None if t is None else torch.empty_like(t)  # noqa: E731
+        dx, ddt, dA, dB, dC = like(x), like(dt), like(A), like(B), like(C)
+        dD, dz, dbias = like(D), like(z), like(dt_bias)
+        dh0 = torch.empty((b, ch, N), dtype=torch.float32, device=dev) if ctx.has_h0 else None
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            n = lib.gdn_selective_scan_bwd_workspace_bytes(b, T, ch, N, G)
+            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+            rc = lib.gdn_selective_scan_bwd(
+                _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
+                _ptr(ck), _ptr(dy), _ptr(dhT), _ptr(dx), _ptr(ddt), _ptr(dA), _ptr(dB), _ptr(dC),
+                _ptr(dD), _ptr(dz), _ptr(dbias), _ptr(dh0), b, T, ch, N, G, ctx.softplus,
+                _DTYPES[x.dtype], _ptr(ws), n, torch.cuda.current_stream(dev).cuda_stream)
+        _lib.check(rc, "gdn_selective_scan_bwd")
+        to = lambda t, d: None if t is None else t.to(d)  # noqa: E731
+        Ad, Dd, bd, hd = ctx.dtypes
+        return (dx, ddt, to(dA, Ad), dB, dC, to(dD, Dd), dz, to(dbias, bd), to(dh0, hd), None)
+
+
+def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus: bool = True,
+                   initial_state=None, output_final_state: bool = False,
+                   final_state_out: Optional[torch.Tensor] = None
+                   ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Selective state-space scan (gdn_selective_scan_fwd), for prompts, training
+    and single tokens.  Per row, channel c and token t, with an fp32 state h of
+    N values::
+
+        delta = softplus(dt + dt_bias[c])          # dt + dt_bias[c] without dt_softplus
+        h     = exp(delta * A[c]) * h + delta * x * B[t]
+        y     = (sum(C[t] * h) + D[c] * x) * silu(z)
+
+    x, dt, z ``[B,T,Ch]`` and B, C ``[B,T,N]`` or ``[B,T,G,N]`` (channel c uses
+    group ``c // (Ch // G)``) in one dtype, bfloat16 or float32, on a CUDA
+    device; A ``[Ch,N]`` (negative in practice), D and dt_bias ``[Ch]`` (taken
+    to float32; None: zero; z None: no gate); N up to 64.  Returns ``(y,
+    state)`` like the recurrent op: state float32 ``[B,Ch,N]`` when
+    ``output_final_state`` or ``final_state_out`` is given (decode:
+    ``initial_state=S, final_state_out=S`` updates S in place), else None.
+    Differentiable in every tensor, through y and the returned state (without
+    ``final_state_out``; gdn_selective_scan_bwd).  Its layer feeds x through
+    :func:`short_convolution` first.
+    """
+    _cuda_input("x", x)
+    if x.dim() != 3:
+        raise ValueError(f"x must be [B,T,Ch]; got {tuple(x.shape)}")
+    dev = x.device
+    _check_inputs((("dt", dt), ("B", B), ("C", C)) + ((("z", z),) if z is not None else ()), dev,
+                  x.dtype)
+    b, T, ch = x.shape
+    if dt.shape != x.shape or (z is not None and z.shape != x.shape):
+        raise ValueError(f"dt and z must have x's shape {tuple(x.shape)}")
+    A = torch.as_tensor(A, device=dev)
+    if A.dim() != 2 or A.shape[0] != ch:
+        raise ValueError(f"A must be [{ch},N]; got {tuple(A.shape)}")
+    N = A.shape[1]
+    if B.dim() == 3:
+        B = B.unsqueeze(2)
+    if C.dim() == 3:
+        C = C.unsqueeze(2)
+    if B.dim() != 4 or tuple(B.shape[:2]) != (b, T) or B.shape[3] != N or C.shape != B.shape:
+        raise ValueError(f"B and C must be [{b},{T},{N}] or [{b},{T},G,{N}]; got "
+                         f"{tuple(B.shape)}, {tuple(C.shape)}")
+    G = B.shape[2]
+    if G < 1 or ch % G:
+        raise ValueError(f"x's {ch} channels must be a multiple of the {G} groups of B and C")
+    for name, t in (("D", D), ("dt_bias", dt_bias)):
+        if t is not None and tuple(t.shape) != (ch,):
+            raise ValueError(f"{name} must be [{ch}]; got {tuple(t.shape)}")
+    D = None if D is None else torch.as_tensor(D, device=dev)
+    dt_bias = None if dt_bias is None else torch.as_tensor(dt_bias, device=dev)
+    shape = (b, ch, N)
+    if initial_state is not None and (tuple(initial_state.shape) != shape
+                                      or initial_state.device != dev):
+        raise ValueError(f"initial_state must be {shape} on {dev}")
+    softplus = int(bool(dt_softplus))
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
+        if final_state_out is not None:
+            raise NotImplementedError("the backward does not cover final_state_out")
+        y, hT = _SelectiveScanFn.apply(x, dt, A, B, C, D, z, dt_bias, initial_state, softplus)
+        return y, hT if output_final_state else None
+    hT = final_state_out
+    if hT is not None:
+        if (tuple(hT.shape) != shape or hT.dtype != torch.float32 or not hT.is_contiguous()
+                or hT.device != dev or hT.data_ptr() % 16):
+            raise ValueError(f"final_state_out must be a contiguous, 16-byte aligned float32 "
+                             f"{shape} tensor on {dev}")
+    elif output_final_state:
+        hT = torch.empty(shape, dtype=torch.float32, device=dev)
+    h0 = None if initial_state is None else _aligned(initial_state.to(torch.float32))
+    y, _ = _scan_fwd(_aligned(x), _aligned(dt), _float_vec(A, (ch, N), "A", dev), _aligned(B),
+                     _aligned(C), _float_vec(D, (ch,), "D", dev),
+                     None if z is None else _aligned(z), _float_vec(dt_bias, (ch,), "dt_bias", dev),
+                     softplus, h0, hT, False)
+    return y, hT
 
 
 def gated_rms_norm(o, gate=None, weight=None, eps: float = 1e-5, *,
@@ -573,4 +875,6 @@ __all__ = [
     "gated_delta_rule_chunk_layer",
     "short_convolution",
     "gated_rms_norm",
+    "gated_linear_unit",
+    "selective_scan",
 ]

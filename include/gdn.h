@@ -385,6 +385,89 @@ int gdn_short_conv_fwd(const void* x, const float* weight, const void* state_in,
 int gdn_gated_rmsnorm_fwd(const void* o, const void* gate, const float* weight, float eps,
                           void* y, long long rows, int dv, int dtype, void* stream);
 
+/*
+ * gdn_short_conv_fwd with a bias [C] fp32 (NULL: none) added before the
+ * activation (nnx.Conv's use_bias, model.py:24-31).  gdn_short_conv_fwd is the
+ * call without one.
+ */
+int gdn_short_conv_fwd_bias(const void* x, const float* weight, const float* bias,
+                            const void* state_in, void* state_out, void* y, int B, int T, int C,
+                            int K, int activation, int dtype, void* stream);
+
+/*
+ * Gradients of gdn_short_conv_fwd_bias (the reference differentiates its
+ * convolution with JAX).  dy [B, T, C] and dstate_out [B, K - 1, C] (NULL:
+ * zero) are the gradients of y and of the final state, in x's dtype.  Written:
+ * dx [B, T, C] and dstate_in [B, K - 1, C] (NULL: not wanted) in x's dtype,
+ * dweight [K, C] and dbias [C] (NULL: not wanted) in fp32.  dx may not be x or
+ * dy.  `workspace`: gdn_short_conv_bwd_workspace_bytes() bytes.  The sums over
+ * tokens run in a fixed order.
+ */
+size_t gdn_short_conv_bwd_workspace_bytes(int B, int T, int C, int K);
+int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
+                       const void* state_in, const void* dy, const void* dstate_out, void* dx,
+                       float* dweight, float* dbias, void* dstate_in, int B, int T, int C, int K,
+                       int activation, int dtype, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * The gated linear unit of the feed-forward block (GatedDeltaNetMLP,
+ * model.py:162-180, before its down projection):
+ *   h = silu(x w_gate^T) * (x w_up^T),
+ * x [M, D], w_gate, w_up [I, D] (torch's [out, in]; the flax kernels
+ * transposed), h [M, I], all bf16 or all fp32, products summed in fp32.  g and
+ * u [M, I] (both or neither) receive the two projections for the backward, in
+ * the same dtype.
+ */
+int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, void* g, void* u,
+                int M, int D, int I, int dtype, void* stream);
+
+/*
+ * Its gradients from dh [M, I] and the forward's g and u: dx [M, D] (NULL: not
+ * wanted), dw_gate and dw_up [I, D] (both or neither), in the inputs' dtype.
+ * `workspace`: gdn_glu_bwd_workspace_bytes() bytes (the gradients of g and u,
+ * in the inputs' dtype).
+ */
+size_t gdn_glu_bwd_workspace_bytes(int M, int I, int dtype);
+int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void* g, const void* u,
+                const void* dh, void* dx, void* dw_gate, void* dw_up, int M, int D, int I,
+                int dtype, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Selective state-space scan (no counterpart in the reference).  Per row b,
+ * channel c and token t, with an fp32 state h [N]:
+ *   delta = softplus(dt + dt_bias[c])   (softplus = 0: dt + dt_bias[c])
+ *   h[n] <- exp(delta A[c, n]) h[n] + delta x B[b, t, grp, n]
+ *   y     = (sum_n C[b, t, grp, n] h[n] + D[c] x) silu(z)
+ * x, dt, z, y [B, T, C] and Bm, Cm [B, T, G, N] in `dtype` (z NULL: no gate);
+ * channel c uses group c / (C / G).  A [C, N], D, dt_bias [C] fp32 (D, dt_bias
+ * NULL: zero).  h0, hT [B, C, N] fp32: NULL h0 starts from zeros, NULL hT drops
+ * the final state, h0 == hT updates in place (decode: T = 1).  N <= 64.
+ * `checkpoints` (NULL: not wanted; gdn_selective_scan_checkpoint_bytes())
+ * receives the states that gdn_selective_scan_bwd restarts from.
+ */
+size_t gdn_selective_scan_checkpoint_bytes(int B, int T, int C, int N);
+int gdn_selective_scan_fwd(const void* x, const void* dt, const float* A, const void* Bm,
+                           const void* Cm, const float* D, const void* z, const float* dt_bias,
+                           const float* h0, void* y, float* hT, float* checkpoints, int B, int T,
+                           int C, int N, int G, int softplus, int dtype, void* stream);
+
+/*
+ * Its gradients from dy [B, T, C] (dtype) and dhT [B, C, N] (fp32, NULL: zero):
+ * dx, ddt, dz [B, T, C] and dB, dC [B, T, G, N] in `dtype`; dA [C, N], dD,
+ * ddt_bias [C] and dh0 [B, C, N] (NULL: not wanted) in fp32.  dD, dz and
+ * ddt_bias are given exactly when D, z and dt_bias are.  `checkpoints`: as the
+ * forward wrote them.  `workspace`: gdn_selective_scan_bwd_workspace_bytes()
+ * bytes.  All sums run in a fixed order.
+ */
+size_t gdn_selective_scan_bwd_workspace_bytes(int B, int T, int C, int N, int G);
+int gdn_selective_scan_bwd(const void* x, const void* dt, const float* A, const void* Bm,
+                           const void* Cm, const float* D, const void* z, const float* dt_bias,
+                           const float* checkpoints, const void* dy, const float* dhT, void* dx,
+                           void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz,
+                           float* ddt_bias, float* dh0, int B, int T, int C, int N, int G,
+                           int softplus, int dtype, void* workspace, size_t ws_bytes,
+                           void* stream);
+
 /* ABI version of this header: (major << 16) | minor (1.3: _gva, _varlen, backward;
  * 1.4: backward of packed sequences, the allocation-free backward;
  * 1.5: the layer form of the decode step; 1.6: the layer form of the chunked
@@ -394,7 +477,9 @@ int gdn_gated_rmsnorm_fwd(const void* o, const void* gate, const float* weight, 
  * gdn_fold_states,
  * gdn_reload_kernel_overrides, gdn_binary_version; 1.9: the layer forms at
  * the other tensor-core shapes and the general recurrent shapes,
- * gdn_short_conv_fwd, gdn_gated_rmsnorm_fwd; 1.10: gdn_chunk_bwd_workspace_bytes_for). */
+ * gdn_short_conv_fwd, gdn_gated_rmsnorm_fwd; 1.10: gdn_chunk_bwd_workspace_bytes_for;
+ * 1.11: the gated linear unit, the selective scan, the short convolution's bias
+ * and gradients). */
 int gdn_abi_version(void);
 
 /*
