@@ -761,7 +761,8 @@ int gdn_device_error(int clear) {
   const int c = gdn::device_error_chunk_scan(clear != 0);
   const int d = gdn::device_error_bwd_prep(clear != 0);
   const int e = gdn::device_error_bwd_grads(clear != 0);
-  return a ? a : (b ? b : (c ? c : (d ? d : e)));
+  const int f = gdn::device_error_glu_tc(clear != 0);
+  return a ? a : (b ? b : (c ? c : (d ? d : (e ? e : f))));
 }
 
 int gdn_abi_version(void) { return (1 << 16) | 11; }

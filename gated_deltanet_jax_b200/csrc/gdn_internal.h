@@ -343,6 +343,12 @@ struct GluBwdArgs {
   int M, D, I, dtype;
 };
 cudaError_t launch_glu_bwd(const GluBwdArgs& a, cudaStream_t st);
+// Their products on tcgen05 (glu_tc.cu): bf16, D and I multiples of 8 (a row's
+// bytes a multiple of 16, as TMA needs).  The backward's reads dg and du.
+bool glu_tc_supported(int M, int D, int I, int dtype);
+cudaError_t launch_glu_tc_fwd(const GluArgs& a, cudaStream_t st);
+cudaError_t launch_glu_tc_bwd(const GluBwdArgs& a, cudaStream_t st);
+int device_error_glu_tc(bool clear);
 
 // Selective state-space scan (selective_scan.cu): x, dt, z, y [B,T,C], B, C
 // [B,T,G,N] in one dtype (z NULL: no gate); A [C,N], D, dt_bias [C] fp32 (D,

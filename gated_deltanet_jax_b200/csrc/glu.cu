@@ -258,6 +258,7 @@ cudaError_t bwd_products_simt(const GluBwdArgs& a, cudaStream_t st) {
 
 cudaError_t launch_glu_fwd(const GluArgs& a, cudaStream_t st) {
   if (a.M == 0 || a.I == 0) return cudaSuccess;
+  if (glu_tc_supported(a.M, a.D, a.I, a.dtype)) return launch_glu_tc_fwd(a, st);
   return a.dtype == kBF16 ? fwd_simt<__nv_bfloat16>(a, st) : fwd_simt<float>(a, st);
 }
 
@@ -268,6 +269,7 @@ cudaError_t launch_glu_bwd(const GluBwdArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
   }
   if (a.D == 0) return cudaSuccess;
+  if (glu_tc_supported(a.M, a.D, a.I, a.dtype)) return launch_glu_tc_bwd(a, st);
   return a.dtype == kBF16 ? bwd_products_simt<__nv_bfloat16>(a, st)
                           : bwd_products_simt<float>(a, st);
 }
