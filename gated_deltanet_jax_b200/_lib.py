@@ -57,6 +57,7 @@ EXPORTED_SYMBOLS = (
     "gdn_selective_scan_fwd",
     "gdn_selective_scan_bwd",
     "gdn_selective_scan_checkpoint_bytes",
+    "gdn_selective_scan_workspace_bytes",
     "gdn_selective_scan_bwd_workspace_bytes",
     "gdn_last_error",
     "gdn_reload_kernel_overrides",
@@ -144,8 +145,10 @@ def _declare(lib):
     lib.gdn_glu_bwd.restype = _i
     lib.gdn_glu_bwd_workspace_bytes.argtypes = [_i] * 3
     lib.gdn_glu_bwd_workspace_bytes.restype = _sz
-    lib.gdn_selective_scan_fwd.argtypes = [_vp] * 12 + [_i] * 7 + [_vp]
+    lib.gdn_selective_scan_fwd.argtypes = [_vp] * 12 + [_i] * 7 + [_vp, _sz, _vp]
     lib.gdn_selective_scan_fwd.restype = _i
+    lib.gdn_selective_scan_workspace_bytes.argtypes = [_i] * 5
+    lib.gdn_selective_scan_workspace_bytes.restype = _sz
     lib.gdn_selective_scan_bwd.argtypes = [_vp] * 20 + [_i] * 7 + [_vp, _sz, _vp]
     lib.gdn_selective_scan_bwd.restype = _i
     lib.gdn_selective_scan_checkpoint_bytes.argtypes = [_i] * 4

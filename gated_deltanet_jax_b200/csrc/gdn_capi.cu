@@ -884,10 +884,16 @@ size_t gdn_selective_scan_checkpoint_bytes(int B, int T, int C, int N) {
   return gdn::scan_checkpoint_bytes(B, T, C, N);
 }
 
+size_t gdn_selective_scan_workspace_bytes(int B, int T, int C, int N, int G) {
+  if (B <= 0 || T <= 0 || C <= 0 || N <= 0 || N > gdn::kScanMaxStates || G <= 0 || C % G) return 0;
+  return gdn::selective_scan_workspace_bytes(B, T, C, N, G);
+}
+
 int gdn_selective_scan_fwd(const void* x, const void* dt, const float* A, const void* Bm,
                            const void* Cm, const float* D, const void* z, const float* dt_bias,
                            const float* h0, void* y, float* hT, float* checkpoints, int B, int T,
-                           int C, int N, int G, int softplus, int dtype, void* stream) {
+                           int C, int N, int G, int softplus, int dtype, void* workspace,
+                           size_t ws_bytes, void* stream) {
   int rc = check_scan(x, dt, A, Bm, Cm, D, z, dt_bias, h0, B, T, C, N, G, softplus, dtype);
   if (rc || B == 0 || C == 0) return rc;
   if ((T > 0 && !y) || !aligned16(y) || !aligned16(hT) || !aligned16(checkpoints))
@@ -898,9 +904,14 @@ int gdn_selective_scan_fwd(const void* x, const void* dt, const float* A, const 
                  "gdn_selective_scan_fwd (T=0 state copy)");
   }
   gdn::ScanArgs a = scan_args(x, dt, A, Bm, Cm, D, z, dt_bias, h0, B, T, C, N, G, softplus, dtype);
+  rc = check_workspace(workspace, ws_bytes, gdn::selective_scan_workspace_bytes(B, T, C, N, G),
+                       "gdn_selective_scan_workspace_bytes");
+  if (rc) return rc;
   a.y = y;
   a.hT = hT;
   a.ckpt = checkpoints;
+  gdn::scan_split_workspace(a, static_cast<float*>(workspace),
+                            gdn::scan_split(B, T, C, G, false));
   return cuda_status(gdn::launch_selective_scan(a, (cudaStream_t)stream),
                      "gdn_selective_scan_fwd");
 }

@@ -369,8 +369,21 @@ struct ScanArgs {
   void* y;
   float* hT;
   float* ckpt;
+  // Rows cut into chunks (scan_split): [chunks][B][C][scan_padded_states(N)] and
+  // [chunks][B][C] of scratch, set by scan_split_workspace.
+  float* chunk_state;
+  float* chunk_sum;
   int B, T, C, N, G, softplus, dtype, nck;
 };
+struct ScanSplit {
+  int chunks, tokens;
+};
+ScanSplit scan_split(int B, int T, int C, int G, bool backward);
+size_t scan_split_bytes(int B, int C, int N, const ScanSplit& s);
+void scan_split_workspace(ScanArgs& a, float* ws, const ScanSplit& s);
+cudaError_t launch_scan_chain(const ScanArgs& a, const float* first, int chunks, bool reverse,
+                              cudaStream_t st);
+size_t selective_scan_workspace_bytes(int B, int T, int C, int N, int G);
 int scan_padded_states(int N);
 int scan_checkpoint_tokens(int N);
 size_t scan_checkpoint_bytes(int B, int T, int C, int N);

@@ -8,9 +8,9 @@
 //   gated_norm_kernel   FusedRMSNormGated (model.py:41-53) over the op's output:
 //                       y = o rsqrt(mean(o^2) + eps) w silu(gate), in place.
 //
-// Both are HBM-bound: each element is read once and written once.  A thread
-// owns one 16-byte vector of channels (8 bf16 or 4 fp32), so a warp moves 512
-// contiguous bytes per access.
+// Both are HBM-bound: each element is read once and written once.  A thread of
+// the norm owns 16-byte vectors (8 bf16 or 4 fp32), one of the convolution four
+// channels.
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 
@@ -55,7 +55,23 @@ struct Vec16<float> {
 
 __device__ __forceinline__ float silu_acc(float x) { return x / (1.f + expf(-x)); }
 
+// Four consecutive channels (8 bytes of bf16, 16 of fp32): with eight of bf16 the
+// windows and weights of K = 4 take 139 registers, and too few warps fit an SM
+// to cover the loads (142 us at 8 x 2048 x 4096).
+template <typename Tin>
+struct Vec4 {
+  static constexpr int N = 4;
+  __device__ static void load(const Tin* p, float (&f)[N]) {
+    const float4 q = load4(p);
+    f[0] = q.x; f[1] = q.y; f[2] = q.z; f[3] = q.w;
+  }
+  __device__ static void store(Tin* p, const float (&f)[N]) {
+    store4(p, make_float4(f[0], f[1], f[2], f[3]));
+  }
+};
+
 constexpr int kConvThreads = 128;
+constexpr int kConvAhead = 4;
 
 // x, y [B, T, C]; w [K, C] fp32 (the flax kernel (K, 1, C) as stored); bias [C]
 // fp32 or NULL;
@@ -68,7 +84,7 @@ __global__ void __launch_bounds__(kConvThreads)
 short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
                   const float* __restrict__ bias, const Tin* state_in, Tin* state_out, Tin* __restrict__ y, int T, int C,
                   int TT, int act) {
-  using V = Vec16<Tin>;
+  using V = Vec4<Tin>;
   constexpr int N = V::N;
   const int c = (blockIdx.x * kConvThreads + threadIdx.x) * N;
   if (c >= C) return;
@@ -101,25 +117,33 @@ short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
       for (int e = 0; e < N; ++e) win[j][e] = 0.f;
     }
   }
-  for (int t = t0; t < t1; ++t) {
-    float cur[N], out[N];
-    V::load(xb + (size_t)t * C, cur);
+  for (int tb = t0; tb < t1; tb += kConvAhead) {
+    float cur[kConvAhead][N];   // loads of several tokens in flight together
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      float acc = wk[K - 1][e] * cur[e];
+    for (int i = 0; i < kConvAhead; ++i)
+      if (tb + i < t1) V::load(xb + (size_t)(tb + i) * C, cur[i]);
 #pragma unroll
-      for (int j = 0; j < K - 1; ++j) acc = fmaf(wk[j][e], win[j][e], acc);
-      if (bias) acc += bs[e];
-      out[e] = act ? silu_acc(acc) : acc;
-    }
-    V::store(y + ((size_t)b * T + t) * C + c, out);
+    for (int i = 0; i < kConvAhead; ++i) {
+      const int t = tb + i;
+      if (t >= t1) break;
+      float out[N];
 #pragma unroll
-    for (int j = 0; j + 1 < K - 1; ++j)
+      for (int e = 0; e < N; ++e) {
+        float acc = wk[K - 1][e] * cur[i][e];
 #pragma unroll
-      for (int e = 0; e < N; ++e) win[j][e] = win[j + 1][e];
-    if constexpr (K > 1) {
+        for (int j = 0; j < K - 1; ++j) acc = fmaf(wk[j][e], win[j][e], acc);
+        if (bias) acc += bs[e];
+        out[e] = act ? silu_acc(acc) : acc;
+      }
+      V::store(y + ((size_t)b * T + t) * C + c, out);
 #pragma unroll
-      for (int e = 0; e < N; ++e) win[K - 2][e] = cur[e];
+      for (int j = 0; j + 1 < K - 1; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) win[j][e] = win[j + 1][e];
+      if constexpr (K > 1) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) win[K - 2][e] = cur[i][e];
+      }
     }
   }
   if (state_out && blockIdx.z == gridDim.z - 1) {
@@ -177,7 +201,7 @@ gated_norm_kernel(const Tin* o, const Tin* __restrict__ gate, const float* __res
 template <typename Tin>
 cudaError_t conv_dispatch(const void* x, const float* w, const float* bias, const void* si,
                           void* so, void* y, int B, int T, int C, int K, int TT, int act, cudaStream_t st) {
-  constexpr int N = Vec16<Tin>::N;
+  constexpr int N = Vec4<Tin>::N;
   const dim3 grid((C / N + kConvThreads - 1) / kConvThreads, B, (T + TT - 1) / TT);
   const Tin* xi = static_cast<const Tin*>(x);
   const Tin* s_in = static_cast<const Tin*>(si);
@@ -215,9 +239,12 @@ cudaError_t launch_short_conv(const void* x, const float* w, const float* bias,
                               int dtype, cudaStream_t st) {
   if (B == 0 || T == 0) return cudaSuccess;
   if (!short_conv_supported(C, K, dtype) || B > 65535) return cudaErrorInvalidValue;
-  // Token tiles of 64; a state updated in place is read by the first tile and
-  // written by the last, so it takes one tile over all T.
+  // Token tiles of 64, shorter ones (down to 16) where 64 leave SMs with fewer
+  // than eight blocks: a tile is a serial walk.  A state updated in place is read
+  // by the first tile and written by the last, so it takes one tile over all T.
   int TT = 64;
+  const long long per = (long long)((C / 4 + kConvThreads - 1) / kConvThreads) * B;
+  while (TT > 16 && per * ((T + TT - 1) / TT) < 8LL * device_sm_count()) TT /= 2;
   if (state_in && state_in == state_out) TT = T;
   if ((T + TT - 1) / TT > 65535) TT = (T + 65534) / 65535;
   return dtype == kBF16

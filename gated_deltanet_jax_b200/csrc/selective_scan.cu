@@ -7,14 +7,21 @@
 //
 // What it has to move is x, dt, z and y once (8 bytes a token and channel in
 // bf16); what it has to compute is one exponential and four multiply-adds per
-// state, which at N = 16 takes longer than the bytes.  Four lanes share a
-// channel, each with a quarter of its states in registers, so the exponentials
-// of a token run side by side and few sequences still fill the SMs.  A block
-// owns 32 channels of one row and walks tiles of 32 tokens: every thread forms
-// delta and delta x of eight (token, channel) pairs into shared memory with the
-// next tile's loads in flight, all lanes then run the recurrence over the tile,
-// and four tokens' read-outs at a time are summed over the four lanes in three
-// shuffles.
+// state, which at N = 16 takes longer than the bytes (16 exponentials a clock
+// and SM: 0.24 ms for 8 x 2048 x 4096 against 0.08 ms for its bytes).  Four lanes
+// share a channel, each with a quarter of its states in registers as pairs (two
+// multiply-adds an instruction).  A block owns 32 channels of one row and walks
+// tiles of 32 tokens: every thread forms delta and delta x of eight (token,
+// channel) pairs into shared memory with the next tile's loads in flight, all
+// lanes then run the recurrence over the tile, and four tokens' read-outs at a
+// time are summed over the four lanes in three shuffles.
+//
+// Few rows and a long axis: the recurrence is linear, so a row is cut into
+// chunks.  A first pass runs each from a zero state (no read-out) and keeps its
+// end and the sum of its steps; since the decay over a chunk is exp(A sum delta),
+// a second kernel chains the chunks' entering states, and the main pass starts
+// every chunk from its own.  The exponentials are computed twice, so only rows
+// that leave most SMs idle are cut.
 #include "selective_scan_common.cuh"
 
 namespace gdn {
@@ -24,14 +31,19 @@ namespace {
 constexpr int kTT = 32;   // tokens of a tile
 constexpr int kRows = kTT * kScanCh / (kScanThreads * 4);   // staging rows per thread
 
-template <typename T, int NL>
-__global__ void __launch_bounds__(kScanThreads)
-scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec) {
+// kLocal: the first pass of a cut row (from zero; the end state and the steps'
+// sum out, no y).  chunk / nchunk: tokens of a chunk and their number (grid z).
+template <typename T, int NL, bool kLocal>
+__global__ void __launch_bounds__(kScanThreads, NL > 8 ? 2 : NL > 4 ? 4 : sizeof(T) == 2 ? 7 : 6)
+scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int nchunk) {
   constexpr int NP = NL * kScanLanes;
+  constexpr int P = scan_pairs<NL>();
   constexpr int CK = scan_tile<NL>();
-  __shared__ float2 sDU[kTT][kScanCh];
-  __shared__ float sY[kTT][kScanCh + 8];   // padded: four tokens of eight channels at once
-  __shared__ __align__(16) float sB[kTT][NP], sC[kTT][NP];
+  constexpr int BV = kTT * NL;                                      // vectors of B in a tile
+  constexpr int BPT = (BV + kScanThreads - 1) / kScanThreads;       // per thread
+  __shared__ __align__(16) float4 sDU[kTT][kScanCh];   // delta twice, delta x twice
+  __shared__ float sY[kLocal ? 1 : kTT][kScanCh + 8];  // padded: four tokens of eight channels
+  __shared__ __align__(16) float sB[kTT][NP], sC[kLocal ? 1 : kTT][NP];
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int Cg = a.C / a.G;
@@ -39,110 +51,177 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec) {
   const int cl0 = (blockIdx.x % tiles_per_group) * kScanCh;   // first channel in the group
   const int nch = min(kScanCh, Cg - cl0);
   const int c0 = grp * Cg + cl0;
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, kc = blockIdx.z;
+  const int tbeg = kc * chunk, tend = min(a.T, tbeg + chunk);
   const T* x = static_cast<const T*>(a.x);
   const T* dt = static_cast<const T*>(a.dt);
-  const T* z = static_cast<const T*>(a.z);
+  const T* z = kLocal ? nullptr : static_cast<const T*>(a.z);
   const T* Bp = static_cast<const T*>(a.Bm) + ((size_t)b * a.T * a.G + grp) * a.N;
   const T* Cp = static_cast<const T*>(a.Cm) + ((size_t)b * a.T * a.G + grp) * a.N;
-  T* y = static_cast<T*>(a.y);
+  const bool vecn = a.N % 4 == 0;
 
   // the lane's channel and states
   const int chl = tid / kScanLanes, q = tid % kScanLanes;
   const bool chan = chl < nch;
-  float A2[NL], h[NL];
-  const size_t st = ((size_t)b * a.C + c0 + chl) * a.N + q * NL;
+  const size_t row = (size_t)b * a.C + c0 + chl;
+  const size_t st = row * a.N + q * NL;
+  float* slot = a.chunk_state + (((size_t)kc * a.B + b) * a.C + c0 + chl) * NP + q * NL;
+  float2 A2[P], h[P];
 #pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const bool ok = chan && q * NL + i < a.N;
-    A2[i] = ok ? a.A[(size_t)(c0 + chl) * a.N + q * NL + i] * kLog2e : 0.f;
-    h[i] = ok && a.h0 ? a.h0[st + i] : 0.f;
+  for (int i = 0; i < 2 * P; ++i) {
+    const bool ok = chan && i < NL && q * NL + i < a.N;
+    pair_at(A2[i / 2], i & 1) = ok ? a.A[(size_t)(c0 + chl) * a.N + q * NL + i] * kLog2e : 0.f;
+    pair_at(h[i / 2], i & 1) = !kLocal && nchunk == 1 && ok && a.h0 ? a.h0[st + i] : 0.f;
   }
+  if (!kLocal && nchunk > 1 && chan) load_pairs<NL>(slot, h);
   // the staging role: channels sc .. sc + 3 of rows sr, sr + 16
   const int sc = tid % 8 * 4, sr = tid / 8;
   const int sn = nch - sc;
-  float bias[4], Dv[4];
+  float bias[4], Dv[4], dsum[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     bias[e] = a.dt_bias && e < sn ? a.dt_bias[c0 + sc + e] : 0.f;
-    Dv[e] = a.D && e < sn ? a.D[c0 + sc + e] : 0.f;
+    Dv[e] = !kLocal && a.D && e < sn ? a.D[c0 + sc + e] : 0.f;
+    dsum[e] = 0.f;
   }
   const size_t row0 = (size_t)b * a.T;
-  float xv[kRows][4], dv[kRows][4], zv[kRows][4];
+  Raw4<T> xv[kRows], dv[kRows], zv[kRows], bv[BPT], cv[BPT];
   auto fetch = [&](int t0) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const int t = t0 + sr + r * 16;
-      const int n = t < a.T ? sn : 0;
+      const int n = t < tend ? sn : 0;
       const size_t off = (row0 + t) * a.C + c0 + sc;
-      load_ch4(x + off, n, vec, xv[r]);
-      load_ch4(dt + off, n, vec, dv[r]);
-      if (z) load_ch4(z + off, n, vec, zv[r]);
+      xv[r].load(x + off, n, vec);
+      dv[r].load(dt + off, n, vec);
+      if (z) zv[r].load(z + off, n, vec);
+    }
+#pragma unroll
+    for (int r = 0; r < BPT; ++r) {
+      const int i = tid + r * kScanThreads, t = t0 + i / NL, n0 = i % NL * 4;
+      const int n = i < BV && t < tend ? a.N - n0 : 0;
+      const size_t off = (size_t)t * a.G * a.N + n0;
+      bv[r].load(Bp + off, n, vecn);
+      if (!kLocal) cv[r].load(Cp + off, n, vecn);
     }
   };
-  fetch(0);
-  for (int t0 = 0; t0 < a.T; t0 += kTT) {
-    float xs[kRows][4], zs[kRows][4];
+  fetch(tbeg);
+  for (int t0 = tbeg; t0 < tend; t0 += kTT) {
+    Raw4<T> xs[kRows], zs[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       const int tl = sr + r * 16;
+      float xf[4], df[4];
+      xv[r].get(xf);
+      dv[r].get(df);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float sig, d = dv[r][e] + bias[e];
+        float sig, d = df[e] + bias[e];
         if (a.softplus) d = softplus_sig(d, sig);
-        if (t0 + tl >= a.T) d = 0.f;   // past the end: the state stays
-        sDU[tl][sc + e] = make_float2(d, d * xv[r][e]);
-        xs[r][e] = xv[r][e];
-        zs[r][e] = z ? zv[r][e] : 0.f;
+        if (t0 + tl >= tend) d = 0.f;   // past the end: the state stays
+        const float u = d * xf[e];
+        sDU[tl][sc + e] = make_float4(d, d, u, u);
+        if (kLocal) dsum[e] += d;
       }
+      xs[r] = xv[r];
+      if (z) zs[r] = zv[r];
     }
-    for (int i = tid; i < kTT * NP; i += kScanThreads) {
-      const int tl = i / NP, n = i % NP;
-      const bool ok = t0 + tl < a.T && n < a.N;
-      const size_t off = (size_t)(t0 + tl) * a.G * a.N + n;
-      sB[tl][n] = load1(Bp + off, ok);
-      sC[tl][n] = load1(Cp + off, ok);
+#pragma unroll
+    for (int r = 0; r < BPT; ++r) {
+      const int i = tid + r * kScanThreads;
+      if (i < BV) {
+        float v[4];
+        bv[r].get(v);
+        store4(&sB[i / NL][i % NL * 4], make_float4(v[0], v[1], v[2], v[3]));
+        if (!kLocal) {
+          cv[r].get(v);
+          store4(&sC[i / NL][i % NL * 4], make_float4(v[0], v[1], v[2], v[3]));
+        }
+      }
     }
     __syncthreads();
-    if (t0 + kTT < a.T) fetch(t0 + kTT);
+    if (t0 + kTT < tend) fetch(t0 + kTT);
 #pragma unroll 1
     for (int g = 0; g < kTT; g += 4) {
-      if (a.ckpt && g % CK == 0 && t0 + g < a.T && chan) {
-        float* ck = a.ckpt + (((size_t)b * a.nck + (t0 + g) / CK) * a.C + c0 + chl) * NP + q * NL;
-        store_states(ck, h);
-      }
+      if (!kLocal && a.ckpt && g % CK == 0 && t0 + g < a.T && chan)
+        store_pairs<NL>(
+            a.ckpt + (((size_t)b * a.nck + (t0 + g) / CK) * a.C + c0 + chl) * NP + q * NL, h);
       float ys[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 du = sDU[g + j][chl];
-        float acc = 0.f;
+        const float4 du = sDU[g + j][chl];
+        const float2 d2 = make_float2(du.x, du.y), u2 = make_float2(du.z, du.w);
+        float2 B2[P], C2[P], acc = make_float2(0.f, 0.f);
+        load_pairs<NL>(&sB[g + j][q * NL], B2);
+        if (!kLocal) load_pairs<NL>(&sC[g + j][q * NL], C2);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const float dec = ex2(du.x * A2[i]);
-          h[i] = fmaf(dec, h[i], du.y * sB[g + j][q * NL + i]);
-          acc = fmaf(sC[g + j][q * NL + i], h[i], acc);
+        for (int i = 0; i < P; ++i) {
+          const float2 e = mul2(d2, A2[i]);
+          h[i] = fma2(make_float2(ex2(e.x), ex2(e.y)), h[i], mul2(u2, B2[i]));
+          if (!kLocal) acc = fma2(C2[i], h[i], acc);
         }
-        ys[j] = acc;
+        ys[j] = acc.x + acc.y;
       }
-      sY[g + q][chl] = quad_sum4(ys[0], ys[1], ys[2], ys[3], lane);
+      if (!kLocal) sY[g + q][chl] = quad_sum4(ys[0], ys[1], ys[2], ys[3], lane);
     }
     __syncthreads();
+    if (!kLocal) {
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int tl = sr + r * 16, t = t0 + tl;
-      float o[4];
+      for (int r = 0; r < kRows; ++r) {
+        const int tl = sr + r * 16, t = t0 + tl;
+        float o[4], xf[4], zf[4];
+        xs[r].get(xf);
+        if (z) zs[r].get(zf);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[e] = fmaf(Dv[e], xs[r][e], sY[tl][sc + e]);
-        if (z) o[e] *= __fdividef(zs[r][e], 1.f + __expf(-zs[r][e]));
+        for (int e = 0; e < 4; ++e) {
+          o[e] = fmaf(Dv[e], xf[e], sY[tl][sc + e]);
+          if (z) o[e] *= __fdividef(zf[e], 1.f + __expf(-zf[e]));
+        }
+        if (t < tend) store_ch4(static_cast<T*>(a.y) + (row0 + t) * a.C + c0 + sc, sn, vec, o);
       }
-      if (t < a.T) store_ch4(y + (row0 + t) * a.C + c0 + sc, sn, vec, o);
     }
   }
-  if (a.hT && chan) {
+  if (kLocal) {
+    if (chan) store_pairs<NL>(slot, h);
+    // the staging rows' sums of delta, added up in a fixed order
+    float* red = reinterpret_cast<float*>(sDU);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[sr * kScanCh + sc + e] = dsum[e];
+    __syncthreads();
+    if (tid < nch) {
+      float s = 0.f;
+      for (int r = 0; r < 16; ++r) s += red[r * kScanCh + tid];
+      a.chunk_sum[((size_t)kc * a.B + b) * a.C + c0 + tid] = s;
+    }
+  } else if (a.hT && chan && kc == nchunk - 1) {
 #pragma unroll
     for (int i = 0; i < NL; ++i)
-      if (q * NL + i < a.N) a.hT[st + i] = h[i];
+      if (q * NL + i < a.N) a.hT[st + i] = pair_at(h[i / 2], i & 1);
+  }
+}
+
+// Chains a cut row's chunks: state [chunk][rows = B C][NP] holds each chunk's end
+// from zero (the last chunk's is not read) and takes the state entering it.
+// kReverse: from the last chunk to the first (the backward's adjoint states),
+// the sum of steps being that of the chunk the state leaves through.
+template <bool kReverse>
+__global__ void __launch_bounds__(256)
+scan_chain_kernel(float* __restrict__ state, const float* __restrict__ sum,
+                  const float* __restrict__ A, const float* __restrict__ first, long long rows,
+                  int C, int N, int NP, int nchunk) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long row = i / NP;
+  const int n = (int)(i % NP);
+  if (row >= rows) return;
+  const float a2 = n < N ? A[(row % C) * N + n] * kLog2e : 0.f;
+  float h = n < N && first ? first[row * N + n] : 0.f;
+  for (int s = 0; s < nchunk; ++s) {
+    const long long k = kReverse ? nchunk - 1 - s : s;
+    float* p = state + k * rows * NP + i;
+    const float loc = s + 1 < nchunk ? *p : 0.f;
+    const float dec = s + 1 < nchunk ? ex2(a2 * sum[k * rows + row]) : 0.f;
+    *p = h;
+    h = fmaf(dec, h, loc);
   }
 }
 
@@ -196,6 +275,20 @@ cudaError_t launch_step(const ScanArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+template <typename T, int NL>
+cudaError_t launch_fwd(const ScanArgs& a, int tpg, int vec, const ScanSplit& sp, cudaStream_t st) {
+  const dim3 grid((unsigned)(tpg * a.G), a.B, sp.chunks);
+  if (sp.chunks > 1) {
+    scan_fwd_kernel<T, NL, true><<<dim3(grid.x, grid.y, sp.chunks - 1), kScanThreads, 0, st>>>(
+        a, tpg, vec, sp.tokens, sp.chunks);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_scan_chain(a, a.h0, sp.chunks, false, st);
+    if (e != cudaSuccess) return e;
+  }
+  scan_fwd_kernel<T, NL, false><<<grid, kScanThreads, 0, st>>>(a, tpg, vec, sp.tokens, sp.chunks);
+  return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t fwd_dispatch(const ScanArgs& a, cudaStream_t st) {
   if (a.T == 1 && !a.ckpt) {
@@ -211,16 +304,54 @@ cudaError_t fwd_dispatch(const ScanArgs& a, cudaStream_t st) {
   const int Cg = a.C / a.G;
   const int tpg = (Cg + kScanCh - 1) / kScanCh;
   const int vec = a.C % 4 == 0 && Cg % 4 == 0;
-  const dim3 grid((unsigned)(tpg * a.G), a.B);
-  if (a.N <= 4) scan_fwd_kernel<T, 1><<<grid, kScanThreads, 0, st>>>(a, tpg, vec);
-  else if (a.N <= 8) scan_fwd_kernel<T, 2><<<grid, kScanThreads, 0, st>>>(a, tpg, vec);
-  else if (a.N <= 16) scan_fwd_kernel<T, 4><<<grid, kScanThreads, 0, st>>>(a, tpg, vec);
-  else if (a.N <= 32) scan_fwd_kernel<T, 8><<<grid, kScanThreads, 0, st>>>(a, tpg, vec);
-  else scan_fwd_kernel<T, 16><<<grid, kScanThreads, 0, st>>>(a, tpg, vec);
-  return cudaGetLastError();
+  const ScanSplit sp = scan_split(a.B, a.T, a.C, a.G, false);
+  if (a.N <= 4) return launch_fwd<T, 1>(a, tpg, vec, sp, st);
+  if (a.N <= 8) return launch_fwd<T, 2>(a, tpg, vec, sp, st);
+  if (a.N <= 16) return launch_fwd<T, 4>(a, tpg, vec, sp, st);
+  if (a.N <= 32) return launch_fwd<T, 8>(a, tpg, vec, sp, st);
+  return launch_fwd<T, 16>(a, tpg, vec, sp, st);
 }
 
 }  // namespace
+
+// How a row is cut: blocks of the whole rows against those that fill the SMs
+// (seven of the forward's, three of the backward's fit one).
+ScanSplit scan_split(int B, int T, int C, int G, bool backward) {
+  const long long blocks = (long long)((C / G + kScanCh - 1) / kScanCh) * G * B;
+  const long long fill = 148LL * (backward ? 3 : 7);
+  ScanSplit s{1, T};
+  if (blocks > 148 || blocks <= 0) return s;
+  const long long want = fill / blocks;
+  long long tokens = (T + want - 1) / want;
+  if (tokens < 128) tokens = 128;   // a chunk's launch and chaining against its walk
+  tokens = (tokens + 31) / 32 * 32;
+  s.tokens = (int)tokens;
+  s.chunks = (int)((T + tokens - 1) / tokens);
+  return s;
+}
+
+size_t scan_split_bytes(int B, int C, int N, const ScanSplit& s) {
+  if (s.chunks <= 1) return 0;
+  return (size_t)s.chunks * B * C * (scan_padded_states(N) + 1) * sizeof(float);
+}
+
+void scan_split_workspace(ScanArgs& a, float* ws, const ScanSplit& s) {
+  a.chunk_state = ws;
+  a.chunk_sum = ws ? ws + (size_t)s.chunks * a.B * a.C * scan_padded_states(a.N) : nullptr;
+}
+
+cudaError_t launch_scan_chain(const ScanArgs& a, const float* first, int chunks, bool reverse,
+                              cudaStream_t st) {
+  const int NP = scan_padded_states(a.N);
+  const long long rows = (long long)a.B * a.C, blocks = (rows * NP + 255) / 256;
+  if (reverse)
+    scan_chain_kernel<true><<<(unsigned)blocks, 256, 0, st>>>(a.chunk_state, a.chunk_sum, a.A,
+                                                              first, rows, a.C, a.N, NP, chunks);
+  else
+    scan_chain_kernel<false><<<(unsigned)blocks, 256, 0, st>>>(a.chunk_state, a.chunk_sum, a.A,
+                                                               first, rows, a.C, a.N, NP, chunks);
+  return cudaGetLastError();
+}
 
 int scan_padded_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
@@ -229,6 +360,10 @@ int scan_checkpoint_tokens(int N) { return N <= 16 ? 16 : N <= 32 ? 8 : 4; }
 size_t scan_checkpoint_bytes(int B, int T, int C, int N) {
   const int k = scan_checkpoint_tokens(N);
   return (size_t)B * ((T + k - 1) / k) * C * scan_padded_states(N) * sizeof(float);
+}
+
+size_t selective_scan_workspace_bytes(int B, int T, int C, int N, int G) {
+  return scan_split_bytes(B, C, N, scan_split(B, T, C, G, false));
 }
 
 cudaError_t launch_selective_scan(const ScanArgs& a, cudaStream_t st) {

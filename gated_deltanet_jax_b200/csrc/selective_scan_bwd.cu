@@ -121,17 +121,17 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, float* __rest
   }
   const size_t row0 = (size_t)b * f.T;
   const int ntiles = (f.T + CK - 1) / CK;
-  float xv[ROWS][4], dv[ROWS][4], zv[ROWS][4], gv[ROWS][4];
+  Raw4<T> xr[ROWS], dr[ROWS], zr[ROWS], gr[ROWS];
   auto fetch = [&](int t0) {
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const int t = t0 + sr + r * RT;
       const int n = stages && t < f.T ? sn : 0;
       const size_t off = (row0 + t) * f.C + c0 + sc;
-      load_ch4(x + off, n, vec, xv[r]);
-      load_ch4(dt + off, n, vec, dv[r]);
-      load_ch4(dy + off, n, vec, gv[r]);
-      if (z) load_ch4(z + off, n, vec, zv[r]);
+      xr[r].load(x + off, n, vec);
+      dr[r].load(dt + off, n, vec);
+      gr[r].load(dy + off, n, vec);
+      if (z) zr[r].load(z + off, n, vec);
     }
   };
   if (ntiles > 0) fetch((ntiles - 1) * CK);
@@ -142,21 +142,26 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, float* __rest
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const int tl = sr + r * RT;
+      float xv[4], dv[4], gv[4], zv[4];
+      xr[r].get(xv);
+      dr[r].get(dv);
+      gr[r].get(gv);
+      if (z) zr[r].get(zv);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float sig = 1.f, d = dv[r][e] + bias[e];
+        float sig = 1.f, d = dv[e] + bias[e];
         if (f.softplus) d = softplus_sig(d, sig);
         if (t0 + tl >= f.T) d = 0.f;
-        float g = gv[r][e];
+        float g = gv[e];
         kz[r][e] = 0.f;
         if (z) {
-          const float zz = zv[r][e];
+          const float zz = zv[e];
           const float sz = __fdividef(1.f, 1.f + __expf(-zz));
           kz[r][e] = g * (sz * fmaf(zz, 1.f - sz, 1.f));
           g *= zz * sz;
         }
         ks[r][e] = sig;
-        if (stages) s.p[tl][sc + e] = make_float4(d, d * xv[r][e], g, xv[r][e]);
+        if (stages) s.p[tl][sc + e] = make_float4(d, d * xv[e], g, xv[e]);
       }
     }
     for (int i = tid; i < CK * NP; i += kScanThreads) {

@@ -39,18 +39,53 @@ __device__ __forceinline__ float load1(const T* p, bool ok) {
   return ok ? to_f32(*p) : 0.f;
 }
 
-// Four consecutive channels of a row: one vector when the row allows it, else
-// element by element.  `n`: channels in range (<= 0: none).
+// Four consecutive elements as they lie in memory (a load in flight holds two
+// registers in bf16), the ones past `n` zero.  `vec`: the row allows one vector.
 template <typename T>
-__device__ __forceinline__ void load_ch4(const T* p, int n, bool vec, float (&v)[4]) {
-  if (vec && n >= 4) {
-    const float4 q = load4(p);
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = load1(p + e, e < n);
+struct Raw4;
+template <>
+struct Raw4<__nv_bfloat16> {
+  uint2 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int n, bool vec) {
+    u = make_uint2(0u, 0u);
+    if (n <= 0) return;
+    if (vec && n >= 4) {
+      u = *reinterpret_cast<const uint2*>(p);
+    } else {
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+      u.x = q[0];
+      if (n > 1) u.x |= (uint32_t)q[1] << 16;
+      if (n > 2) u.y = q[2];
+      if (n > 3) u.y |= (uint32_t)q[3] << 16;
+    }
   }
-}
+  __device__ __forceinline__ void get(float (&v)[4]) const {
+    v[0] = __uint_as_float(u.x << 16);
+    v[1] = __uint_as_float(u.x & 0xffff0000u);
+    v[2] = __uint_as_float(u.y << 16);
+    v[3] = __uint_as_float(u.y & 0xffff0000u);
+  }
+};
+template <>
+struct Raw4<float> {
+  float4 u;
+  __device__ __forceinline__ void load(const float* p, int n, bool vec) {
+    u = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (n <= 0) return;
+    if (vec && n >= 4) {
+      u = load4(p);
+    } else {
+      u.x = p[0];
+      if (n > 1) u.y = p[1];
+      if (n > 2) u.z = p[2];
+      if (n > 3) u.w = p[3];
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[4]) const {
+    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ void store_ch4(T* p, int n, bool vec, const float (&v)[4]) {
   if (vec && n >= 4) {
@@ -60,6 +95,23 @@ __device__ __forceinline__ void store_ch4(T* p, int n, bool vec, const float (&v
     for (int e = 0; e < 4; ++e)
       if (e < n) p[e] = from_f32<T>(v[e]);
   }
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return r;
 }
 
 // Sums four tokens' values over the four lanes of a channel in three shuffles:
@@ -107,6 +159,40 @@ __device__ __forceinline__ void load_states(const float* p, float (&v)[NL]) {
     for (int i = 0; i < NL; ++i) v[i] = p[i];
   }
 }
+
+// A lane's states as pairs (NL = 1: one state and an idle second).
+template <int NL>
+constexpr int scan_pairs() { return NL == 1 ? 1 : NL / 2; }
+
+// One token's row of B or C for a lane from shared memory.
+template <int NL>
+__device__ __forceinline__ void load_pairs(const float* p, float2 (&v)[scan_pairs<NL>()]) {
+  if constexpr (NL == 1) {
+    v[0] = make_float2(p[0], 0.f);
+  } else if constexpr (NL == 2) {
+    v[0] = *reinterpret_cast<const float2*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NL; i += 4) {
+      const float4 q = load4(p + i);
+      v[i / 2] = make_float2(q.x, q.y);
+      v[i / 2 + 1] = make_float2(q.z, q.w);
+    }
+  }
+}
+template <int NL>
+__device__ __forceinline__ void store_pairs(float* p, const float2 (&v)[scan_pairs<NL>()]) {
+  if constexpr (NL == 1) {
+    p[0] = v[0].x;
+  } else if constexpr (NL == 2) {
+    *reinterpret_cast<float2*>(p) = v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NL; i += 4)
+      store4(p + i, make_float4(v[i / 2].x, v[i / 2].y, v[i / 2 + 1].x, v[i / 2 + 1].y));
+  }
+}
+__device__ __forceinline__ float& pair_at(float2& v, int i) { return i ? v.y : v.x; }
 
 // Tokens of the backward's tile (and the distance of the forward's checkpoints)
 // for NL states a lane: 64 decay factors a lane stay in registers.

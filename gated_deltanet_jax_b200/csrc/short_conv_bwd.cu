@@ -8,7 +8,7 @@
 //   dw[j]   = sum_{b,t} dpre[t] xe[t + j],   dbias = sum_{b,t} dpre[t].
 //
 // HBM-bound: x and dy are read once and dx is written once (pre is formed
-// again from x; it is not kept between the passes).  A thread owns four
+// again from x; it is not kept between the passes).  A thread owns two
 // channels and walks a tile of tokens with x and dpre in sliding register
 // windows; a tile reads K - 1 rows before it and K - 1 after it again.  The
 // sums over tokens stay in registers (fp32) and leave as one partial row per
@@ -22,16 +22,22 @@ namespace gdn {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kVec = 4;        // channels of a thread: 8 bytes of bf16, 16 of fp32
+constexpr int kVec = 2;        // channels of a thread: a warp reads 128 bytes of bf16 a row
 constexpr int kAhead = 4;      // tokens whose loads are in flight together
 
-__device__ __forceinline__ void ld4(const float* p, float (&v)[kVec]) {
-  const float4 q = load4(p);
-  v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+__device__ __forceinline__ void ld(const float* p, float (&v)[kVec]) {
+  const float2 q = *reinterpret_cast<const float2*>(p);
+  v[0] = q.x; v[1] = q.y;
 }
-__device__ __forceinline__ void ld4(const __nv_bfloat16* p, float (&v)[kVec]) {
-  const float4 q = load4(p);
-  v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+__device__ __forceinline__ void ld(const __nv_bfloat16* p, float (&v)[kVec]) {
+  const float2 q = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
+  v[0] = q.x; v[1] = q.y;
+}
+__device__ __forceinline__ void st2(float* p, const float (&v)[kVec]) {
+  *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+}
+__device__ __forceinline__ void st2(__nv_bfloat16* p, const float (&v)[kVec]) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v[0], v[1]);
 }
 
 // Block (channel group, token tile, row b).  part [B * tiles][K + 1][C]: this
@@ -51,7 +57,7 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
   constexpr int W = K > 1 ? K - 1 : 1;
   float wk[K][kVec], bs[kVec], win[W][kVec], dwin[W][kVec], dw[K][kVec], db[kVec];
 #pragma unroll
-  for (int j = 0; j < K; ++j) ld4(w + (size_t)j * C + c, wk[j]);
+  for (int j = 0; j < K; ++j) ld(w + (size_t)j * C + c, wk[j]);
 #pragma unroll
   for (int e = 0; e < kVec; ++e) {
     bs[e] = bias ? bias[c + e] : 0.f;
@@ -67,9 +73,9 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
   for (int j = 0; j < K - 1; ++j) {
     const int tt = t0 - (K - 1) + j;
     if (tt >= 0) {
-      ld4(x + (row0 + tt) * C + c, win[j]);
+      ld(x + (row0 + tt) * C + c, win[j]);
     } else if (state_in) {
-      ld4(state_in + ((size_t)b * (K - 1) + (K - 1) + tt) * C + c, win[j]);
+      ld(state_in + ((size_t)b * (K - 1) + (K - 1) + tt) * C + c, win[j]);
     } else {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) win[j][e] = 0.f;
@@ -83,8 +89,8 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
     for (int i = 0; i < kAhead; ++i) {
       const int t = tb + i;
       if (t < T && t < tend) {
-        ld4(x + (row0 + t) * C + c, xv[i]);
-        ld4(dy + (row0 + t) * C + c, gv[i]);
+        ld(x + (row0 + t) * C + c, xv[i]);
+        ld(dy + (row0 + t) * C + c, gv[i]);
       } else {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) xv[i][e] = gv[i][e] = 0.f;
@@ -102,7 +108,7 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
         for (int j = 0; j < K - 1; ++j) pre = fmaf(wk[j][e], win[j][e], pre);
         float d = gv[i][e];
         if (act) {
-          const float sg = 1.f / (1.f + __expf(-pre));
+          const float sg = __fdividef(1.f, 1.f + __expf(-pre));
           d *= sg * fmaf(pre, 1.f - sg, 1.f);
         }
         if (t >= T) d = 0.f;
@@ -133,22 +139,20 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
       // the final window's rows are the inputs s = T - (K - 1) .. T - 1
       if (dstate_out && s >= T - (K - 1)) {
         float g[kVec];
-        ld4(dstate_out + ((size_t)b * (K - 1) + (s - (T - (K - 1)))) * C + c, g);
+        ld(dstate_out + ((size_t)b * (K - 1) + (s - (T - (K - 1)))) * C + c, g);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) out[e] += g[e];
       }
-      const float4 o4 = make_float4(out[0], out[1], out[2], out[3]);
       if (s >= 0)
-        store4(dx + (row0 + s) * C + c, o4);
+        st2(dx + (row0 + s) * C + c, out);
       else if (dstate_in)
-        store4(dstate_in + ((size_t)b * (K - 1) + (K - 1) + s) * C + c, o4);
+        st2(dstate_in + ((size_t)b * (K - 1) + (K - 1) + s) * C + c, out);
     }
   }
   float* pr = part + ((size_t)b * gridDim.y + blockIdx.y) * (K + 1) * C + c;
 #pragma unroll
-  for (int j = 0; j < K; ++j)
-    store4(pr + (size_t)j * C, make_float4(dw[j][0], dw[j][1], dw[j][2], dw[j][3]));
-  store4(pr + (size_t)K * C, make_float4(db[0], db[1], db[2], db[3]));
+  for (int j = 0; j < K; ++j) st2(pr + (size_t)j * C, dw[j]);
+  st2(pr + (size_t)K * C, db);
 }
 
 template <typename Tin>
@@ -177,13 +181,13 @@ cudaError_t bwd_dispatch(const ShortConvBwdArgs& a, int TT, int tiles, cudaStrea
 }
 
 // Token tiles: enough warps to keep loads in flight on every SM (24 a SM),
-// tiles of 32 to 512 tokens (a tile reads 2 (K - 1) rows more than it owns).
+// tiles of 16 to 512 tokens (a tile reads 2 (K - 1) rows more than it owns).
 int conv_bwd_tile(int B, int T, int C) {
   const long long warps_per_row = (C + kVec * 32 - 1) / (kVec * 32);
   const long long want = 24LL * 148;
   long long tt = (long long)B * T * warps_per_row / want;
   tt = (tt + 15) / 16 * 16;
-  if (tt < 32) tt = 32;
+  if (tt < 16) tt = 16;
   if (tt > 512) tt = 512;
   if ((T + tt - 1) / tt > 65535) tt = ((long long)T + 65534) / 65535;
   return (int)tt;

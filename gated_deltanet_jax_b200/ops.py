@@ -41,6 +41,7 @@ Differences from the reference, all additive:
 
 from __future__ import annotations
 
+import contextlib
 from typing import Optional, Tuple
 
 import torch
@@ -471,31 +472,50 @@ def _layer_impl(entry, q, k, v, a, b, A_log, dt_bias, gate, norm_weight, eps, in
 _ACTIVATIONS = {"silu": 1, "swish": 1, None: 0}
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on_device(index: int):
+    """``torch.cuda.device`` where it is not the current one already (single-token
+    calls are bound by their host work)."""
+    return _NO_SWITCH if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def _stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """Contiguous and 16-byte aligned, as the kernels read and write."""
-    t = t.contiguous()
+    if t is None:
+        return None
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _float_vec(t, shape, name, dev):
-    """An optional fp32 parameter of the given shape on ``dev``."""
-    if t is None:
-        return None
-    t = torch.as_tensor(t, device=dev).to(torch.float32)
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be {list(shape)}; got {tuple(t.shape)}")
+def _aligned32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """The same in fp32."""
+    if t is not None and t.dtype is not torch.float32:
+        t = t.to(torch.float32)
     return _aligned(t)
 
 
-def _check_inputs(pairs, dev, dtype):
-    """CUDA tensors of one device and one dtype."""
-    for name, t in pairs:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, not on {dev}")
-        if t.dtype != dtype:
-            raise TypeError(f"{name} must be {dtype} like the other inputs; got {t.dtype}")
+def _on(t, dev):
+    """A parameter on ``dev``: CUDA tensors stay, host values are copied."""
+    if isinstance(t, torch.Tensor) and t.device == dev:
+        return t
+    return torch.as_tensor(t, device=dev)
+
+
+def _check_input(name, t, dev, dtype):
+    """A CUDA tensor on the same device and of the same dtype as the first input."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, not on {dev}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} like the other inputs; got {t.dtype}")
 
 
 def _cuda_input(name, t):
@@ -511,9 +531,7 @@ class _ShortConvFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, conv_state, act):
         x = _aligned(x)
-        w32 = _aligned(w.to(torch.float32))
-        b32 = None if bias is None else _aligned(bias.to(torch.float32))
-        st = None if conv_state is None else _aligned(conv_state)
+        w32, b32, st = _aligned32(w), _aligned32(bias), _aligned(conv_state)
         s_out = x.new_empty((x.shape[0], w.shape[0] - 1, x.shape[2]))
         y = _short_conv_fwd(x, w32, b32, st, s_out, act)
         ctx.act = act
@@ -529,18 +547,19 @@ class _ShortConvFn(torch.autograd.Function):
         B, T, C = x.shape
         K = w.shape[0]
         dy = torch.zeros_like(x) if dy is None else _aligned(dy)
-        ds = None if ds is None else _aligned(ds)
+        ds = _aligned(ds)
         dx, dw = torch.empty_like(x), torch.empty_like(w)
         db = None if bias is None else torch.empty_like(bias)
         dst = None if st is None else torch.empty_like(st)
         lib = _lib.load()
-        with torch.cuda.device(x.device):
+        dev = x.get_device()
+        with _on_device(dev):
             n = lib.gdn_short_conv_bwd_workspace_bytes(B, T, C, K)
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
             rc = lib.gdn_short_conv_bwd(
                 _ptr(x), _ptr(w), _ptr(bias), _ptr(st), _ptr(dy), _ptr(ds), _ptr(dx), _ptr(dw),
                 _ptr(db), _ptr(dst), B, T, C, K, ctx.act, _DTYPES[x.dtype], _ptr(ws), n,
-                torch.cuda.current_stream(x.device).cuda_stream)
+                _stream(dev))
         _lib.check(rc, "gdn_short_conv_bwd")
         return (dx, dw.to(ctx.w_dtype), None if db is None else db.to(ctx.b_dtype), dst, None)
 
@@ -550,10 +569,11 @@ def _short_conv_fwd(x, w, bias, s_in, s_out, act):
     B, T, C = x.shape
     y = torch.empty_like(x)
     lib = _lib.load()
-    with torch.cuda.device(x.device):
+    dev = x.get_device()
+    with _on_device(dev):
         rc = lib.gdn_short_conv_fwd_bias(_ptr(x), _ptr(w), _ptr(bias), _ptr(s_in), _ptr(s_out),
                                          _ptr(y), B, T, C, w.shape[0], act, _DTYPES[x.dtype],
-                                         torch.cuda.current_stream(x.device).cuda_stream)
+                                         _stream(dev))
     _lib.check(rc, "gdn_short_conv_fwd")
     return y
 
@@ -583,7 +603,8 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
     if act is None:
         raise ValueError(f"activation must be 'silu', 'swish' or None; got {activation!r}")
     B, T, C = x.shape
-    w = torch.as_tensor(weight, device=x.device)
+    dev = x.device
+    w = _on(weight, dev)
     if w.dim() == 3:
         w = w.reshape(w.shape[0], w.shape[-1])
     if w.dim() != 2 or w.shape[1] != C:
@@ -594,8 +615,8 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
     def state(t, name):
         if t is None:
             return None
-        if tuple(t.shape) != shape or t.dtype != x.dtype or t.device != x.device:
-            raise ValueError(f"{name} must be {shape} {x.dtype} on {x.device}")
+        if tuple(t.shape) != shape or t.dtype != x.dtype or t.device != dev:
+            raise ValueError(f"{name} must be {shape} {x.dtype} on {dev}")
         if not t.is_contiguous() or t.data_ptr() % 16:
             raise ValueError(f"{name} must be contiguous and 16-byte aligned")
         return t
@@ -603,7 +624,7 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
     s_in = state(conv_state, "conv_state")
     s_out = state(final_state_out, "final_state_out")
     if bias is not None:
-        bias = torch.as_tensor(bias, device=x.device)
+        bias = _on(bias, dev)
         if tuple(bias.shape) != (C,):
             raise ValueError(f"bias must be [{C}]; got {tuple(bias.shape)}")
     if _wants_grad(x, w, bias, conv_state):
@@ -612,10 +633,8 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
         y, s_out = _ShortConvFn.apply(x, w, bias, s_in, act)
         return y, s_out if output_final_state else None
     if s_out is None and output_final_state:
-        s_out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    y = _short_conv_fwd(_aligned(x), _aligned(w.to(torch.float32)),
-                        None if bias is None else _aligned(bias.to(torch.float32)), s_in, s_out,
-                        act)
+        s_out = torch.empty(shape, dtype=x.dtype, device=dev)
+    y = _short_conv_fwd(_aligned(x), _aligned32(w), _aligned32(bias), s_in, s_out, act)
     return y, s_out
 
 
@@ -626,9 +645,10 @@ def _glu_fwd(x, wg, wu, keep):
     h = x.new_empty((M, I))
     g, u = (x.new_empty((M, I)), x.new_empty((M, I))) if keep else (None, None)
     lib = _lib.load()
-    with torch.cuda.device(x.device):
+    dev = x.get_device()
+    with _on_device(dev):
         rc = lib.gdn_glu_fwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(h), _ptr(g), _ptr(u), M, D, I,
-                             _DTYPES[x.dtype], torch.cuda.current_stream(x.device).cuda_stream)
+                             _DTYPES[x.dtype], _stream(dev))
     _lib.check(rc, "gdn_glu_fwd")
     return h, g, u
 
@@ -651,12 +671,13 @@ class _GluFn(torch.autograd.Function):
         dx = torch.empty_like(x) if need_x else None
         dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_w else (None, None)
         lib = _lib.load()
-        with torch.cuda.device(x.device):
+        dev = x.get_device()
+        with _on_device(dev):
             n = lib.gdn_glu_bwd_workspace_bytes(M, I, _DTYPES[x.dtype])
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
             rc = lib.gdn_glu_bwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(g), _ptr(u), _ptr(dh),
                                  _ptr(dx), _ptr(dwg), _ptr(dwu), M, D, I, _DTYPES[x.dtype],
-                                 _ptr(ws), n, torch.cuda.current_stream(x.device).cuda_stream)
+                                 _ptr(ws), n, _stream(dev))
         _lib.check(rc, "gdn_glu_bwd")
         return dx, dwg, dwu
 
@@ -677,17 +698,18 @@ def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") ->
     if x.dim() < 1:
         raise ValueError("x must be [...,D]")
     D = x.shape[-1]
-    _check_inputs((("gate_weight", gate_weight), ("up_weight", up_weight)), x.device, x.dtype)
+    dev, dtype = x.device, x.dtype
+    _check_input("gate_weight", gate_weight, dev, dtype)
+    _check_input("up_weight", up_weight, dev, dtype)
     if gate_weight.dim() != 2 or gate_weight.shape[1] != D or up_weight.shape != gate_weight.shape:
         raise ValueError(f"gate_weight and up_weight must both be [I,{D}]; got "
                          f"{tuple(gate_weight.shape)}, {tuple(up_weight.shape)}")
-    M = x.numel() // D if D else x.shape[:-1].numel()
-    x2 = x.reshape(M, D)
+    x2 = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), D)
     if _wants_grad(x, gate_weight, up_weight):
         h = _GluFn.apply(x2, gate_weight, up_weight)
     else:
         h, _, _ = _glu_fwd(_aligned(x2), _aligned(gate_weight), _aligned(up_weight), False)
-    return h.reshape(*x.shape[:-1], gate_weight.shape[0])
+    return h if x2 is x else h.reshape(*x.shape[:-1], gate_weight.shape[0])
 
 
 def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, keep):
@@ -697,15 +719,18 @@ def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, keep):
     G, N = B.shape[2], A.shape[1]
     y = torch.empty_like(x)
     lib = _lib.load()
-    with torch.cuda.device(x.device):
+    dev = x.get_device()
+    with _on_device(dev):
         ck = None
         if keep:
             n = lib.gdn_selective_scan_checkpoint_bytes(b, T, ch, N)
             ck = torch.empty(max(n // 4, 4), dtype=torch.float32, device=x.device)
+        n = lib.gdn_selective_scan_workspace_bytes(b, T, ch, N, G) if T > 1 else 0
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
         rc = lib.gdn_selective_scan_fwd(
             _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
             _ptr(h0), _ptr(y), _ptr(hT), _ptr(ck), b, T, ch, N, G, softplus, _DTYPES[x.dtype],
-            torch.cuda.current_stream(x.device).cuda_stream)
+            _ptr(ws), n, _stream(dev))
     _lib.check(rc, "gdn_selective_scan_fwd")
     return y, ck
 
@@ -713,11 +738,9 @@ def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, keep):
 class _SelectiveScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, h0, softplus):
-        f32 = lambda t: None if t is None else _aligned(t.to(torch.float32))  # noqa: E731
-        x, dt, B, C = _aligned(x), _aligned(dt), _aligned(B), _aligned(C)
-        z = None if z is None else _aligned(z)
+        x, dt, B, C, z = _aligned(x), _aligned(dt), _aligned(B), _aligned(C), _aligned(z)
         ctx.dtypes = [None if t is None else t.dtype for t in (A, D, dt_bias, h0)]
-        A, D, dt_bias, h0 = f32(A), f32(D), f32(dt_bias), f32(h0)
+        A, D, dt_bias, h0 = (_aligned32(t) for t in (A, D, dt_bias, h0))
         hT = torch.empty((x.shape[0], x.shape[2], A.shape[1]), dtype=torch.float32,
                          device=x.device)
         y, ck = _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, True)
@@ -732,22 +755,22 @@ class _SelectiveScanFn(torch.autograd.Function):
         x, dt, A, B, C, D, z, dt_bias, ck = ctx.saved_tensors
         b, T, ch = x.shape
         G, N = B.shape[2], A.shape[1]
-        dev = x.device
+        dev = x.get_device()
         dy = torch.zeros_like(x) if dy is None else _aligned(dy)
-        dhT = None if dhT is None else _aligned(dhT.to(torch.float32))
+        dhT = _aligned32(dhT)
         like = lambda t: None if t is None else torch.empty_like(t)  # noqa: E731
         dx, ddt, dA, dB, dC = like(x), like(dt), like(A), like(B), like(C)
         dD, dz, dbias = like(D), like(z), like(dt_bias)
         dh0 = torch.empty((b, ch, N), dtype=torch.float32, device=dev) if ctx.has_h0 else None
         lib = _lib.load()
-        with torch.cuda.device(dev):
+        with _on_device(dev):
             n = lib.gdn_selective_scan_bwd_workspace_bytes(b, T, ch, N, G)
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
             rc = lib.gdn_selective_scan_bwd(
                 _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
                 _ptr(ck), _ptr(dy), _ptr(dhT), _ptr(dx), _ptr(ddt), _ptr(dA), _ptr(dB), _ptr(dC),
                 _ptr(dD), _ptr(dz), _ptr(dbias), _ptr(dh0), b, T, ch, N, G, ctx.softplus,
-                _DTYPES[x.dtype], _ptr(ws), n, torch.cuda.current_stream(dev).cuda_stream)
+                _DTYPES[x.dtype], _ptr(ws), n, _stream(dev))
         _lib.check(rc, "gdn_selective_scan_bwd")
         to = lambda t, d: None if t is None else t.to(d)  # noqa: E731
         Ad, Dd, bd, hd = ctx.dtypes
@@ -781,12 +804,16 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
     if x.dim() != 3:
         raise ValueError(f"x must be [B,T,Ch]; got {tuple(x.shape)}")
     dev = x.device
-    _check_inputs((("dt", dt), ("B", B), ("C", C)) + ((("z", z),) if z is not None else ()), dev,
-                  x.dtype)
+    dtype = x.dtype
+    _check_input("dt", dt, dev, dtype)
+    _check_input("B", B, dev, dtype)
+    _check_input("C", C, dev, dtype)
+    if z is not None:
+        _check_input("z", z, dev, dtype)
     b, T, ch = x.shape
     if dt.shape != x.shape or (z is not None and z.shape != x.shape):
         raise ValueError(f"dt and z must have x's shape {tuple(x.shape)}")
-    A = torch.as_tensor(A, device=dev)
+    A = _on(A, dev)
     if A.dim() != 2 or A.shape[0] != ch:
         raise ValueError(f"A must be [{ch},N]; got {tuple(A.shape)}")
     N = A.shape[1]
@@ -803,8 +830,8 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
     for name, t in (("D", D), ("dt_bias", dt_bias)):
         if t is not None and tuple(t.shape) != (ch,):
             raise ValueError(f"{name} must be [{ch}]; got {tuple(t.shape)}")
-    D = None if D is None else torch.as_tensor(D, device=dev)
-    dt_bias = None if dt_bias is None else torch.as_tensor(dt_bias, device=dev)
+    D = None if D is None else _on(D, dev)
+    dt_bias = None if dt_bias is None else _on(dt_bias, dev)
     shape = (b, ch, N)
     if initial_state is not None and (tuple(initial_state.shape) != shape
                                       or initial_state.device != dev):
@@ -823,11 +850,9 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
                              f"{shape} tensor on {dev}")
     elif output_final_state:
         hT = torch.empty(shape, dtype=torch.float32, device=dev)
-    h0 = None if initial_state is None else _aligned(initial_state.to(torch.float32))
-    y, _ = _scan_fwd(_aligned(x), _aligned(dt), _float_vec(A, (ch, N), "A", dev), _aligned(B),
-                     _aligned(C), _float_vec(D, (ch,), "D", dev),
-                     None if z is None else _aligned(z), _float_vec(dt_bias, (ch,), "dt_bias", dev),
-                     softplus, h0, hT, False)
+    y, _ = _scan_fwd(_aligned(x), _aligned(dt), _aligned32(A), _aligned(B), _aligned(C),
+                     _aligned32(D), _aligned(z), _aligned32(dt_bias), softplus,
+                     _aligned32(initial_state), hT, False)
     return y, hT
 
 

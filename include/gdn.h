@@ -443,13 +443,17 @@ int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void*
  * NULL: zero).  h0, hT [B, C, N] fp32: NULL h0 starts from zeros, NULL hT drops
  * the final state, h0 == hT updates in place (decode: T = 1).  N <= 64.
  * `checkpoints` (NULL: not wanted; gdn_selective_scan_checkpoint_bytes())
- * receives the states that gdn_selective_scan_bwd restarts from.
+ * receives the states that gdn_selective_scan_bwd restarts from.  `workspace`:
+ * gdn_selective_scan_workspace_bytes() bytes (0 where the rows are not cut:
+ * long rows of few channels run as chunks).
  */
 size_t gdn_selective_scan_checkpoint_bytes(int B, int T, int C, int N);
+size_t gdn_selective_scan_workspace_bytes(int B, int T, int C, int N, int G);
 int gdn_selective_scan_fwd(const void* x, const void* dt, const float* A, const void* Bm,
                            const void* Cm, const float* D, const void* z, const float* dt_bias,
                            const float* h0, void* y, float* hT, float* checkpoints, int B, int T,
-                           int C, int N, int G, int softplus, int dtype, void* stream);
+                           int C, int N, int G, int softplus, int dtype, void* workspace,
+                           size_t ws_bytes, void* stream);
 
 /*
  * Its gradients from dy [B, T, C] (dtype) and dhT [B, C, N] (fp32, NULL: zero):

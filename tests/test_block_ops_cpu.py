@@ -111,9 +111,9 @@ def test_glu_rejects_bad_arguments(lib):
 
 def test_scan_rejects_bad_arguments(lib):
     def fwd(x=P, dt=P, A=P, B=P, C=P, D=None, z=None, h0=None, y=P, hT=None, ck=None, b=2, T=5,
-            ch=8, N=4, G=1, sp=1, dtype=BF16):
+            ch=8, N=4, G=1, sp=1, dtype=BF16, ws=None, n=0):
         return lib.gdn_selective_scan_fwd(x, dt, A, B, C, D, z, None, h0, y, hT, ck, b, T, ch, N,
-                                          G, sp, dtype, None)
+                                          G, sp, dtype, ws, n, None)
     for kw in (dict(T=-1), dict(dtype=9), dict(sp=2), dict(G=0), dict(G=3), dict(x=None),
                dict(A=None), dict(y=None), dict(z=BAD), dict(h0=BAD), dict(hT=BAD), dict(ck=BAD),
                dict(T=(1 << 30) + 1)):
@@ -121,6 +121,11 @@ def test_scan_rejects_bad_arguments(lib):
     for kw in (dict(N=0), dict(N=65), dict(b=65536)):
         assert fwd(**kw) == UNSUPPORTED, kw
     assert fwd(b=0) == OK and fwd(ch=0) == OK and fwd(T=0) == OK
+    # a long row of few channels is cut into chunks and needs room for their states
+    need = lib.gdn_selective_scan_workspace_bytes(2, 5000, 8, 4, 1)
+    assert need > 0 and lib.gdn_selective_scan_workspace_bytes(2, 5, 8, 4, 1) == 0
+    assert fwd(T=5000) == INVALID and fwd(T=5000, ws=P, n=need - 1) == INVALID
+    assert fwd(T=5000, ws=BAD, n=need) == INVALID
     assert lib.gdn_selective_scan_checkpoint_bytes(2, 33, 8, 16) == 2 * 3 * 8 * 16 * 4
     assert lib.gdn_selective_scan_checkpoint_bytes(2, 33, 8, 65) == 0
 

@@ -160,7 +160,8 @@ SCAN = [(1, 1, 8, 16, 1, True), (3, 1, 40, 16, 1, False), (2, 1, 24, 5, 2, True)
         (1, 15, 33, 16, 1, True), (2, 16, 64, 16, 2, False), (1, 17, 66, 16, 3, True),
         (2, 33, 40, 3, 1, True), (1, 64, 96, 8, 1, True), (2, 31, 20, 7, 1, False),
         (1, 40, 48, 24, 2, True), (1, 35, 36, 32, 1, True), (1, 23, 40, 64, 1, True),
-        (1, 130, 7, 16, 1, True), (2, 200, 64, 16, 1, True), (1, 300, 34, 12, 2, False)]
+        (1, 130, 7, 16, 1, True), (2, 200, 64, 16, 1, True), (1, 300, 34, 12, 2, False),
+        (1, 700, 40, 16, 1, True), (3, 129, 8, 6, 1, True)]
 
 
 def _scan_inputs(b, T, ch, N, G, full, dtype, dev, seed):
