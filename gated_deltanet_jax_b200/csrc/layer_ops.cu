@@ -11,6 +11,8 @@
 // Both are HBM-bound: each element is read once and written once.  A thread of
 // the norm owns 16-byte vectors (8 bf16 or 4 fp32), one of the convolution four
 // channels.
+#include <type_traits>
+
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 
@@ -61,9 +63,15 @@ __device__ __forceinline__ float silu_acc(float x) { return x / (1.f + expf(-x))
 template <typename Tin>
 struct Vec4 {
   static constexpr int N = 4;
-  __device__ static void load(const Tin* p, float (&f)[N]) {
-    const float4 q = load4(p);
-    f[0] = q.x; f[1] = q.y; f[2] = q.z; f[3] = q.w;
+  using Raw = typename std::conditional<sizeof(Tin) == 2, uint2, float4>::type;
+  __device__ static Raw load_raw(const Tin* p) { return *reinterpret_cast<const Raw*>(p); }
+  __device__ static void get(const uint2& u, float2 (&f)[N / 2]) {
+    f[0] = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u));
+    f[1] = make_float2(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+  }
+  __device__ static void get(const float4& u, float2 (&f)[N / 2]) {
+    f[0] = make_float2(u.x, u.y);
+    f[1] = make_float2(u.z, u.w);
   }
   __device__ static void store(Tin* p, const float (&f)[N]) {
     store4(p, make_float4(f[0], f[1], f[2], f[3]));
@@ -91,64 +99,74 @@ short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
   const int b = blockIdx.y;
   const int t0 = blockIdx.z * TT;
   const int t1 = min(T, t0 + TT);
-  float wk[K][N];
+  float2 wk[K][N / 2], bs[N / 2];
 #pragma unroll
-  for (int j = 0; j < K; ++j)
-#pragma unroll
-    for (int e = 0; e < N; e += 4) {
-      const float4 q = *reinterpret_cast<const float4*>(w + (size_t)j * C + c + e);
-      wk[j][e] = q.x; wk[j][e + 1] = q.y; wk[j][e + 2] = q.z; wk[j][e + 3] = q.w;
-    }
-  float bs[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) bs[e] = bias ? bias[c + e] : 0.f;
+  for (int j = 0; j < K; ++j) {
+    const float4 q = load4(w + (size_t)j * C + c);
+    wk[j][0] = make_float2(q.x, q.y);
+    wk[j][1] = make_float2(q.z, q.w);
+  }
+  const float4 bq = bias ? load4(bias + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  bs[0] = make_float2(bq.x, bq.y);
+  bs[1] = make_float2(bq.z, bq.w);
   const Tin* xb = x + (size_t)b * T * C + c;
   // win[j] = input at token t - (K - 1) + j for the next output t
-  float win[K > 1 ? K - 1 : 1][N];
+  float2 win[K > 1 ? K - 1 : 1][N / 2];
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) {
     const int tt = t0 - (K - 1) + j;
     if (tt >= 0) {
-      V::load(xb + (size_t)tt * C, win[j]);
+      V::get(V::load_raw(xb + (size_t)tt * C), win[j]);
     } else if (state_in) {
-      V::load(state_in + ((size_t)b * (K - 1) + (K - 1) + tt) * C + c, win[j]);
+      V::get(V::load_raw(state_in + ((size_t)b * (K - 1) + (K - 1) + tt) * C + c), win[j]);
     } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) win[j][e] = 0.f;
+      for (int e = 0; e < N / 2; ++e) win[j][e] = make_float2(0.f, 0.f);
     }
   }
-  for (int tb = t0; tb < t1; tb += kConvAhead) {
-    float cur[kConvAhead][N];   // loads of several tokens in flight together
+  typename V::Raw nxt[kConvAhead];   // loads of four tokens in flight under four others' work
+  auto fetch = [&](int tb) {
 #pragma unroll
     for (int i = 0; i < kConvAhead; ++i)
-      if (tb + i < t1) V::load(xb + (size_t)(tb + i) * C, cur[i]);
+      if (tb + i < t1) nxt[i] = V::load_raw(xb + (size_t)(tb + i) * C);
+  };
+  fetch(t0);
+  for (int tb = t0; tb < t1; tb += kConvAhead) {
+    float2 cur[kConvAhead][N / 2];
+#pragma unroll
+    for (int i = 0; i < kConvAhead; ++i) V::get(nxt[i], cur[i]);
+    fetch(tb + kConvAhead);
 #pragma unroll
     for (int i = 0; i < kConvAhead; ++i) {
       const int t = tb + i;
       if (t >= t1) break;
       float out[N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        float acc = wk[K - 1][e] * cur[i][e];
+      for (int e = 0; e < N / 2; ++e) {
+        float2 acc = mul2(wk[K - 1][e], cur[i][e]);
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) acc = fmaf(wk[j][e], win[j][e], acc);
-        if (bias) acc += bs[e];
-        out[e] = act ? silu_acc(acc) : acc;
+        for (int j = 0; j < K - 1; ++j) acc = fma2(wk[j][e], win[j][e], acc);
+        if (bias) acc = add2(acc, bs[e]);
+        out[2 * e] = act ? silu_acc(acc.x) : acc.x;
+        out[2 * e + 1] = act ? silu_acc(acc.y) : acc.y;
       }
       V::store(y + ((size_t)b * T + t) * C + c, out);
 #pragma unroll
       for (int j = 0; j + 1 < K - 1; ++j)
 #pragma unroll
-        for (int e = 0; e < N; ++e) win[j][e] = win[j + 1][e];
+        for (int e = 0; e < N / 2; ++e) win[j][e] = win[j + 1][e];
       if constexpr (K > 1) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) win[K - 2][e] = cur[i][e];
+        for (int e = 0; e < N / 2; ++e) win[K - 2][e] = cur[i][e];
       }
     }
   }
   if (state_out && blockIdx.z == gridDim.z - 1) {
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) V::store(state_out + ((size_t)b * (K - 1) + j) * C + c, win[j]);
+    for (int j = 0; j < K - 1; ++j) {
+      const float v[N] = {win[j][0].x, win[j][0].y, win[j][1].x, win[j][1].y};
+      V::store(state_out + ((size_t)b * (K - 1) + j) * C + c, v);
+    }
   }
 }
 

@@ -42,7 +42,7 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
   constexpr int BV = kTT * NL;                                      // vectors of B in a tile
   constexpr int BPT = (BV + kScanThreads - 1) / kScanThreads;       // per thread
   __shared__ __align__(16) float4 sDU[kTT][kScanCh];   // delta twice, delta x twice
-  __shared__ float sY[kLocal ? 1 : kTT][kScanCh + 8];  // padded: four tokens of eight channels
+  __shared__ __align__(16) float sY[kLocal ? 1 : kTT][kScanCh + 8];  // padded: four tokens of eight channels
   __shared__ __align__(16) float sB[kTT][NP], sC[kLocal ? 1 : kTT][NP];
 
   const int tid = threadIdx.x, lane = tid & 31;
@@ -116,8 +116,8 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
       dv[r].get(df);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float sig, d = df[e] + bias[e];
-        if (a.softplus) d = softplus_sig(d, sig);
+        float d = df[e] + bias[e];
+        if (a.softplus) d = softplus_fast(d);
         if (t0 + tl >= tend) d = 0.f;   // past the end: the state stays
         const float u = d * xf[e];
         sDU[tl][sc + e] = make_float4(d, d, u, u);
@@ -169,13 +169,15 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const int tl = sr + r * 16, t = t0 + tl;
-        float o[4], xf[4], zf[4];
+        float xf[4], zf[4];
+        const float4 yv = load4(&sY[tl][sc]);
+        float o[4] = {yv.x, yv.y, yv.z, yv.w};
         xs[r].get(xf);
         if (z) zs[r].get(zf);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          o[e] = fmaf(Dv[e], xf[e], sY[tl][sc + e]);
-          if (z) o[e] *= __fdividef(zf[e], 1.f + __expf(-zf[e]));
+          o[e] = fmaf(Dv[e], xf[e], o[e]);
+          if (z) o[e] *= zf[e] * fast_sigmoid(zf[e]);
         }
         if (t < tend) store_ch4(static_cast<T*>(a.y) + (row0 + t) * a.C + c0 + sc, sn, vec, o);
       }
@@ -247,8 +249,7 @@ scan_step_kernel(const ScanArgs a) {
   const float4 Cv = load4(static_cast<const T*>(a.Cm) + bc);
   const float x = to_f32(static_cast<const T*>(a.x)[row]);
   float d = to_f32(static_cast<const T*>(a.dt)[row]) + (a.dt_bias ? a.dt_bias[c] : 0.f);
-  float sig;
-  if (a.softplus) d = softplus_sig(d, sig);
+  if (a.softplus) d = softplus_fast(d);
   const float u = d * x, d2 = d * kLog2e;
   h.x = fmaf(ex2(d2 * A.x), h.x, u * B.x);
   h.y = fmaf(ex2(d2 * A.y), h.y, u * B.y);
@@ -262,7 +263,7 @@ scan_step_kernel(const ScanArgs a) {
     if (a.D) y = fmaf(a.D[c], x, y);
     if (a.z) {
       const float zv = to_f32(static_cast<const T*>(a.z)[row]);
-      y *= __fdividef(zv, 1.f + __expf(-zv));
+      y *= zv * fast_sigmoid(zv);
     }
     static_cast<T*>(a.y)[row] = from_f32<T>(y);
   }

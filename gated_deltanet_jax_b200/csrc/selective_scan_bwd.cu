@@ -156,7 +156,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, float* __rest
         kz[r][e] = 0.f;
         if (z) {
           const float zz = zv[e];
-          const float sz = __fdividef(1.f, 1.f + __expf(-zz));
+          const float sz = fast_sigmoid(zz);
           kz[r][e] = g * (sz * fmaf(zz, 1.f - sz, 1.f));
           g *= zz * sz;
         }

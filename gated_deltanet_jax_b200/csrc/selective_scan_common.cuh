@@ -10,27 +10,37 @@ constexpr int kScanThreads = 128;
 constexpr int kScanLanes = 4;                            // lanes of a channel
 constexpr int kScanCh = kScanThreads / kScanLanes;       // channels of a block
 
-// log(1 + e) for 0 <= e <= 1 as 2 atanh(e / (2 + e)): with s = e / (2 + e) <= 1/3
-// the series s + s^3 / 3 + ... + s^15 / 15 leaves less than s^17 / 17 / (1 - s^2) <
-// 2^-29 of it out.  No cancellation at small e, where step sizes lie.
-__device__ __forceinline__ float log1p_unit(float e) {
-  const float s = __fdividef(e, 2.f + e);
-  const float q = s * s;
-  float p = fmaf(q, 1.f / 15.f, 1.f / 13.f);
-  p = fmaf(q, p, 1.f / 11.f);
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, the logarithm as
+// 2 atanh(s) with s = e / (2 + e) <= 1/3: the series s + s^3 / 3 + ... + s^13 / 13
+// leaves less than s^15 / 15 / (1 - s^2) < 2^-27 of it out.  No cancellation at small
+// e, where step sizes lie.  A NaN stays one (through e).
+__device__ __forceinline__ float softplus_e(float v, float e) {
+  const float s = e * fast_rcp(2.f + e);
+  const float q = s * s, s2 = s + s;
+  float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
   p = fmaf(q, p, 1.f / 9.f);
   p = fmaf(q, p, 1.f / 7.f);
   p = fmaf(q, p, 1.f / 5.f);
   p = fmaf(q, p, 1.f / 3.f);
-  return 2.f * fmaf(q * p, s, s);
+  return fmaxf(v, 0.f) + fmaf(q * p, s2, s2);
 }
-
-// softplus(v) and, through `sig`, its derivative sigmoid(v).  A NaN stays one.
+__device__ __forceinline__ float softplus_fast(float v) {
+  return softplus_e(v, ex2(-fabsf(v) * kLog2e));
+}
+// The same and its derivative sigmoid(v).
 __device__ __forceinline__ float softplus_sig(float v, float& sig) {
-  const float e = expf(-fabsf(v));
-  const float r = __fdividef(1.f, 1.f + e);
+  const float e = ex2(-fabsf(v) * kLog2e);
+  const float r = fast_rcp(1.f + e);
   sig = v >= 0.f ? r : e * r;
-  return (v > 0.f ? v : (v == v ? 0.f : v)) + log1p_unit(e);
+  return softplus_e(v, e);
 }
 
 // One element, zero where `ok` is false.
@@ -97,23 +107,6 @@ __device__ __forceinline__ void store_ch4(T* p, int n, bool vec, const float (&v
   }
 }
 
-// Two fp32 operations an instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(r))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(r))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
-        "l"(reinterpret_cast<uint64_t&>(c)));
-  return r;
-}
-
 // Sums four tokens' values over the four lanes of a channel in three shuffles:
 // lane j (lane & 3) returns the sum of v[j].
 __device__ __forceinline__ float quad_sum4(float v0, float v1, float v2, float v3, int lane) {
@@ -126,14 +119,6 @@ __device__ __forceinline__ float quad_sum4(float v0, float v1, float v2, float v
   const float k = odd ? k1 : k0, g = odd ? k0 : k1;
   return k + __shfl_xor_sync(0xffffffffu, g, 1);
 }
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-constexpr float kLog2e = 1.4426950408889634f;
 
 // NL fp32 values to / from memory in 16-byte vectors where NL allows.
 template <int NL>

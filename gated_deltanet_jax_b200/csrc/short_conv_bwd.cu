@@ -23,21 +23,32 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kVec = 2;        // channels of a thread: a warp reads 128 bytes of bf16 a row
-constexpr int kAhead = 4;      // tokens whose loads are in flight together
+constexpr int kAhead = 4;      // tokens whose loads are in flight while four others are worked on
 
-__device__ __forceinline__ void ld(const float* p, float (&v)[kVec]) {
-  const float2 q = *reinterpret_cast<const float2*>(p);
-  v[0] = q.x; v[1] = q.y;
+// Two channels as they lie in memory.
+template <typename T>
+struct Raw2;
+template <>
+struct Raw2<float> {
+  float2 u;
+  __device__ __forceinline__ float2 get() const { return u; }
+};
+template <>
+struct Raw2<__nv_bfloat16> {
+  uint32_t u;
+  __device__ __forceinline__ float2 get() const {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+};
+template <typename T>
+__device__ __forceinline__ Raw2<T> ldr(const T* p) {
+  Raw2<T> r;
+  r.u = *reinterpret_cast<const decltype(r.u)*>(p);
+  return r;
 }
-__device__ __forceinline__ void ld(const __nv_bfloat16* p, float (&v)[kVec]) {
-  const float2 q = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
-  v[0] = q.x; v[1] = q.y;
-}
-__device__ __forceinline__ void st2(float* p, const float (&v)[kVec]) {
-  *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
-}
-__device__ __forceinline__ void st2(__nv_bfloat16* p, const float (&v)[kVec]) {
-  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v[0], v[1]);
+__device__ __forceinline__ void st2(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
+__device__ __forceinline__ void st2(__nv_bfloat16* p, float2 v) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
 }
 
 // Block (channel group, token tile, row b).  part [B * tiles][K + 1][C]: this
@@ -55,94 +66,89 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
   const int t0 = blockIdx.y * TT;
   const int t1 = min(T, t0 + TT);
   constexpr int W = K > 1 ? K - 1 : 1;
-  float wk[K][kVec], bs[kVec], win[W][kVec], dwin[W][kVec], dw[K][kVec], db[kVec];
+  const float2 zero = make_float2(0.f, 0.f), one = make_float2(1.f, 1.f);
+  float2 wk[K], win[W], dwin[W], dw[K], db = zero, bs = zero;
 #pragma unroll
-  for (int j = 0; j < K; ++j) ld(w + (size_t)j * C + c, wk[j]);
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    bs[e] = bias ? bias[c + e] : 0.f;
-    db[e] = 0.f;
-#pragma unroll
-    for (int j = 0; j < K; ++j) dw[j][e] = 0.f;
-#pragma unroll
-    for (int j = 0; j < W; ++j) dwin[j][e] = 0.f;
+  for (int j = 0; j < K; ++j) {
+    wk[j] = ldr(w + (size_t)j * C + c).get();
+    dw[j] = zero;
   }
+  if (bias) bs = ldr(bias + c).get();
+#pragma unroll
+  for (int j = 0; j < W; ++j) win[j] = dwin[j] = zero;
   const size_t row0 = (size_t)b * T;
   // win[j] = xe[t + j] for the next token t (the K - 1 inputs before it)
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) {
     const int tt = t0 - (K - 1) + j;
-    if (tt >= 0) {
-      ld(x + (row0 + tt) * C + c, win[j]);
-    } else if (state_in) {
-      ld(state_in + ((size_t)b * (K - 1) + (K - 1) + tt) * C + c, win[j]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) win[j][e] = 0.f;
-    }
+    if (tt >= 0)
+      win[j] = ldr(x + (row0 + tt) * C + c).get();
+    else if (state_in)
+      win[j] = ldr(state_in + ((size_t)b * (K - 1) + (K - 1) + tt) * C + c).get();
   }
   // Token t closes row s = t - (K - 1) of dxe: dxe[s] takes dpre[s .. t].
-  const int tend = t1 + K - 1;
-  for (int tb = t0; tb < tend; tb += kAhead) {
-    float xv[kAhead][kVec], gv[kAhead][kVec];
+  const int tend = t1 + K - 1, tload = min(T, tend);
+  Raw2<Tin> xr[kAhead], gr[kAhead];
+  auto fetch = [&](int tb) {
+    const Tin* xp = x + (row0 + tb) * C + c;
+    const Tin* gp = dy + (row0 + tb) * C + c;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int t = tb + i;
-      if (t < T && t < tend) {
-        ld(x + (row0 + t) * C + c, xv[i]);
-        ld(dy + (row0 + t) * C + c, gv[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) xv[i][e] = gv[i][e] = 0.f;
+      xr[i].u = {};
+      gr[i].u = {};
+      if (tb + i < tload) {
+        xr[i] = ldr(xp + (size_t)i * C);
+        gr[i] = ldr(gp + (size_t)i * C);
       }
     }
+  };
+  fetch(t0);
+  for (int tb = t0; tb < tend; tb += kAhead) {
+    float2 xv[kAhead], gv[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      xv[i] = xr[i].get();
+      gv[i] = gr[i].get();
+    }
+    if (tb + kAhead < tend) fetch(tb + kAhead);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int t = tb + i;
       if (t >= tend) break;
-      float dpre[kVec], out[kVec];
+      float2 pre = fma2(wk[K - 1], xv[i], bs);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        float pre = fmaf(wk[K - 1][e], xv[i][e], bs[e]);
+      for (int j = 0; j < K - 1; ++j) pre = fma2(wk[j], win[j], pre);
+      float2 d = gv[i];   // zero past the last token
+      if (act) {
+        const float2 sg = make_float2(fast_sigmoid(pre.x), fast_sigmoid(pre.y));
+        const float2 q = fma2(sg, make_float2(-1.f, -1.f), one);
+        d = mul2(mul2(d, sg), fma2(pre, q, one));
+      }
+      if (t < t1) {
+        db = add2(db, d);
+        dw[K - 1] = fma2(d, xv[i], dw[K - 1]);
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) pre = fmaf(wk[j][e], win[j][e], pre);
-        float d = gv[i][e];
-        if (act) {
-          const float sg = __fdividef(1.f, 1.f + __expf(-pre));
-          d *= sg * fmaf(pre, 1.f - sg, 1.f);
-        }
-        if (t >= T) d = 0.f;
-        dpre[e] = d;
-        if (t < t1) {
-          db[e] += d;
-          dw[K - 1][e] = fmaf(d, xv[i][e], dw[K - 1][e]);
+        for (int j = 0; j < K - 1; ++j) dw[j] = fma2(d, win[j], dw[j]);
+      }
+      // dxe[s] = w[0] dpre[t] + w[1] dpre[t - 1] + ...
+      float2 out = mul2(wk[0], d);
 #pragma unroll
-          for (int j = 0; j < K - 1; ++j) dw[j][e] = fmaf(d, win[j][e], dw[j][e]);
-        }
-        // dxe[s] = w[0] dpre[t] + w[1] dpre[t - 1] + ...
-        float acc = wk[0][e] * d;
+      for (int j = 1; j < K; ++j) out = fma2(wk[j], dwin[K - 1 - j], out);
 #pragma unroll
-        for (int j = 1; j < K; ++j) acc = fmaf(wk[j][e], dwin[K - 1 - j][e], acc);
-        out[e] = acc;
-#pragma unroll
-        for (int j = 0; j + 1 < K - 1; ++j) {
-          win[j][e] = win[j + 1][e];
-          dwin[j][e] = dwin[j + 1][e];
-        }
-        if constexpr (K > 1) {
-          win[K - 2][e] = xv[i][e];
-          dwin[K - 2][e] = dpre[e];
-        }
+      for (int j = 0; j + 1 < K - 1; ++j) {
+        win[j] = win[j + 1];
+        dwin[j] = dwin[j + 1];
+      }
+      if constexpr (K > 1) {
+        win[K - 2] = xv[i];
+        dwin[K - 2] = d;
       }
       const int s = t - (K - 1);
       if (s < t0 && blockIdx.y != 0) continue;
       // the final window's rows are the inputs s = T - (K - 1) .. T - 1
-      if (dstate_out && s >= T - (K - 1)) {
-        float g[kVec];
-        ld(dstate_out + ((size_t)b * (K - 1) + (s - (T - (K - 1)))) * C + c, g);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) out[e] += g[e];
-      }
+      if (dstate_out && s >= T - (K - 1))
+        out = add2(out, ldr(dstate_out + ((size_t)b * (K - 1) + (s - (T - (K - 1)))) * C + c)
+                            .get());
       if (s >= 0)
         st2(dx + (row0 + s) * C + c, out);
       else if (dstate_in)
