@@ -28,22 +28,25 @@ namespace gdn {
 
 namespace {
 
-constexpr int kTT = 32;   // tokens of a tile
-constexpr int kRows = kTT * kScanCh / (kScanThreads * 4);   // staging rows per thread
+constexpr int kFwdThreads = 64;       // 16 slots of four lanes, two channels a lane
+constexpr int kTT = 32;               // tokens of a tile
+constexpr int kSRows = kFwdThreads / 8;                     // rows staged side by side
+constexpr int kRows = kTT / kSRows;                         // staging rows per thread
 
 // kLocal: the first pass of a cut row (from zero; the end state and the steps'
 // sum out, no y).  chunk / nchunk: tokens of a chunk and their number (grid z).
 template <typename T, int NL, bool kLocal>
-__global__ void __launch_bounds__(kScanThreads, NL > 8 ? 2 : NL > 4 ? 4 : sizeof(T) == 2 ? 7 : 6)
+__global__ void __launch_bounds__(kFwdThreads, NL > 8 ? 4 : 7)
 scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int nchunk) {
   constexpr int NP = NL * kScanLanes;
   constexpr int P = scan_pairs<NL>();
   constexpr int CK = scan_tile<NL>();
-  constexpr int BV = kTT * NL;                                      // vectors of B in a tile
-  constexpr int BPT = (BV + kScanThreads - 1) / kScanThreads;       // per thread
-  __shared__ __align__(16) float4 sDU[kTT][kScanCh];   // delta twice, delta x twice
-  __shared__ __align__(16) float sY[kLocal ? 1 : kTT][kScanCh + 8];  // padded: four tokens of eight channels
+  constexpr int BV = kTT * NL;                                    // vectors of B in a tile
+  constexpr int BPT = (BV + kFwdThreads - 1) / kFwdThreads;       // per thread
+  __shared__ __align__(16) float2 sDU[kTT][kScanCh];              // delta, delta x
+  __shared__ __align__(16) float sY[kLocal ? 1 : kTT][kScanCh + 8];
   __shared__ __align__(16) float sB[kTT][NP], sC[kLocal ? 1 : kTT][NP];
+  __shared__ __align__(16) float sPar[2][kScanCh];                // dt_bias, D
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int Cg = a.C / a.G;
@@ -60,45 +63,46 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
   const T* Cp = static_cast<const T*>(a.Cm) + ((size_t)b * a.T * a.G + grp) * a.N;
   const bool vecn = a.N % 4 == 0;
 
-  // the lane's channel and states
-  const int chl = tid / kScanLanes, q = tid % kScanLanes;
-  const bool chan = chl < nch;
+  // the lane's channels chl, chl + 1 and its quarter of their states
+  const int chl = tid / kScanLanes * 2, q = tid % kScanLanes;
   const size_t row = (size_t)b * a.C + c0 + chl;
-  const size_t st = row * a.N + q * NL;
   float* slot = a.chunk_state + (((size_t)kc * a.B + b) * a.C + c0 + chl) * NP + q * NL;
-  float2 A2[P], h[P];
+  float2 A2[2][P], h[2][P];
 #pragma unroll
-  for (int i = 0; i < 2 * P; ++i) {
-    const bool ok = chan && i < NL && q * NL + i < a.N;
-    pair_at(A2[i / 2], i & 1) = ok ? a.A[(size_t)(c0 + chl) * a.N + q * NL + i] * kLog2e : 0.f;
-    pair_at(h[i / 2], i & 1) = !kLocal && nchunk == 1 && ok && a.h0 ? a.h0[st + i] : 0.f;
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int i = 0; i < 2 * P; ++i) {
+      const bool ok = chl + c < nch && i < NL && q * NL + i < a.N;
+      pair_at(A2[c][i / 2], i & 1) =
+          ok ? a.A[(size_t)(c0 + chl + c) * a.N + q * NL + i] * kLog2e : 0.f;
+      pair_at(h[c][i / 2], i & 1) =
+          !kLocal && nchunk == 1 && ok && a.h0 ? a.h0[(row + c) * a.N + q * NL + i] : 0.f;
+    }
+    if (!kLocal && nchunk > 1 && chl + c < nch) load_pairs<NL>(slot + c * NP, h[c]);
   }
-  if (!kLocal && nchunk > 1 && chan) load_pairs<NL>(slot, h);
-  // the staging role: channels sc .. sc + 3 of rows sr, sr + 16
+  // the staging role: channels sc .. sc + 3 of rows sr, sr + kSRows, ...
   const int sc = tid % 8 * 4, sr = tid / 8;
   const int sn = nch - sc;
-  float bias[4], Dv[4], dsum[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    bias[e] = a.dt_bias && e < sn ? a.dt_bias[c0 + sc + e] : 0.f;
-    Dv[e] = !kLocal && a.D && e < sn ? a.D[c0 + sc + e] : 0.f;
-    dsum[e] = 0.f;
+  if (tid < kScanCh) {
+    sPar[0][tid] = a.dt_bias && tid < nch ? a.dt_bias[c0 + tid] : 0.f;
+    sPar[1][tid] = !kLocal && a.D && tid < nch ? a.D[c0 + tid] : 0.f;
   }
+  __syncthreads();
+  float dsum[4] = {0.f, 0.f, 0.f, 0.f};
   const size_t row0 = (size_t)b * a.T;
   Raw4<T> xv[kRows], dv[kRows], zv[kRows], bv[BPT], cv[BPT];
   auto fetch = [&](int t0) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int t = t0 + sr + r * 16;
+      const int t = t0 + sr + r * kSRows;
       const int n = t < tend ? sn : 0;
       const size_t off = (row0 + t) * a.C + c0 + sc;
       xv[r].load(x + off, n, vec);
       dv[r].load(dt + off, n, vec);
-      if (z) zv[r].load(z + off, n, vec);
     }
 #pragma unroll
     for (int r = 0; r < BPT; ++r) {
-      const int i = tid + r * kScanThreads, t = t0 + i / NL, n0 = i % NL * 4;
+      const int i = tid + r * kFwdThreads, t = t0 + i / NL, n0 = i % NL * 4;
       const int n = i < BV && t < tend ? a.N - n0 : 0;
       const size_t off = (size_t)t * a.G * a.N + n0;
       bv[r].load(Bp + off, n, vecn);
@@ -107,28 +111,30 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
   };
   fetch(tbeg);
   for (int t0 = tbeg; t0 < tend; t0 += kTT) {
-    Raw4<T> xs[kRows], zs[kRows];
+    const float4 bias4 = load4(&sPar[0][sc]), D4 = load4(&sPar[1][sc]);
+    const float bias[4] = {bias4.x, bias4.y, bias4.z, bias4.w};
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int tl = sr + r * 16;
-      float xf[4], df[4];
+      const int tl = sr + r * kSRows;
+      float xf[4], d[4];
       xv[r].get(xf);
-      dv[r].get(df);
+      dv[r].get(d);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float d = df[e] + bias[e];
-        if (a.softplus) d = softplus_fast(d);
-        if (t0 + tl >= tend) d = 0.f;   // past the end: the state stays
-        const float u = d * xf[e];
-        sDU[tl][sc + e] = make_float4(d, d, u, u);
-        if (kLocal) dsum[e] += d;
+        d[e] += bias[e];
+        if (a.softplus) d[e] = softplus_fast(d[e]);
+        if (t0 + tl >= tend) d[e] = 0.f;   // past the end: the state stays
+        if (kLocal) dsum[e] += d[e];
       }
-      xs[r] = xv[r];
-      if (z) zs[r] = zv[r];
+      float* du = reinterpret_cast<float*>(&sDU[tl][sc]);
+      store4(du, make_float4(d[0], d[0] * xf[0], d[1], d[1] * xf[1]));
+      store4(du + 4, make_float4(d[2], d[2] * xf[2], d[3], d[3] * xf[3]));
+      if (!kLocal)
+        store4(&sY[tl][sc], make_float4(D4.x * xf[0], D4.y * xf[1], D4.z * xf[2], D4.w * xf[3]));
     }
 #pragma unroll
     for (int r = 0; r < BPT; ++r) {
-      const int i = tid + r * kScanThreads;
+      const int i = tid + r * kFwdThreads;
       if (i < BV) {
         float v[4];
         bv[r].get(v);
@@ -140,51 +146,72 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
       }
     }
     __syncthreads();
+    if (z) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int t = t0 + sr + r * kSRows;
+        zv[r].load(z + (row0 + t) * a.C + c0 + sc, t < tend ? sn : 0, vec);
+      }
+    }
     if (t0 + kTT < tend) fetch(t0 + kTT);
 #pragma unroll 1
     for (int g = 0; g < kTT; g += 4) {
-      if (!kLocal && a.ckpt && g % CK == 0 && t0 + g < a.T && chan)
-        store_pairs<NL>(
-            a.ckpt + (((size_t)b * a.nck + (t0 + g) / CK) * a.C + c0 + chl) * NP + q * NL, h);
-      float ys[4];
+      if (!kLocal && a.ckpt && g % CK == 0 && t0 + g < a.T) {
+        float* ck = a.ckpt + (((size_t)b * a.nck + (t0 + g) / CK) * a.C + c0 + chl) * NP + q * NL;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (chl + c < nch) store_pairs<NL>(ck + c * NP, h[c]);
+      }
+      float ys[2][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float4 du = sDU[g + j][chl];
-        const float2 d2 = make_float2(du.x, du.y), u2 = make_float2(du.z, du.w);
-        float2 B2[P], C2[P], acc = make_float2(0.f, 0.f);
+        const float4 du = load4(reinterpret_cast<const float*>(&sDU[g + j][chl]));
+        float2 B2[P], C2[P];
         load_pairs<NL>(&sB[g + j][q * NL], B2);
         if (!kLocal) load_pairs<NL>(&sC[g + j][q * NL], C2);
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const float2 e = mul2(d2, A2[i]);
-          h[i] = fma2(make_float2(ex2(e.x), ex2(e.y)), h[i], mul2(u2, B2[i]));
-          if (!kLocal) acc = fma2(C2[i], h[i], acc);
+        for (int c = 0; c < 2; ++c) {
+          const float2 d2 = c ? make_float2(du.z, du.z) : make_float2(du.x, du.x);
+          const float2 u2 = c ? make_float2(du.w, du.w) : make_float2(du.y, du.y);
+          float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const float2 e = mul2(d2, A2[c][i]);
+            h[c][i] = fma2(make_float2(ex2(e.x), ex2(e.y)), h[c][i], mul2(u2, B2[i]));
+            if (!kLocal) acc = i ? fma2(C2[i], h[c][i], acc) : mul2(C2[i], h[c][i]);
+          }
+          ys[c][j] = acc.x + acc.y;
         }
-        ys[j] = acc.x + acc.y;
       }
-      if (!kLocal) sY[g + q][chl] = quad_sum4(ys[0], ys[1], ys[2], ys[3], lane);
+      if (!kLocal) {
+        float2* yp = reinterpret_cast<float2*>(&sY[g + q][chl]);
+        float2 v = *yp;
+        v.x += quad_sum4(ys[0][0], ys[0][1], ys[0][2], ys[0][3], lane);
+        v.y += quad_sum4(ys[1][0], ys[1][1], ys[1][2], ys[1][3], lane);
+        *yp = v;
+      }
     }
     __syncthreads();
     if (!kLocal) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        const int tl = sr + r * 16, t = t0 + tl;
-        float xf[4], zf[4];
+        const int tl = sr + r * kSRows, t = t0 + tl;
         const float4 yv = load4(&sY[tl][sc]);
         float o[4] = {yv.x, yv.y, yv.z, yv.w};
-        xs[r].get(xf);
-        if (z) zs[r].get(zf);
+        if (z) {
+          float zf[4];
+          zv[r].get(zf);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[e] = fmaf(Dv[e], xf[e], o[e]);
-          if (z) o[e] *= zf[e] * fast_sigmoid(zf[e]);
+          for (int e = 0; e < 4; ++e) o[e] *= zf[e] * fast_sigmoid(zf[e]);
         }
         if (t < tend) store_ch4(static_cast<T*>(a.y) + (row0 + t) * a.C + c0 + sc, sn, vec, o);
       }
     }
   }
   if (kLocal) {
-    if (chan) store_pairs<NL>(slot, h);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (chl + c < nch) store_pairs<NL>(slot + c * NP, h[c]);
     // the staging rows' sums of delta, added up in a fixed order
     float* red = reinterpret_cast<float*>(sDU);
 #pragma unroll
@@ -192,13 +219,16 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
     __syncthreads();
     if (tid < nch) {
       float s = 0.f;
-      for (int r = 0; r < 16; ++r) s += red[r * kScanCh + tid];
+      for (int r = 0; r < kSRows; ++r) s += red[r * kScanCh + tid];
       a.chunk_sum[((size_t)kc * a.B + b) * a.C + c0 + tid] = s;
     }
-  } else if (a.hT && chan && kc == nchunk - 1) {
+  } else if (a.hT && kc == nchunk - 1) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
-      if (q * NL + i < a.N) a.hT[st + i] = pair_at(h[i / 2], i & 1);
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+        if (chl + c < nch && q * NL + i < a.N)
+          a.hT[(row + c) * a.N + q * NL + i] = pair_at(h[c][i / 2], i & 1);
   }
 }
 
@@ -280,13 +310,13 @@ template <typename T, int NL>
 cudaError_t launch_fwd(const ScanArgs& a, int tpg, int vec, const ScanSplit& sp, cudaStream_t st) {
   const dim3 grid((unsigned)(tpg * a.G), a.B, sp.chunks);
   if (sp.chunks > 1) {
-    scan_fwd_kernel<T, NL, true><<<dim3(grid.x, grid.y, sp.chunks - 1), kScanThreads, 0, st>>>(
+    scan_fwd_kernel<T, NL, true><<<dim3(grid.x, grid.y, sp.chunks - 1), kFwdThreads, 0, st>>>(
         a, tpg, vec, sp.tokens, sp.chunks);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = launch_scan_chain(a, a.h0, sp.chunks, false, st);
     if (e != cudaSuccess) return e;
   }
-  scan_fwd_kernel<T, NL, false><<<grid, kScanThreads, 0, st>>>(a, tpg, vec, sp.tokens, sp.chunks);
+  scan_fwd_kernel<T, NL, false><<<grid, kFwdThreads, 0, st>>>(a, tpg, vec, sp.tokens, sp.chunks);
   return cudaGetLastError();
 }
 
