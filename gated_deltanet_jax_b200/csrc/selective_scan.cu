@@ -346,12 +346,12 @@ cudaError_t fwd_dispatch(const ScanArgs& a, cudaStream_t st) {
 }  // namespace
 
 // How a row is cut: blocks of the whole rows against those that fill the SMs
-// (seven of the forward's, three of the backward's fit one).
+// (seven of the forward's, six of the backward's fit one).
 ScanSplit scan_split(int B, int T, int C, int G, bool backward) {
   const long long blocks = (long long)((C / G + kScanCh - 1) / kScanCh) * G * B;
-  const long long fill = 148LL * (backward ? 3 : 7);
+  const long long fill = 148LL * (backward ? 6 : 7);
   ScanSplit s{1, T};
-  if (blocks > 148 || blocks <= 0) return s;
+  if (blocks > fill / 3 || blocks <= 0 || T <= 0) return s;
   const long long want = fill / blocks;
   long long tokens = (T + want - 1) / want;
   if (tokens < 128) tokens = 128;   // a chunk's launch and chaining against its walk

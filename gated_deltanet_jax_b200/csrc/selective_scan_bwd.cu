@@ -6,16 +6,18 @@
 //   ddelta_t = sum_n r a_t h_{t-1} A + x_t sum_n r B,    ddt = ddelta sigmoid(dt + bias),
 //   dA[n]    = sum_t r delta a_t h_{t-1},   dD = sum dyp x,   dz = dy ypre silu'(z).
 //
-// A block owns 32 channels of one row, four lanes a channel as in the forward,
-// and walks its tiles backwards.  A tile restarts from the state that the
-// forward kept at its first token (one fp32 state every 16 tokens at N <= 16:
-// four bytes a token and channel, less time than forming it again), runs the
-// recurrence over the tile with the decay factors in registers and the states
-// in shared memory, then the adjoint recurrence backwards.  Bound by issue
-// slots: about a dozen multiply-adds a state and token, and seven shuffles a
-// token that sum dB and dC over a warp's eight channels.  Sums over channels,
-// rows and tokens leave as one partial per block and are added up in a fixed
-// order by further kernels: no atomics, the same bits on every run.
+// A block owns 32 channels of one row, four lanes and two channels a lane as in
+// the forward, and walks its tiles backwards.  A tile restarts from the state
+// that the forward kept at its first token (one fp32 state every 16 tokens at
+// N <= 16: four bytes a token and channel, less time than forming it again).  Its
+// halves take turns, the later one first: the recurrence runs over the half with
+// the states in registers, then the adjoint recurrence backwards.  Rows that
+// leave most SMs idle are cut as in the forward, the chunks' adjoint states
+// chained from the end.  Bound by issue slots and exponentials: two to three
+// exponentials and about a dozen multiply-adds a state and token, and seven
+// shuffles a token that sum dB and dC over a warp's 16 channels.  Sums over
+// channels, rows and tokens leave as one partial per block and are added up in a
+// fixed order by further kernels: no atomics, the same bits on every run.
 #include "selective_scan_common.cuh"
 
 namespace gdn {
@@ -59,29 +61,40 @@ struct ChanSum {
   }
 };
 
-template <int NL>
-struct BwdSmem {
-  static constexpr int CK = scan_tile<NL>();
-  static constexpr int NP = NL * kScanLanes;
-  float h[CK][kScanThreads][NL];          // states after each token of the tile
-  float4 p[CK][kScanCh];                  // delta, delta x, dyp, x
-  float o[3][CK][kScanCh + 8];            // sum C h, sum r B, sum r a h A
-  float B[CK][NP];
-  float C[CK][NP];
-  float red[kScanThreads / 32][CK][2 * NP];   // a warp's dB and dC
-};
+#ifndef EXR
+#define EXR ex2_again
+#endif
+#ifndef MINB
+#define MINB 6
+#endif
+#ifndef KEEPDEC
+#define KEEPDEC 0
+#endif
+constexpr bool kKeepDec = KEEPDEC;
+constexpr int kBwdThreads = 64;   // 16 slots of four lanes, two channels a lane
+constexpr int kBwdWarps = kBwdThreads / 32;
 
-template <typename T, int NL>
-__global__ void __launch_bounds__(kScanThreads)
-scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, float* __restrict__ pBC,
-                float* __restrict__ pA, float* __restrict__ pD) {
-  using S = BwdSmem<NL>;
-  constexpr int CK = S::CK, NP = S::NP;
-  constexpr int RPT = CK * kScanCh / (kScanThreads * 4);    // staging rows per thread
-  constexpr int ROWS = RPT > 0 ? RPT : 1;
-  constexpr int RT = CK < 16 ? CK : 16;                     // rows of one staging pass
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  S& s = *reinterpret_cast<S*>(smem_raw);
+// kLocal: the first pass of a cut row (chunks 1 ..: the adjoint from zero over
+// the chunk and the steps' sum out, no gradients).
+template <typename T, int NL, bool kLocal>
+__global__ void __launch_bounds__(kBwdThreads, NL <= 4 ? MINB : 4)
+scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, int nchunk,
+                float* __restrict__ pBC, float* __restrict__ pA, float* __restrict__ pD) {
+  constexpr int CK = scan_tile<NL>(), SUB = CK / 2;
+  constexpr int NP = NL * kScanLanes;
+  constexpr int P = scan_pairs<NL>();
+  constexpr int RT = CK < kBwdThreads / 8 ? CK : kBwdThreads / 8;   // rows staged side by side
+  constexpr int ROWS = CK / RT;
+  constexpr int BV = CK * NL, BPT = (BV + kBwdThreads - 1) / kBwdThreads;
+  __shared__ __align__(16) float2 sDU[CK][kScanCh];       // delta, delta x
+  __shared__ __align__(16) float sG[CK][kScanCh];         // dyp
+  __shared__ __align__(16) float sB[CK][NP], sC[CK][NP];
+  __shared__ __align__(16) float sPar[2][kScanCh];        // dt_bias, D
+  // x, sigmoid(dt + bias), dy silu'(z); sum C h, sum r B, sum r a h A; a warp's dB and dC
+  __shared__ __align__(16) float sK[kLocal ? 1 : 3][CK][kScanCh];
+  __shared__ __align__(16) float sO[kLocal ? 1 : 3][CK][kScanCh + 8];
+  __shared__ __align__(16) float sRed[kLocal ? 1 : kBwdWarps][CK][2 * NP];
+  __shared__ __align__(16) float sSum[2][kBwdThreads / 8][kScanCh];
 
   const ScanArgs& f = a.fwd;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -90,227 +103,337 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, float* __rest
   const int cl0 = (blockIdx.x % tiles_per_group) * kScanCh;
   const int nch = min(kScanCh, Cg - cl0);
   const int c0 = grp * Cg + cl0;
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, kc = blockIdx.z + (kLocal ? 1 : 0);
+  const int tbeg = kc * chunk, tend = min(f.T, tbeg + chunk);
   const T* x = static_cast<const T*>(f.x);
   const T* dt = static_cast<const T*>(f.dt);
   const T* z = static_cast<const T*>(f.z);
   const T* dy = static_cast<const T*>(a.dy);
   const T* Bp = static_cast<const T*>(f.Bm) + ((size_t)b * f.T * f.G + grp) * f.N;
   const T* Cp = static_cast<const T*>(f.Cm) + ((size_t)b * f.T * f.G + grp) * f.N;
+  const bool vecn = f.N % 4 == 0;
 
-  const int chl = tid / kScanLanes, q = tid % kScanLanes;
-  const bool chan = chl < nch;
-  float A2[NL], ar[NL], dA[NL];
-  const size_t st = ((size_t)b * f.C + c0 + chl) * f.N + q * NL;
+  const int chl = tid / kScanLanes * 2, q = tid % kScanLanes;
+  const size_t row = (size_t)b * f.C + c0 + chl;
+  float* slot = f.chunk_state + (((size_t)kc * f.B + b) * f.C + c0 + chl) * NP + q * NL;
+  float2 A2[2][P], ar[2][P], dA[2][P];
 #pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const bool ok = chan && q * NL + i < f.N;
-    A2[i] = ok ? f.A[(size_t)(c0 + chl) * f.N + q * NL + i] * kLog2e : 0.f;
-    ar[i] = ok && a.dhT ? a.dhT[st + i] : 0.f;
-    dA[i] = 0.f;
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int i = 0; i < 2 * P; ++i) {
+      const bool ok = chl + c < nch && i < NL && q * NL + i < f.N;
+      pair_at(A2[c][i / 2], i & 1) =
+          ok ? f.A[(size_t)(c0 + chl + c) * f.N + q * NL + i] * kLog2e : 0.f;
+      pair_at(ar[c][i / 2], i & 1) =
+          !kLocal && nchunk == 1 && ok && a.dhT ? a.dhT[(row + c) * f.N + q * NL + i] : 0.f;
+      pair_at(dA[c][i / 2], i & 1) = 0.f;
+    }
+    if (!kLocal && nchunk > 1 && chl + c < nch) load_pairs<NL>(slot + c * NP, ar[c]);
   }
   const int sc = tid % 8 * 4, sr = tid / 8;
-  const bool stages = sr < CK;
-  const int sn = nch - sc;
-  float bias[4], Dv[4], accD[4], accB[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    bias[e] = f.dt_bias && e < sn ? f.dt_bias[c0 + sc + e] : 0.f;
-    Dv[e] = f.D && e < sn ? f.D[c0 + sc + e] : 0.f;
-    accD[e] = accB[e] = 0.f;
+  const bool stages = sr < RT;
+  const int sn = stages ? nch - sc : 0;
+  if (tid < kScanCh) {
+    sPar[0][tid] = f.dt_bias && tid < nch ? f.dt_bias[c0 + tid] : 0.f;
+    sPar[1][tid] = f.D && tid < nch ? f.D[c0 + tid] : 0.f;
   }
+  __syncthreads();
+  float accD[4] = {0.f, 0.f, 0.f, 0.f}, accB[4] = {0.f, 0.f, 0.f, 0.f};
   const size_t row0 = (size_t)b * f.T;
-  const int ntiles = (f.T + CK - 1) / CK;
-  Raw4<T> xr[ROWS], dr[ROWS], zr[ROWS], gr[ROWS];
+  Raw4<T> xr[ROWS], dr[ROWS], zr[ROWS], gr[ROWS], bv[BPT], cv[BPT];
   auto fetch = [&](int t0) {
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       const int t = t0 + sr + r * RT;
-      const int n = stages && t < f.T ? sn : 0;
+      const int n = t < tend ? sn : 0;
       const size_t off = (row0 + t) * f.C + c0 + sc;
-      xr[r].load(x + off, n, vec);
+      if (!kLocal) xr[r].load(x + off, n, vec);
       dr[r].load(dt + off, n, vec);
       gr[r].load(dy + off, n, vec);
       if (z) zr[r].load(z + off, n, vec);
     }
+#pragma unroll
+    for (int r = 0; r < BPT; ++r) {
+      const int i = tid + r * kBwdThreads, t = t0 + i / NL, n0 = i % NL * 4;
+      const int n = i < BV && t < tend ? f.N - n0 : 0;
+      const size_t off = (size_t)t * f.G * f.N + n0;
+      if (!kLocal) bv[r].load(Bp + off, n, vecn);
+      cv[r].load(Cp + off, n, vecn);
+    }
   };
-  if (ntiles > 0) fetch((ntiles - 1) * CK);
+  const int ntiles = (tend - tbeg + CK - 1) / CK;
+  if (ntiles > 0) fetch(tbeg + (ntiles - 1) * CK);
   for (int k = ntiles - 1; k >= 0; --k) {
-    const int t0 = k * CK;
-    // kept for the tile's last step: sigmoid(dt + bias), dy silu'(z), delta, dyp, x
-    float ks[ROWS][4], kz[ROWS][4];
+    const int t0 = tbeg + k * CK;
+    if (stages) {
+      const float4 b4 = load4(&sPar[0][sc]);
+      const float bias[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      const int tl = sr + r * RT;
-      float xv[4], dv[4], gv[4], zv[4];
-      xr[r].get(xv);
-      dr[r].get(dv);
-      gr[r].get(gv);
-      if (z) zr[r].get(zv);
+      for (int r = 0; r < ROWS; ++r) {
+        const int tl = sr + r * RT;
+        float xv[4] = {0.f, 0.f, 0.f, 0.f}, d[4], g[4], sg[4], kz[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!kLocal) xr[r].get(xv);
+        dr[r].get(d);
+        gr[r].get(g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float sig = 1.f, d = dv[e] + bias[e];
-        if (f.softplus) d = softplus_sig(d, sig);
-        if (t0 + tl >= f.T) d = 0.f;
-        float g = gv[e];
-        kz[r][e] = 0.f;
-        if (z) {
-          const float zz = zv[e];
-          const float sz = fast_sigmoid(zz);
-          kz[r][e] = g * (sz * fmaf(zz, 1.f - sz, 1.f));
-          g *= zz * sz;
+        for (int e = 0; e < 4; ++e) {
+          d[e] += bias[e];
+          sg[e] = 1.f;
+          if (f.softplus) d[e] = softplus_sig(d[e], sg[e]);
+          if (t0 + tl >= tend) d[e] = 0.f;
+          if (kLocal) accD[e] += d[e];
         }
-        ks[r][e] = sig;
-        if (stages) s.p[tl][sc + e] = make_float4(d, d * xv[e], g, xv[e]);
+        if (z) {
+          float zz[4];
+          zr[r].get(zz);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float sz = fast_sigmoid(zz[e]);
+            kz[e] = g[e] * (sz * fmaf(zz[e], 1.f - sz, 1.f));
+            g[e] *= zz[e] * sz;
+          }
+        }
+        float* du = reinterpret_cast<float*>(&sDU[tl][sc]);
+        store4(du, make_float4(d[0], d[0] * xv[0], d[1], d[1] * xv[1]));
+        store4(du + 4, make_float4(d[2], d[2] * xv[2], d[3], d[3] * xv[3]));
+        store4(&sG[tl][sc], make_float4(g[0], g[1], g[2], g[3]));
+        if (!kLocal) {
+          store4(&sK[0][tl][sc], make_float4(xv[0], xv[1], xv[2], xv[3]));
+          store4(&sK[1][tl][sc], make_float4(sg[0], sg[1], sg[2], sg[3]));
+          if (z) store4(&sK[2][tl][sc], make_float4(kz[0], kz[1], kz[2], kz[3]));
+        }
       }
     }
-    for (int i = tid; i < CK * NP; i += kScanThreads) {
-      const int tl = i / NP, n = i % NP;
-      const bool ok = t0 + tl < f.T && n < f.N;
-      const size_t off = (size_t)(t0 + tl) * f.G * f.N + n;
-      s.B[tl][n] = load1(Bp + off, ok);
-      s.C[tl][n] = load1(Cp + off, ok);
-    }
-    float h0[NL];
-    if (chan) {
-      load_states(f.ckpt + (((size_t)b * f.nck + k) * f.C + c0 + chl) * NP + q * NL, h0);
-    } else {
 #pragma unroll
-      for (int i = 0; i < NL; ++i) h0[i] = 0.f;
+    for (int r = 0; r < BPT; ++r) {
+      const int i = tid + r * kBwdThreads;
+      if (i < BV) {
+        float v[4];
+        cv[r].get(v);
+        store4(&sC[i / NL][i % NL * 4], make_float4(v[0], v[1], v[2], v[3]));
+        if (!kLocal) {
+          bv[r].get(v);
+          store4(&sB[i / NL][i % NL * 4], make_float4(v[0], v[1], v[2], v[3]));
+        }
+      }
     }
     __syncthreads();
-    if (k > 0) fetch((k - 1) * CK);
-
-    // the recurrence over the tile
-    float dec[CK][NL], h[NL];
+    if (k > 0) fetch(t0 - CK);
+    if (kLocal) {
+#pragma unroll 4
+      for (int t = CK - 1; t >= 0; --t) {
+        const float4 du = load4(reinterpret_cast<const float*>(&sDU[t][chl]));
+        const float2 g = *reinterpret_cast<const float2*>(&sG[t][chl]);
+        float2 C2[P];
+        load_pairs<NL>(&sC[t][q * NL], C2);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) h[i] = h0[i];
+        for (int c = 0; c < 2; ++c) {
+          const float dd = c ? du.z : du.x, gg = c ? g.y : g.x;
 #pragma unroll
-    for (int g = 0; g < CK; g += 4) {
-      float ys[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 p = s.p[g + j][chl];
-        float acc = 0.f;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          dec[g + j][i] = ex2(p.x * A2[i]);
-          h[i] = fmaf(dec[g + j][i], h[i], p.y * s.B[g + j][q * NL + i]);
-          acc = fmaf(s.C[g + j][q * NL + i], h[i], acc);
+          for (int i = 0; i < P; ++i) {
+            const float2 e = mul2(make_float2(dd, dd), A2[c][i]);
+            ar[c][i] = mul2(make_float2(ex2(e.x), ex2(e.y)),
+                            fma2(C2[i], make_float2(gg, gg), ar[c][i]));
+          }
         }
-        ys[j] = acc;
-        store_states(s.h[g + j][tid], h);
       }
-      if (z) s.o[0][g + q][chl] = quad_sum4(ys[0], ys[1], ys[2], ys[3], lane);
+      __syncthreads();
+      continue;
     }
-    // the adjoint recurrence, backwards; h holds h_t and becomes h_{t-1}
+    // Halves of the tile, the later one first, each with its states in registers.
+    const float* ck = f.ckpt + (((size_t)b * f.nck + t0 / CK) * f.C + c0 + chl) * NP + q * NL;
+#pragma unroll 1
+    for (int hf = 1; hf >= 0; --hf) {
+      float2 hs[2][P], h[SUB][2][P];
+      float2 dec[kKeepDec ? SUB : 1][2][P];
 #pragma unroll
-    for (int g = CK - 4; g >= 0; g -= 4) {
-      float rb[4], fa[4];
+      for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        const int t = g + j;
-        const float4 p = s.p[t][chl];
-        float hp[NL];
-        if (t > 0) {
-          load_states(s.h[t > 0 ? t - 1 : 0][tid], hp);
-        } else {
+        for (int i = 0; i < P; ++i) hs[c][i] = make_float2(0.f, 0.f);
+        if (chl + c < nch) load_pairs<NL>(ck + c * NP, hs[c]);
+      }
+      auto advance = [&](int t, float2 (&s)[2][P], float2 (&dk)[2][P]) {
+        const float4 du = load4(reinterpret_cast<const float*>(&sDU[t][chl]));
+        float2 B2[P];
+        load_pairs<NL>(&sB[t][q * NL], B2);
 #pragma unroll
-          for (int i = 0; i < NL; ++i) hp[i] = h0[i];
+        for (int c = 0; c < 2; ++c) {
+          const float2 d2 = c ? make_float2(du.z, du.z) : make_float2(du.x, du.x);
+          const float2 u2 = c ? make_float2(du.w, du.w) : make_float2(du.y, du.y);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const float2 e = mul2(d2, A2[c][i]);
+            dk[c][i] = make_float2(ex2(e.x), ex2(e.y));
+            s[c][i] = fma2(dk[c][i], s[c][i], mul2(u2, B2[i]));
+          }
         }
-        float v[2 * NL];
-        float sb = 0.f, sa = 0.f;
+      };
+      if (hf) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const float r = fmaf(s.C[t][q * NL + i], p.z, ar[i]);
-          v[i] = r * p.y;
-          v[NL + i] = p.z * h[i];
-          sb = fmaf(r, s.B[t][q * NL + i], sb);
-          ar[i] = dec[t][i] * r;
-          const float fl = ar[i] * hp[i];
-          dA[i] = fmaf(fl, p.x, dA[i]);
-          sa = fmaf(fl, A2[i], sa);
-          h[i] = hp[i];
-        }
-        rb[j] = sb;
-        fa[j] = sa;
-        using CS = ChanSum<2 * NL>;
-        float tot[CS::K3];
-        CS::run(v, tot, lane);
-        const int first = CS::first(lane);
-#pragma unroll
-        for (int i = 0; i < CS::K3; ++i) {
-          const int w = first + i;   // < NL: dB of state q NL + w, else dC
-          s.red[warp][t][w < NL ? q * NL + w : NP + q * NL + w - NL] = tot[i];
+        for (int t = 0; t < SUB; ++t) {
+          float2 dk[2][P];
+          advance(t, hs, dk);
         }
       }
-      s.o[1][g + q][chl] = quad_sum4(rb[0], rb[1], rb[2], rb[3], lane);
-      s.o[2][g + q][chl] = quad_sum4(fa[0], fa[1], fa[2], fa[3], lane);
+      const int base = hf * SUB;
+      {
+        float2 s[2][P];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < P; ++i) s[c][i] = hs[c][i];
+#pragma unroll
+        for (int t = 0; t < SUB; ++t) {
+          advance(base + t, s, dec[kKeepDec ? t : 0]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < P; ++i) h[t][c][i] = s[c][i];
+        }
+      }
+      // the adjoint recurrence, backwards
+      constexpr int QT = SUB < 4 ? SUB : 4;   // tokens whose lane sums are taken together
+#pragma unroll
+      for (int g0 = SUB - QT; g0 >= 0; g0 -= QT) {
+        float yc[2][4] = {}, rb[2][4] = {}, fa[2][4] = {};
+#pragma unroll
+        for (int j = QT - 1; j >= 0; --j) {
+          const int tl = g0 + j, t = base + tl;
+          const float4 du = load4(reinterpret_cast<const float*>(&sDU[t][chl]));
+          const float2 gg = *reinterpret_cast<const float2*>(&sG[t][chl]);
+          float2 B2[P], C2[P], dBv[P], dCv[P];
+          load_pairs<NL>(&sB[t][q * NL], B2);
+          load_pairs<NL>(&sC[t][q * NL], C2);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float2 d2 = c ? make_float2(du.z, du.z) : make_float2(du.x, du.x);
+            const float2 u2 = c ? make_float2(du.w, du.w) : make_float2(du.y, du.y);
+            const float2 g2 = c ? make_float2(gg.y, gg.y) : make_float2(gg.x, gg.x);
+            float2 sy = make_float2(0.f, 0.f), sb = sy, sa = sy;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              const float2 r = fma2(C2[i], g2, ar[c][i]);
+              const float2 hn = h[tl][c][i], hp = tl > 0 ? h[tl > 0 ? tl - 1 : 0][c][i] : hs[c][i];
+              dBv[i] = c ? fma2(r, u2, dBv[i]) : mul2(r, u2);
+              dCv[i] = c ? fma2(hn, g2, dCv[i]) : mul2(hn, g2);
+              sy = i ? fma2(C2[i], hn, sy) : mul2(C2[i], hn);
+              sb = i ? fma2(r, B2[i], sb) : mul2(r, B2[i]);
+              float2 dk;
+              if (kKeepDec) {
+                dk = dec[kKeepDec ? tl : 0][c][i];
+              } else {
+                const float2 e = mul2(d2, A2[c][i]);
+                dk = make_float2(EXR(e.x), EXR(e.y));
+              }
+              ar[c][i] = mul2(dk, r);
+              const float2 fl = mul2(ar[c][i], hp);
+              dA[c][i] = fma2(fl, d2, dA[c][i]);
+              sa = i ? fma2(fl, A2[c][i], sa) : mul2(fl, A2[c][i]);
+            }
+            yc[c][j] = sy.x + sy.y;
+            rb[c][j] = sb.x + sb.y;
+            fa[c][j] = sa.x + sa.y;
+          }
+          float v[2 * NL];
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            v[i] = pair_at(dBv[i / 2], i & 1);
+            v[NL + i] = pair_at(dCv[i / 2], i & 1);
+          }
+          using CS = ChanSum<2 * NL>;
+          float tot[CS::K3];
+          CS::run(v, tot, lane);
+          const int first = CS::first(lane);
+#pragma unroll
+          for (int i = 0; i < CS::K3; ++i) {
+            const int w = first + i;   // < NL: dB of state q NL + w, else dC
+            sRed[warp][t][w < NL ? q * NL + w : NP + q * NL + w - NL] = tot[i];
+          }
+        }
+        const int t = base + g0 + q;
+        float s0, s1;
+        if (z) {
+          s0 = quad_sum4(yc[0][0], yc[0][1], yc[0][2], yc[0][3], lane);
+          s1 = quad_sum4(yc[1][0], yc[1][1], yc[1][2], yc[1][3], lane);
+          if (q < QT) *reinterpret_cast<float2*>(&sO[0][t][chl]) = make_float2(s0, s1);
+        }
+        s0 = quad_sum4(rb[0][0], rb[0][1], rb[0][2], rb[0][3], lane);
+        s1 = quad_sum4(rb[1][0], rb[1][1], rb[1][2], rb[1][3], lane);
+        if (q < QT) *reinterpret_cast<float2*>(&sO[1][t][chl]) = make_float2(s0, s1);
+        s0 = quad_sum4(fa[0][0], fa[0][1], fa[0][2], fa[0][3], lane);
+        s1 = quad_sum4(fa[1][0], fa[1][1], fa[1][2], fa[1][3], lane);
+        if (q < QT) *reinterpret_cast<float2*>(&sO[2][t][chl]) = make_float2(s0, s1);
+      }
     }
     __syncthreads();
     // the block's dB and dC of the tile
-    for (int i = tid; i < CK * 2 * NP; i += kScanThreads) {
+    for (int i = tid; i < CK * 2 * NP; i += kBwdThreads) {
       const int tl = i / (2 * NP), n = i % (2 * NP);
-      if (t0 + tl < f.T) {
+      if (t0 + tl < tend) {
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kScanThreads / 32; ++w) sum += s.red[w][tl][n];
+        for (int w = 0; w < kBwdWarps; ++w) sum += sRed[w][tl][n];
         pBC[(((size_t)blockIdx.x * f.B + b) * f.T + t0 + tl) * (2 * NP) + n] = sum;
       }
     }
     // dx, ddt, dz
     if (stages) {
+      const float4 D4 = load4(&sPar[1][sc]);
+      const float Dv[4] = {D4.x, D4.y, D4.z, D4.w};
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         const int tl = sr + r * RT, t = t0 + tl;
+        if (t >= tend) continue;
         float ox[4], ot[4], oz[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float4 p = s.p[tl][sc + e];
-          const float rbv = s.o[1][tl][sc + e];
-          ox[e] = fmaf(rbv, p.x, Dv[e] * p.z);
+          const float d = sDU[tl][sc + e].x, g = sG[tl][sc + e];
+          const float xv = sK[0][tl][sc + e], rbv = sO[1][tl][sc + e];
+          ox[e] = fmaf(rbv, d, Dv[e] * g);
           // the factors A came in as A log2(e)
-          ot[e] = fmaf(s.o[2][tl][sc + e], 0.6931471805599453f, rbv * p.w) * ks[r][e];
-          oz[e] = kz[r][e] * (z ? fmaf(Dv[e], p.w, s.o[0][tl][sc + e]) : 0.f);
-          if (t < f.T) {
-            accD[e] = fmaf(p.z, p.w, accD[e]);
-            accB[e] += ot[e];
-          }
+          ot[e] = fmaf(sO[2][tl][sc + e], 0.6931471805599453f, rbv * xv) * sK[1][tl][sc + e];
+          if (z) oz[e] = sK[2][tl][sc + e] * fmaf(Dv[e], xv, sO[0][tl][sc + e]);
+          accD[e] = fmaf(g, xv, accD[e]);
+          accB[e] += ot[e];
         }
-        if (t < f.T) {
-          const size_t off = (row0 + t) * f.C + c0 + sc;
-          store_ch4(static_cast<T*>(a.dx) + off, sn, vec, ox);
-          store_ch4(static_cast<T*>(a.ddt) + off, sn, vec, ot);
-          if (z) store_ch4(static_cast<T*>(a.dz) + off, sn, vec, oz);
-        }
+        const size_t off = (row0 + t) * f.C + c0 + sc;
+        store_ch4(static_cast<T*>(a.dx) + off, sn, vec, ox);
+        store_ch4(static_cast<T*>(a.ddt) + off, sn, vec, ot);
+        if (z) store_ch4(static_cast<T*>(a.dz) + off, sn, vec, oz);
       }
     }
     __syncthreads();
   }
-  if (chan) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    if (chl + c >= nch) continue;
+    if (kLocal) {
+      store_pairs<NL>(slot + c * NP, ar[c]);
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < NL; ++i)
       if (q * NL + i < f.N) {
-        pA[st + i] = dA[i];
-        if (a.dh0) a.dh0[st + i] = ar[i];
+        const size_t st = (row + c) * f.N + q * NL + i;
+        pA[(size_t)kc * f.B * f.C * f.N + st] = pair_at(dA[c][i / 2], i & 1);
+        if (a.dh0 && kc == 0) a.dh0[st] = pair_at(ar[c][i / 2], i & 1);
       }
   }
-  // dD and ddt_bias: the staging rows' sums
-  float* red = &s.h[0][0][0];
-  static_assert(sizeof(s.h) >= kScanThreads * 8 * sizeof(float), "room for the rows' sums");
+  // the staging rows' sums: dD and ddt_bias, or the local pass's steps
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    red[(sr * 2 + 0) * kScanCh + sc + e] = accD[e];
-    red[(sr * 2 + 1) * kScanCh + sc + e] = accB[e];
+    sSum[0][sr][sc + e] = accD[e];
+    sSum[1][sr][sc + e] = accB[e];
   }
   __syncthreads();
-  if (tid < 2 * kScanCh) {
-    const int which = tid / kScanCh, c = tid % kScanCh;
-    if (c < nch) {
-      float sum = 0.f;
-      for (int r = 0; r < kScanThreads / 8; ++r) sum += red[(r * 2 + which) * kScanCh + c];
-      pD[((size_t)b * 2 + which) * f.C + c0 + c] = sum;
-    }
+  const int which = tid / kScanCh, c = tid % kScanCh;
+  if (c < nch) {
+    float sum = 0.f;
+    for (int r = 0; r < kBwdThreads / 8; ++r) sum += sSum[which][r][c];
+    if (!kLocal)
+      pD[(((size_t)kc * f.B + b) * 2 + which) * f.C + c0 + c] = sum;
+    else if (which == 0)
+      f.chunk_sum[((size_t)kc * f.B + b) * f.C + c0 + c] = sum;
   }
 }
 
@@ -333,33 +456,53 @@ sum_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict_
 }
 
 template <typename T, int NL>
-cudaError_t bwd_form(const ScanBwdArgs& a, int tpg, int vec, float* pBC, float* pA, float* pD,
-                     cudaStream_t st) {
-  static std::atomic<int> slot[kMaxDevices] = {};
-  const int smem = (int)sizeof(BwdSmem<NL>);
-  const cudaError_t e = ensure_smem(scan_bwd_kernel<T, NL>, smem, slot);
-  if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)(tpg * a.fwd.G), a.fwd.B);
-  scan_bwd_kernel<T, NL><<<grid, kScanThreads, smem, st>>>(a, tpg, vec, pBC, pA, pD);
+cudaError_t bwd_form(const ScanBwdArgs& a, int tpg, int vec, const ScanSplit& sp, float* pBC,
+                     float* pA, float* pD, cudaStream_t st) {
+  const dim3 grid((unsigned)(tpg * a.fwd.G), a.fwd.B, sp.chunks);
+  if (sp.chunks > 1) {
+    scan_bwd_kernel<T, NL, true><<<dim3(grid.x, grid.y, sp.chunks - 1), kBwdThreads, 0, st>>>(
+        a, tpg, vec, sp.tokens, sp.chunks, nullptr, nullptr, nullptr);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_scan_chain(a.fwd, a.dhT, sp.chunks, true, st);
+    if (e != cudaSuccess) return e;
+  }
+  scan_bwd_kernel<T, NL, false><<<grid, kBwdThreads, 0, st>>>(a, tpg, vec, sp.tokens, sp.chunks,
+                                                              pBC, pA, pD);
   return cudaGetLastError();
 }
 
+// The workspace's parts, in floats from its start.
+struct BwdLayout {
+  ScanSplit sp;
+  size_t bc, pA, pD, split, total;
+  BwdLayout(int B, int T, int C, int N, int G) {
+    sp = scan_split(B, T, C, G, true);
+    const size_t tiles = (size_t)((C / G + kScanCh - 1) / kScanCh) * G;
+    bc = 0;
+    pA = tiles * B * T * 2 * scan_padded_states(N);
+    pD = pA + ((size_t)sp.chunks * B * C * N + 3) / 4 * 4;
+    split = pD + ((size_t)sp.chunks * B * 2 * C + 3) / 4 * 4;
+    total = split + scan_split_bytes(B, C, N, sp) / sizeof(float);
+  }
+};
+
 template <typename T>
-cudaError_t bwd_dispatch(const ScanBwdArgs& a, cudaStream_t st) {
+cudaError_t bwd_dispatch(const ScanBwdArgs& args, cudaStream_t st) {
+  ScanBwdArgs a = args;
   const ScanArgs& f = a.fwd;
   const int Cg = f.C / f.G, NP = scan_padded_states(f.N);
   const int tpg = (Cg + kScanCh - 1) / kScanCh;
   const int vec = f.C % 4 == 0 && Cg % 4 == 0;
   const long long rows = (long long)f.B * f.T;
-  float* pBC = a.part;
-  float* pA = pBC + (size_t)tpg * f.G * rows * 2 * NP;
-  float* pD = pA + ((size_t)f.B * f.C * f.N + 3) / 4 * 4;
+  const BwdLayout lay(f.B, f.T, f.C, f.N, f.G);
+  float *pBC = a.part + lay.bc, *pA = a.part + lay.pA, *pD = a.part + lay.pD;
+  scan_split_workspace(a.fwd, a.part + lay.split, lay.sp);
   cudaError_t e;
-  if (f.N <= 4) e = bwd_form<T, 1>(a, tpg, vec, pBC, pA, pD, st);
-  else if (f.N <= 8) e = bwd_form<T, 2>(a, tpg, vec, pBC, pA, pD, st);
-  else if (f.N <= 16) e = bwd_form<T, 4>(a, tpg, vec, pBC, pA, pD, st);
-  else if (f.N <= 32) e = bwd_form<T, 8>(a, tpg, vec, pBC, pA, pD, st);
-  else e = bwd_form<T, 16>(a, tpg, vec, pBC, pA, pD, st);
+  if (f.N <= 4) e = bwd_form<T, 1>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
+  else if (f.N <= 8) e = bwd_form<T, 2>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
+  else if (f.N <= 16) e = bwd_form<T, 4>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
+  else if (f.N <= 32) e = bwd_form<T, 8>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
+  else e = bwd_form<T, 16>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
   if (e != cudaSuccess) return e;
   const long long n = rows * f.G * 2 * NP;
   if (n > 0) {
@@ -371,10 +514,11 @@ cudaError_t bwd_dispatch(const ScanBwdArgs& a, cudaStream_t st) {
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  e = launch_sum_partials(pA, a.dA, f.B, (long long)f.C * f.N, (long long)f.C * f.N, st);
-  if (e == cudaSuccess && a.dD) e = launch_sum_partials(pD, a.dD, f.B, 2LL * f.C, f.C, st);
+  const long long parts = (long long)lay.sp.chunks * f.B;
+  e = launch_sum_partials(pA, a.dA, parts, (long long)f.C * f.N, (long long)f.C * f.N, st);
+  if (e == cudaSuccess && a.dD) e = launch_sum_partials(pD, a.dD, parts, 2LL * f.C, f.C, st);
   if (e == cudaSuccess && a.ddt_bias)
-    e = launch_sum_partials(pD + f.C, a.ddt_bias, f.B, 2LL * f.C, f.C, st);
+    e = launch_sum_partials(pD + f.C, a.ddt_bias, parts, 2LL * f.C, f.C, st);
   return e;
 }
 
@@ -382,9 +526,7 @@ cudaError_t bwd_dispatch(const ScanBwdArgs& a, cudaStream_t st) {
 
 size_t selective_scan_bwd_workspace_bytes(int B, int T, int C, int N, int G) {
   if (B <= 0 || C <= 0 || G <= 0 || N <= 0 || T < 0) return 0;
-  const size_t tiles = (size_t)((C / G + kScanCh - 1) / kScanCh) * G;
-  const size_t pA = ((size_t)B * C * N + 3) / 4 * 4;
-  return (tiles * B * T * 2 * scan_padded_states(N) + pA + (size_t)B * 2 * C) * sizeof(float);
+  return BwdLayout(B, T, C, N, G).total * sizeof(float);
 }
 
 cudaError_t launch_selective_scan_bwd(const ScanBwdArgs& a, cudaStream_t st) {

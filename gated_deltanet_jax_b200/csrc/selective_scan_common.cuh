@@ -16,6 +16,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The same, formed again where it stands (not kept in a register from an equal
+// argument's earlier use).
+__device__ __forceinline__ float ex2_again(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, the logarithm as
