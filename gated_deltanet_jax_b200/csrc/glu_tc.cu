@@ -244,7 +244,7 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
           tmem_ld32(acc + 128 + half * 64 + c * 32, u);
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            g[e] = __fdividef(g[e], 1.f + __expf(-g[e])) * u[e];
+            g[e] = g[e] * fast_sigmoid(g[e]) * u[e];
           put(box, c * 4, g);
         }
         if (!sh.keep) release();
@@ -287,6 +287,162 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
+// ---------------------------------------------------------------------------
+// Few tokens: the weights are streamed once
+// ---------------------------------------------------------------------------
+//
+// HBM-bound on Wg and Wu (46 MB at 2048 x 5632).  A CTA owns W output columns:
+// W rows of Wg and the same W of Wu form B (2 W columns of the accumulator), the
+// tokens are A's rows, of which only the ones in use are loaded (the others'
+// products are never read).  Two CTAs share an SM and each keeps as many 64-wide
+// stages in flight as half its shared memory holds.  The same tiles serve
+// products too small to fill the GPU with 256 x 256 tiles.
+constexpr int kNarrowThreads = 192;
+constexpr int kNarrowMaxStages = 12;
+constexpr int kNarrowSmem = 110 * 1024;
+
+struct NarrowShape {
+  int M, I, tiles_m, tiles_n, kblocks, rows_a, stages;
+};
+struct alignas(64) NarrowMaps {
+  CUtensorMap x, wg, wu;
+};
+
+template <int W>
+__global__ void __launch_bounds__(kNarrowThreads, 2)
+glu_narrow_kernel(const __grid_constant__ NarrowMaps maps, const NarrowShape sh,
+                  __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ gk,
+                  __nv_bfloat16* __restrict__ uk) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* sm = smem_raw + (1024u - (smem_u32(smem_raw) & 1023u)) % 1024u;
+  __shared__ __align__(8) uint64_t full[kNarrowMaxStages], empty[kNarrowMaxStages], tfull[2],
+      tempty[2];
+  __shared__ uint32_t tmem_slot;
+  constexpr int kCols = 4 * W;                       // two accumulators of 2 W columns
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int bytes_a = sh.rows_a * 128;               // rows of 128 bytes, 8 an atom
+  constexpr int kBytesB = 2 * W * 128;
+  const int stage_bytes = bytes_a + kBytesB;         // both multiples of 1024
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < sh.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 4);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const long long tiles = (long long)sh.tiles_m * sh.tiles_n;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t it = 0, s = 0, ph = 1;
+      for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const int m = (int)(t % sh.tiles_m), n = (int)(t / sh.tiles_m);
+        for (int k = 0; k < sh.kblocks; ++k, ++it) {
+          ok = mbar_wait(&empty[s], ph);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full[s], (uint32_t)stage_bytes);
+          unsigned char* b = sm + s * stage_bytes;
+          tma_load_2d(b, &maps.wg, k * kBK, n * W, &full[s]);
+          tma_load_2d(b + kBytesB / 2, &maps.wu, k * kBK, n * W, &full[s]);
+          tma_load_2d(b + kBytesB, &maps.x, k * kBK, m * 128, &full[s]);
+          if (++s == (uint32_t)sh.stages) { s = 0; ph ^= 1; }
+        }
+      }
+      // the loads still in flight land before the CTA leaves
+      for (int i = 0; ok && i < sh.stages && (uint32_t)i < it; ++i) {
+        ok = mbar_wait(&empty[s], ph);
+        if (++s == (uint32_t)sh.stages) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_bf16(128, 2 * W, 0, 0);
+      const uint32_t sbase = smem_u32(sm);
+      bool ok = true;
+      uint32_t j = 0, s = 0, ph = 0;
+      for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++j) {
+        const uint32_t acc = tmem + (j & 1) * 2 * W;
+        ok = mbar_wait(&tempty[j & 1], ((j >> 1) & 1) ^ 1);
+        tc_fence_after();
+        for (int k = 0; ok && k < sh.kblocks; ++k) {
+          ok = mbar_wait(&full[s], ph);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t b = sbase + s * stage_bytes, x = b + kBytesB;
+#pragma unroll
+          for (int q = 0; q < kBK / 16; ++q)
+            mma_bf16(acc, umma_desc(x + q * 32, 16, 1024, kSW128),
+                     umma_desc(b + q * 32, 16, 1024, kSW128), idesc, (k | q) != 0);
+          mma_commit(&empty[s]);
+          if (++s == (uint32_t)sh.stages) { s = 0; ph ^= 1; }
+        }
+        if (ok) mma_commit(&tfull[j & 1]);
+      }
+    }
+  } else {
+    const int quad = warp & 3;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    uint32_t j = 0;
+    bool ok = true;
+    for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++j) {
+      const int m = (int)(t % sh.tiles_m), n = (int)(t / sh.tiles_m);
+      ok = mbar_wait(&tfull[j & 1], (j >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (j & 1) * 2 * W + lanes;
+      const long long row = (long long)m * 128 + quad * 32 + lane;
+#pragma unroll
+      for (int c = 0; c < W / 16; ++c) {
+        float g[16], u[16];
+        tmem_ld16x2(acc + c * 16, acc + W + c * 16, g, u);
+        const int col = n * W + c * 16;
+        if (row < sh.M) {
+          auto put = [&](__nv_bfloat16* p, const float (&v)[16]) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+              if (col + e < sh.I) {   // I is a multiple of 8
+                uint4 q;
+                __nv_bfloat162* b2 = reinterpret_cast<__nv_bfloat162*>(&q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  b2[i] = __floats2bfloat162_rn(v[e + 2 * i], v[e + 2 * i + 1]);
+                *reinterpret_cast<uint4*>(p + row * sh.I + col + e) = q;
+              }
+          };
+          if (gk) {
+            put(gk, g);
+            put(uk, u);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) g[e] = g[e] * fast_sigmoid(g[e]) * u[e];
+          put(h, g);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[j & 1]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, kCols);
+}
+
 // [rows, cols] bf16 row-major, boxes of 64 columns x `box_rows`, 128-byte swizzle.
 bool make_map(CUtensorMap* m, const void* base, long long rows, long long cols, int box_rows) {
   auto fn = encode_fn();
@@ -315,6 +471,34 @@ cudaError_t launch_kind(const GluMaps& maps, const GluShape& sh, cudaStream_t st
   return cudaGetLastError();
 }
 
+template <int W>
+cudaError_t launch_narrow(const GluArgs& a, cudaStream_t st) {
+  NarrowMaps m;
+  NarrowShape sh;
+  sh.M = a.M;
+  sh.I = a.I;
+  sh.tiles_m = ceil_div(a.M, 128);
+  sh.tiles_n = ceil_div(a.I, W);
+  sh.kblocks = ceil_div(a.D, kBK);
+  sh.rows_a = a.M >= 128 ? 128 : ceil_div(a.M, 8) * 8;
+  // The products read all 128 rows of A's tile from a stage's start of it (rows past
+  // rows_a are whatever lies there): the last stage's end inside the allocation too.
+  const int bytes_a = sh.rows_a * 128;
+  sh.stages = (kNarrowSmem - 1024 - 128 * 128 + bytes_a) / (bytes_a + 2 * W * 128);
+  if (sh.stages > kNarrowMaxStages) sh.stages = kNarrowMaxStages;
+  if (!make_map(&m.x, a.x, a.M, a.D, sh.rows_a) || !make_map(&m.wg, a.wg, a.I, a.D, W) ||
+      !make_map(&m.wu, a.wu, a.I, a.D, W))
+    return cudaErrorInvalidValue;
+  static std::atomic<int> slot[kMaxDevices] = {};
+  const cudaError_t e = ensure_smem(glu_narrow_kernel<W>, kNarrowSmem, slot);
+  if (e != cudaSuccess) return e;
+  const long long tiles = (long long)sh.tiles_m * sh.tiles_n, most = 2LL * device_sm_count();
+  glu_narrow_kernel<W><<<(unsigned)(tiles < most ? tiles : most), kNarrowThreads, kNarrowSmem,
+                         st>>>(m, sh, static_cast<__nv_bfloat16*>(a.h),
+                               static_cast<__nv_bfloat16*>(a.g), static_cast<__nv_bfloat16*>(a.u));
+  return cudaGetLastError();
+}
+
 }  // namespace
 
 GDN_DEVICE_ERROR_ACCESSOR(device_error_glu_tc)
@@ -325,6 +509,17 @@ bool glu_tc_supported(int M, int D, int I, int dtype) {
 }
 
 cudaError_t launch_glu_tc_fwd(const GluArgs& a, cudaStream_t st) {
+#ifndef NARROW_M
+#define NARROW_M 128
+#endif
+#ifndef NARROW_W
+#define NARROW_W 0
+#endif
+  if (a.M <= NARROW_M) {
+    const int w = NARROW_W ? NARROW_W : a.I > 296 * 32 ? 64 : a.I > 296 * 16 ? 32 : 16;
+    if (w == 64) return launch_narrow<64>(a, st);
+    return w == 32 ? launch_narrow<32>(a, st) : launch_narrow<16>(a, st);
+  }
   GluMaps m;
   if (!make_map(&m.a[0], a.x, a.M, a.D, 128) || !make_map(&m.b[0], a.wg, a.I, a.D, 128) ||
       !make_map(&m.b[1], a.wu, a.I, a.D, 128) || !make_map(&m.out[0], a.h, a.M, a.I, 128) ||

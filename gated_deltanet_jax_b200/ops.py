@@ -114,8 +114,12 @@ def _prepare(q, k, v, g, beta, initial_state, final_state_out, output_final_stat
 
 
 def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                           for t in ts)
+    if not torch.is_grad_enabled():
+        return False
+    for t in ts:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            return True
+    return False
 
 
 class _DeltaRuleFn(torch.autograd.Function):
@@ -482,7 +486,8 @@ def _on_device(index: int):
 
 
 def _stream(index: int) -> int:
-    return torch.cuda.current_stream(index).cuda_stream
+    # the raw handle: torch.cuda.current_stream() builds a Stream object around it
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -525,6 +530,16 @@ def _cuda_input(name, t):
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
     if t.dtype not in _DTYPES:
         raise TypeError(f"{name} must be bfloat16 or float32; got {t.dtype}")
+
+
+def _conv_state(t, name, shape, dtype, dev):
+    if t is None:
+        return None
+    if t.shape != shape or t.dtype != dtype or t.device != dev:
+        raise ValueError(f"{name} must be {shape} {dtype} on {dev}")
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+    return t
 
 
 class _ShortConvFn(torch.autograd.Function):
@@ -609,23 +624,12 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
         w = w.reshape(w.shape[0], w.shape[-1])
     if w.dim() != 2 or w.shape[1] != C:
         raise ValueError(f"weight must be [K,{C}] or [K,1,{C}]; got {tuple(weight.shape)}")
-    K = w.shape[0]
-    shape = (B, K - 1, C)
-
-    def state(t, name):
-        if t is None:
-            return None
-        if tuple(t.shape) != shape or t.dtype != x.dtype or t.device != dev:
-            raise ValueError(f"{name} must be {shape} {x.dtype} on {dev}")
-        if not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError(f"{name} must be contiguous and 16-byte aligned")
-        return t
-
-    s_in = state(conv_state, "conv_state")
-    s_out = state(final_state_out, "final_state_out")
+    shape = (B, w.shape[0] - 1, C)
+    s_in = _conv_state(conv_state, "conv_state", shape, x.dtype, dev)
+    s_out = _conv_state(final_state_out, "final_state_out", shape, x.dtype, dev)
     if bias is not None:
         bias = _on(bias, dev)
-        if tuple(bias.shape) != (C,):
+        if bias.shape != (C,):
             raise ValueError(f"bias must be [{C}]; got {tuple(bias.shape)}")
     if _wants_grad(x, w, bias, conv_state):
         if final_state_out is not None:
@@ -803,16 +807,15 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
     _cuda_input("x", x)
     if x.dim() != 3:
         raise ValueError(f"x must be [B,T,Ch]; got {tuple(x.shape)}")
-    dev = x.device
-    dtype = x.dtype
+    dev, dtype, shape_x = x.device, x.dtype, x.shape
     _check_input("dt", dt, dev, dtype)
     _check_input("B", B, dev, dtype)
     _check_input("C", C, dev, dtype)
     if z is not None:
         _check_input("z", z, dev, dtype)
-    b, T, ch = x.shape
-    if dt.shape != x.shape or (z is not None and z.shape != x.shape):
-        raise ValueError(f"dt and z must have x's shape {tuple(x.shape)}")
+    b, T, ch = shape_x
+    if dt.shape != shape_x or (z is not None and z.shape != shape_x):
+        raise ValueError(f"dt and z must have x's shape {tuple(shape_x)}")
     A = _on(A, dev)
     if A.dim() != 2 or A.shape[0] != ch:
         raise ValueError(f"A must be [{ch},N]; got {tuple(A.shape)}")
@@ -821,19 +824,22 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
         B = B.unsqueeze(2)
     if C.dim() == 3:
         C = C.unsqueeze(2)
-    if B.dim() != 4 or tuple(B.shape[:2]) != (b, T) or B.shape[3] != N or C.shape != B.shape:
+    G = B.shape[2] if B.dim() == 4 else 0
+    if B.shape != (b, T, G, N) or C.shape != B.shape:
         raise ValueError(f"B and C must be [{b},{T},{N}] or [{b},{T},G,{N}]; got "
                          f"{tuple(B.shape)}, {tuple(C.shape)}")
-    G = B.shape[2]
     if G < 1 or ch % G:
         raise ValueError(f"x's {ch} channels must be a multiple of the {G} groups of B and C")
-    for name, t in (("D", D), ("dt_bias", dt_bias)):
-        if t is not None and tuple(t.shape) != (ch,):
-            raise ValueError(f"{name} must be [{ch}]; got {tuple(t.shape)}")
-    D = None if D is None else _on(D, dev)
-    dt_bias = None if dt_bias is None else _on(dt_bias, dev)
+    if D is not None:
+        D = _on(D, dev)
+        if D.shape != (ch,):
+            raise ValueError(f"D must be [{ch}]; got {tuple(D.shape)}")
+    if dt_bias is not None:
+        dt_bias = _on(dt_bias, dev)
+        if dt_bias.shape != (ch,):
+            raise ValueError(f"dt_bias must be [{ch}]; got {tuple(dt_bias.shape)}")
     shape = (b, ch, N)
-    if initial_state is not None and (tuple(initial_state.shape) != shape
+    if initial_state is not None and (initial_state.shape != shape
                                       or initial_state.device != dev):
         raise ValueError(f"initial_state must be {shape} on {dev}")
     softplus = int(bool(dt_softplus))
@@ -844,7 +850,7 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
         return y, hT if output_final_state else None
     hT = final_state_out
     if hT is not None:
-        if (tuple(hT.shape) != shape or hT.dtype != torch.float32 or not hT.is_contiguous()
+        if (hT.shape != shape or hT.dtype != torch.float32 or not hT.is_contiguous()
                 or hT.device != dev or hT.data_ptr() % 16):
             raise ValueError(f"final_state_out must be a contiguous, 16-byte aligned float32 "
                              f"{shape} tensor on {dev}")

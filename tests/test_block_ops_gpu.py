@@ -44,7 +44,7 @@ def _within(out, ref, tol, what):
 
 GLU = [(1, 64, 64), (1, 2048, 136), (2, 256, 96), (3, 40, 24), (7, 250, 66), (33, 128, 200),
        (64, 64, 128), (127, 72, 56), (128, 128, 128), (129, 192, 320), (257, 520, 264),
-       (300, 33, 17), (1000, 256, 768)]
+       (300, 33, 17), (1000, 256, 768), (5, 1600, 4808), (37, 2048, 136), (2, 136, 9600)]
 
 
 def _glu_inputs(M, D, I, dtype, dev, seed):
@@ -78,9 +78,14 @@ def test_glu_gradients(cuda, dtype, M, D, I):
     for k, t in zip(("dx", "dwg", "dwu"), grads):
         _within(t, ref[k], tol[k], k)
         # roundings of single values average out in a norm: five of at most half a
-        # step each, and the arithmetic's share
+        # step each, and the arithmetic's share.  A running fp32 sum of n terms of
+        # size s and random sign: after k of them it is about s sqrt(k), an addition
+        # errs by at most 2^-24 of that (over sqrt(3) in the mean square), together
+        # s 2^-24 / sqrt(3) sqrt(1 + 2 + .. + n) = s 2^-24 n / sqrt(6) beside a result of
+        # s sqrt(n): 2^-24 sqrt(n / 6) of it.  Twice that is allowed.
+        n = 2 * I if k == "dx" else M
         off = (_f64(t) - ref[k]).norm() / ref[k].norm()
-        assert off <= 5 * HALF[dtype] + 2e-6, (k, off)
+        assert off <= 5 * HALF[dtype] + 2e-6 + 2.0 ** -23 * (n / 6) ** 0.5, (k, off)
     assert _lib.load().gdn_device_error(0) == 0
 
 
