@@ -220,6 +220,14 @@ __device__ __forceinline__ void st_async_cluster_f32(uint32_t dst_cluster_addr, 
       : "memory");
 }
 
+// 16 bytes into another CTA's shared memory of the cluster (16-byte aligned).
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t dst_cluster_addr, float a, float b,
+                                                 float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst_cluster_addr),
+               "f"(a), "f"(b), "f"(c), "f"(d)
+               : "memory");
+}
+
 // All threads of every CTA of the cluster.
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
