@@ -17,11 +17,14 @@ The GatedDeltaNet-specific work runs on the CUDA kernels: the short convolution
 (``ops.short_convolution``), and the gates + delta rule + gated RMSNorm in one
 call (``ops.gated_delta_rule_chunk_layer`` in ``'chunk'`` mode on its tensor-core
 shapes, ``ops.gated_delta_rule_decode_layer`` in ``'fused_recurrent'`` mode; the
-separate ops elsewhere).  Embedding, RMSNorm, projections and the MLP are plain
-torch operations (cuBLAS GEMMs).  The fused forms have no backward: when
-gradients are wanted, the layer takes the differentiable route instead (torch
-short convolution and gated RMSNorm, the delta rule through the ops' autograd,
-whose backward is ``gdn_chunk_bwd``).
+separate ops elsewhere).  With gradients wanted (or
+``GatedDeltaNetMLP.fused_inference``) the MLP's two projections, SiLU and product
+are one kernel in bf16 (``ops.gated_linear_unit``).  Embedding, RMSNorm and the other
+projections are plain torch operations (cuBLAS GEMMs).  The layer's fused form
+has no backward: when gradients are wanted, the layer takes the differentiable
+route instead (torch gated RMSNorm, the delta rule through the ops' autograd,
+whose backward is ``gdn_chunk_bwd``); the convolution and the gated linear unit
+have their own (``gdn_short_conv_bwd``, ``gdn_glu_bwd``).
 
 Like the reference, the layer applies no L2 norm and no 1/sqrt(dk) scale to q
 and k, so at the default initialisation the recurrence grows by orders of
@@ -39,6 +42,8 @@ from typing import Optional
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
+from torch.nn.modules import module
 import torch.nn.functional as F
 
 from . import dispatch, ops
@@ -61,11 +66,30 @@ def _linear(d_in: int, d_out: int) -> nn.Linear:
     return lin
 
 
+def _kernel_call_ok(*ts) -> bool:
+    """Whether the kernels may stand in for torch operations on these tensors: plain
+    CUDA tensors of one dtype that the kernels take, outside torch's tracing,
+    function transforms, forward-mode differentiation and autocast."""
+    x = ts[0]
+    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32)
+            and all(type(t) in (torch.Tensor, nn.Parameter) and t.device == x.device for t in ts)
+            and not torch.compiler.is_compiling() and not torch.is_autocast_enabled("cuda")
+            and not torch._C._are_functorch_transforms_active()
+            and forward_ad._current_level < 0)
+
+
+def _plain_linear(m: nn.Module, dtype) -> bool:
+    """An nn.Linear without bias whose call is its product and nothing else."""
+    return (type(m) is nn.Linear and m.bias is None and m.weight.dtype == dtype
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks
+                     or m._backward_pre_hooks or module._has_any_global_hook()))
+
+
 class ShortConvolution(nn.Module):
     """Causal depthwise convolution over time, kernel K, then SiLU (model.py:15-40).
     ``weight`` [K, C] (the Flax depthwise kernel [K, 1, C] squeezed), optional bias.
-    On the GPU kernel (gdn_short_conv_fwd) for inference; torch's conv1d when
-    gradients are wanted or with a bias."""
+    On the GPU kernels (gdn_short_conv_fwd, gdn_short_conv_bwd) at the shapes they
+    take; torch's conv1d elsewhere."""
 
     def __init__(self, hidden_size: int, kernel_size: int, activation: Optional[str] = "silu",
                  use_bias: bool = False):
@@ -85,6 +109,11 @@ class ShortConvolution(nn.Module):
                                          activation="silu" if act else None)
             return y
         K, C = self.weight.shape
+        if (K <= 8 and C % (8 if x.dtype == torch.bfloat16 else 4) == 0
+                and _kernel_call_ok(x, self.weight)):
+            y, _ = ops.short_convolution(x, self.weight, bias=self.bias,
+                                         activation="silu" if act else None)
+            return y
         xt = F.pad(x.transpose(1, 2), (K - 1, 0))
         bias = None if self.bias is None else self.bias.to(x.dtype)
         y = F.conv1d(xt, self.weight.t().reshape(C, 1, K).to(x.dtype), bias, groups=C)
@@ -199,7 +228,14 @@ class GatedDeltaNet(nn.Module):
 
 
 class GatedDeltaNetMLP(nn.Module):
-    """SwiGLU MLP (model.py:162-180)."""
+    """SwiGLU MLP (model.py:162-180).  In bf16 with gradients wanted, the projections,
+    SiLU and product run as one kernel with its own backward
+    (``ops.gated_linear_unit``).  Inference keeps torch's separate operations, and
+    with them the bits it gave before, unless ``fused_inference`` is set (on the
+    class or an instance): the kernel rounds once where they round four times, and
+    takes 0.49 ms against 0.65 for 16384 tokens of 2048 x 5632."""
+
+    fused_inference = False
 
     def __init__(self, config: GatedDeltaNetConfig):
         super().__init__()
@@ -214,7 +250,16 @@ class GatedDeltaNetMLP(nn.Module):
         self.down_proj = _linear(inter, config.hidden_size)
 
     def forward(self, x):
-        return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
+        gate, up = self.gate_proj, self.up_proj
+        grad = torch.is_grad_enabled() and (
+            x.requires_grad or any(p.requires_grad for p in self.parameters()))
+        if ((grad or self.fused_inference) and x.dtype == torch.bfloat16
+                and _plain_linear(gate, x.dtype) and _plain_linear(up, x.dtype)
+                and gate.weight.shape == up.weight.shape
+                and x.shape[-1] % 8 == 0 and gate.out_features % 8 == 0
+                and _kernel_call_ok(x, gate.weight, up.weight)):
+            return self.down_proj(ops.gated_linear_unit(x, gate.weight, up.weight))
+        return self.down_proj(F.silu(gate(x)) * up(x))
 
 
 class GatedDeltaNetBlock(nn.Module):
