@@ -305,9 +305,14 @@ struct ShortConvBwdArgs {
 };
 size_t short_conv_bwd_workspace_bytes(int B, int T, int C, int K);
 cudaError_t launch_short_conv_bwd(const ShortConvBwdArgs& a, cudaStream_t st);
-// out[i] = sum over p < parts of part[p stride + i], i < n, in a fixed order.
-cudaError_t launch_sum_partials(const float* part, float* out, long long parts, long long stride,
-                                long long n, cudaStream_t st);
+// Sums `parts` rows of `stride` floats, in a fixed order; the row's columns go to
+// consecutive segments of n[k] values (n adding up to stride; dst NULL: dropped).
+struct SumSegments {
+  float* dst[3];
+  long long n[3];
+};
+cudaError_t launch_sum_partials(const float* part, long long parts, long long stride,
+                                const SumSegments& out, cudaStream_t st);
 // Gated RMSNorm (model.py:41-53) over `rows` rows of dv; o and y may alias.
 bool gated_norm_supported(int dv, int dtype);
 cudaError_t launch_gated_norm(const void* o, const void* gate, const float* w, void* y,

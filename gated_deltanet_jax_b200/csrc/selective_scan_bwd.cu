@@ -61,25 +61,15 @@ struct ChanSum {
   }
 };
 
-#ifndef EXR
-#define EXR ex2_again
-#endif
-#ifndef MINB
-#define MINB 6
-#endif
-#ifndef KEEPDEC
-#define KEEPDEC 0
-#endif
-constexpr bool kKeepDec = KEEPDEC;
 constexpr int kBwdThreads = 64;   // 16 slots of four lanes, two channels a lane
 constexpr int kBwdWarps = kBwdThreads / 32;
 
 // kLocal: the first pass of a cut row (chunks 1 ..: the adjoint from zero over
 // the chunk and the steps' sum out, no gradients).
 template <typename T, int NL, bool kLocal>
-__global__ void __launch_bounds__(kBwdThreads, NL <= 4 ? MINB : 4)
+__global__ void __launch_bounds__(kBwdThreads, NL <= 4 ? 6 : 4)
 scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, int nchunk,
-                float* __restrict__ pBC, float* __restrict__ pA, float* __restrict__ pD) {
+                float* __restrict__ pBC, float* __restrict__ pP) {
   constexpr int CK = scan_tile<NL>(), SUB = CK / 2;
   constexpr int NP = NL * kScanLanes;
   constexpr int P = scan_pairs<NL>();
@@ -245,14 +235,13 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
 #pragma unroll 1
     for (int hf = 1; hf >= 0; --hf) {
       float2 hs[2][P], h[SUB][2][P];
-      float2 dec[kKeepDec ? SUB : 1][2][P];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int i = 0; i < P; ++i) hs[c][i] = make_float2(0.f, 0.f);
         if (chl + c < nch) load_pairs<NL>(ck + c * NP, hs[c]);
       }
-      auto advance = [&](int t, float2 (&s)[2][P], float2 (&dk)[2][P]) {
+      auto advance = [&](int t, float2 (&s)[2][P]) {
         const float4 du = load4(reinterpret_cast<const float*>(&sDU[t][chl]));
         float2 B2[P];
         load_pairs<NL>(&sB[t][q * NL], B2);
@@ -263,16 +252,14 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             const float2 e = mul2(d2, A2[c][i]);
-            dk[c][i] = make_float2(ex2(e.x), ex2(e.y));
-            s[c][i] = fma2(dk[c][i], s[c][i], mul2(u2, B2[i]));
+            s[c][i] = fma2(make_float2(ex2(e.x), ex2(e.y)), s[c][i], mul2(u2, B2[i]));
           }
         }
       };
       if (hf) {
 #pragma unroll
         for (int t = 0; t < SUB; ++t) {
-          float2 dk[2][P];
-          advance(t, hs, dk);
+          advance(t, hs);
         }
       }
       const int base = hf * SUB;
@@ -284,7 +271,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
           for (int i = 0; i < P; ++i) s[c][i] = hs[c][i];
 #pragma unroll
         for (int t = 0; t < SUB; ++t) {
-          advance(base + t, s, dec[kKeepDec ? t : 0]);
+          advance(base + t, s);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -318,13 +305,10 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
               dCv[i] = c ? fma2(hn, g2, dCv[i]) : mul2(hn, g2);
               sy = i ? fma2(C2[i], hn, sy) : mul2(C2[i], hn);
               sb = i ? fma2(r, B2[i], sb) : mul2(r, B2[i]);
-              float2 dk;
-              if (kKeepDec) {
-                dk = dec[kKeepDec ? tl : 0][c][i];
-              } else {
-                const float2 e = mul2(d2, A2[c][i]);
-                dk = make_float2(EXR(e.x), EXR(e.y));
-              }
+              // (kept from the walk above, the factors spilled: 1.24 against 0.83 ms
+              // for the training pass of 4 x 2048 x 2048)
+              const float2 e = mul2(d2, A2[c][i]);
+              const float2 dk = make_float2(ex2_again(e.x), ex2_again(e.y));
               ar[c][i] = mul2(dk, r);
               const float2 fl = mul2(ar[c][i], hp);
               dA[c][i] = fma2(fl, d2, dA[c][i]);
@@ -404,6 +388,8 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
     }
     __syncthreads();
   }
+  // this chunk's and row's sums for the parameters: dA [C][N], dD [C], ddt_bias [C]
+  const size_t prow = ((size_t)kc * f.B + b) * f.C * (f.N + 2);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (chl + c >= nch) continue;
@@ -414,9 +400,9 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
 #pragma unroll
     for (int i = 0; i < NL; ++i)
       if (q * NL + i < f.N) {
-        const size_t st = (row + c) * f.N + q * NL + i;
-        pA[(size_t)kc * f.B * f.C * f.N + st] = pair_at(dA[c][i / 2], i & 1);
-        if (a.dh0 && kc == 0) a.dh0[st] = pair_at(ar[c][i / 2], i & 1);
+        pP[prow + (size_t)(c0 + chl + c) * f.N + q * NL + i] = pair_at(dA[c][i / 2], i & 1);
+        if (a.dh0 && kc == 0)
+          a.dh0[(row + c) * f.N + q * NL + i] = pair_at(ar[c][i / 2], i & 1);
       }
   }
   // the staging rows' sums: dD and ddt_bias, or the local pass's steps
@@ -431,7 +417,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
     float sum = 0.f;
     for (int r = 0; r < kBwdThreads / 8; ++r) sum += sSum[which][r][c];
     if (!kLocal)
-      pD[(((size_t)kc * f.B + b) * 2 + which) * f.C + c0 + c] = sum;
+      pP[prow + (size_t)f.C * (f.N + which) + c0 + c] = sum;
     else if (which == 0)
       f.chunk_sum[((size_t)kc * f.B + b) * f.C + c0 + c] = sum;
   }
@@ -457,31 +443,30 @@ sum_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict_
 
 template <typename T, int NL>
 cudaError_t bwd_form(const ScanBwdArgs& a, int tpg, int vec, const ScanSplit& sp, float* pBC,
-                     float* pA, float* pD, cudaStream_t st) {
+                     float* pP, cudaStream_t st) {
   const dim3 grid((unsigned)(tpg * a.fwd.G), a.fwd.B, sp.chunks);
   if (sp.chunks > 1) {
     scan_bwd_kernel<T, NL, true><<<dim3(grid.x, grid.y, sp.chunks - 1), kBwdThreads, 0, st>>>(
-        a, tpg, vec, sp.tokens, sp.chunks, nullptr, nullptr, nullptr);
+        a, tpg, vec, sp.tokens, sp.chunks, nullptr, nullptr);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = launch_scan_chain(a.fwd, a.dhT, sp.chunks, true, st);
     if (e != cudaSuccess) return e;
   }
   scan_bwd_kernel<T, NL, false><<<grid, kBwdThreads, 0, st>>>(a, tpg, vec, sp.tokens, sp.chunks,
-                                                              pBC, pA, pD);
+                                                              pBC, pP);
   return cudaGetLastError();
 }
 
 // The workspace's parts, in floats from its start.
 struct BwdLayout {
   ScanSplit sp;
-  size_t bc, pA, pD, split, total;
+  size_t bc, params, split, total;
   BwdLayout(int B, int T, int C, int N, int G) {
     sp = scan_split(B, T, C, G, true);
     const size_t tiles = (size_t)((C / G + kScanCh - 1) / kScanCh) * G;
     bc = 0;
-    pA = tiles * B * T * 2 * scan_padded_states(N);
-    pD = pA + ((size_t)sp.chunks * B * C * N + 3) / 4 * 4;
-    split = pD + ((size_t)sp.chunks * B * 2 * C + 3) / 4 * 4;
+    params = tiles * B * T * 2 * scan_padded_states(N);
+    split = params + ((size_t)sp.chunks * B * C * (N + 2) + 3) / 4 * 4;
     total = split + scan_split_bytes(B, C, N, sp) / sizeof(float);
   }
 };
@@ -495,14 +480,14 @@ cudaError_t bwd_dispatch(const ScanBwdArgs& args, cudaStream_t st) {
   const int vec = f.C % 4 == 0 && Cg % 4 == 0;
   const long long rows = (long long)f.B * f.T;
   const BwdLayout lay(f.B, f.T, f.C, f.N, f.G);
-  float *pBC = a.part + lay.bc, *pA = a.part + lay.pA, *pD = a.part + lay.pD;
+  float *pBC = a.part + lay.bc, *pP = a.part + lay.params;
   scan_split_workspace(a.fwd, a.part + lay.split, lay.sp);
   cudaError_t e;
-  if (f.N <= 4) e = bwd_form<T, 1>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
-  else if (f.N <= 8) e = bwd_form<T, 2>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
-  else if (f.N <= 16) e = bwd_form<T, 4>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
-  else if (f.N <= 32) e = bwd_form<T, 8>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
-  else e = bwd_form<T, 16>(a, tpg, vec, lay.sp, pBC, pA, pD, st);
+  if (f.N <= 4) e = bwd_form<T, 1>(a, tpg, vec, lay.sp, pBC, pP, st);
+  else if (f.N <= 8) e = bwd_form<T, 2>(a, tpg, vec, lay.sp, pBC, pP, st);
+  else if (f.N <= 16) e = bwd_form<T, 4>(a, tpg, vec, lay.sp, pBC, pP, st);
+  else if (f.N <= 32) e = bwd_form<T, 8>(a, tpg, vec, lay.sp, pBC, pP, st);
+  else e = bwd_form<T, 16>(a, tpg, vec, lay.sp, pBC, pP, st);
   if (e != cudaSuccess) return e;
   const long long n = rows * f.G * 2 * NP;
   if (n > 0) {
@@ -514,12 +499,9 @@ cudaError_t bwd_dispatch(const ScanBwdArgs& args, cudaStream_t st) {
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  const long long parts = (long long)lay.sp.chunks * f.B;
-  e = launch_sum_partials(pA, a.dA, parts, (long long)f.C * f.N, (long long)f.C * f.N, st);
-  if (e == cudaSuccess && a.dD) e = launch_sum_partials(pD, a.dD, parts, 2LL * f.C, f.C, st);
-  if (e == cudaSuccess && a.ddt_bias)
-    e = launch_sum_partials(pD + f.C, a.ddt_bias, parts, 2LL * f.C, f.C, st);
-  return e;
+  const SumSegments out{{a.dA, a.dD, a.ddt_bias}, {(long long)f.C * f.N, f.C, f.C}};
+  return launch_sum_partials(pP, (long long)lay.sp.chunks * f.B, (long long)f.C * (f.N + 2), out,
+                             st);
 }
 
 }  // namespace

@@ -215,15 +215,13 @@ cudaError_t launch_short_conv_bwd(const ShortConvBwdArgs& a, cudaStream_t st) {
                                    : bwd_dispatch<float>(a, TT, tiles, st);
   if (e != cudaSuccess) return e;
   // dw rows 0 .. K - 1, dbias row K of every partial
-  const long long stride = (long long)(a.K + 1) * a.C;
-  e = launch_sum_partials(a.part, a.dw, (long long)a.B * tiles, stride, (long long)a.K * a.C, st);
-  if (e != cudaSuccess || !a.dbias) return e;
-  return launch_sum_partials(a.part + (size_t)a.K * a.C, a.dbias, (long long)a.B * tiles, stride,
-                             a.C, st);
+  const long long n = (long long)a.K * a.C;
+  const SumSegments out{{a.dw, a.dbias, nullptr}, {n, a.C, 0}};
+  return launch_sum_partials(a.part, (long long)a.B * tiles, n + a.C, out, st);
 }
 
 // ---------------------------------------------------------------------------
-// out[i] = sum_p part[p * stride + i], p in a fixed order
+// Sums of partial rows, in a fixed order
 // ---------------------------------------------------------------------------
 
 namespace {
@@ -232,13 +230,13 @@ constexpr int kSumCols = 32;   // columns of a block
 constexpr int kSumRows = 16;   // rows of threads, each over every 16th partial
 
 __global__ void __launch_bounds__(kSumCols * kSumRows)
-sum_partials_kernel(const float* __restrict__ part, float* __restrict__ out, long long parts,
-                    long long stride, long long n) {
+sum_partials_kernel(const float* __restrict__ part, const SumSegments out, long long parts,
+                    long long stride) {
   __shared__ float red[kSumRows][kSumCols];
   const int col = threadIdx.x % kSumCols, row = threadIdx.x / kSumCols;
   const long long i = (long long)blockIdx.x * kSumCols + col;
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-  if (i < n) {
+  if (i < stride) {
     long long p = row;
     for (; p + 3 * kSumRows < parts; p += 4 * kSumRows) {
       s0 += part[p * stride + i];
@@ -250,23 +248,27 @@ sum_partials_kernel(const float* __restrict__ part, float* __restrict__ out, lon
   }
   red[row][col] = (s0 + s1) + (s2 + s3);
   __syncthreads();
-  if (row == 0 && i < n) {
+  if (row == 0 && i < stride) {
     float s = 0.f;
 #pragma unroll
     for (int r = 0; r < kSumRows; ++r) s += red[r][col];
-    out[i] = s;
+    long long at = i;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (at >= 0 && at < out.n[k] && out.dst[k]) out.dst[k][at] = s;
+      at -= out.n[k];
+    }
   }
 }
 
 }  // namespace
 
-cudaError_t launch_sum_partials(const float* part, float* out, long long parts, long long stride,
-                                long long n, cudaStream_t st) {
-  if (n <= 0) return cudaSuccess;
-  const long long blocks = (n + kSumCols - 1) / kSumCols;
+cudaError_t launch_sum_partials(const float* part, long long parts, long long stride,
+                                const SumSegments& out, cudaStream_t st) {
+  if (stride <= 0) return cudaSuccess;
+  const long long blocks = (stride + kSumCols - 1) / kSumCols;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  sum_partials_kernel<<<(unsigned)blocks, kSumCols * kSumRows, 0, st>>>(part, out, parts, stride,
-                                                                        n);
+  sum_partials_kernel<<<(unsigned)blocks, kSumCols * kSumRows, 0, st>>>(part, out, parts, stride);
   return cudaGetLastError();
 }
 
