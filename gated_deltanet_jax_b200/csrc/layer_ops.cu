@@ -125,21 +125,23 @@ short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
     }
   }
   typename V::Raw nxt[kConvAhead];   // loads of four tokens in flight under four others' work
+  const Tin* xt = xb + (size_t)t0 * C;   // the next row to load
+  Tin* yt = y + ((size_t)b * T + t0) * C + c;
   auto fetch = [&](int tb) {
 #pragma unroll
     for (int i = 0; i < kConvAhead; ++i)
-      if (tb + i < t1) nxt[i] = V::load_raw(xb + (size_t)(tb + i) * C);
+      if (tb + i < t1) nxt[i] = V::load_raw(xt + (size_t)i * C);
+    xt += (size_t)kConvAhead * C;
   };
   fetch(t0);
   for (int tb = t0; tb < t1; tb += kConvAhead) {
     float2 cur[kConvAhead][N / 2];
 #pragma unroll
     for (int i = 0; i < kConvAhead; ++i) V::get(nxt[i], cur[i]);
-    fetch(tb + kConvAhead);
+    if (tb + kConvAhead < t1) fetch(tb + kConvAhead);
 #pragma unroll
-    for (int i = 0; i < kConvAhead; ++i) {
-      const int t = tb + i;
-      if (t >= t1) break;
+    for (int i = 0; i < kConvAhead; ++i, yt += C) {
+      if (tb + i >= t1) break;
       float out[N];
 #pragma unroll
       for (int e = 0; e < N / 2; ++e) {
@@ -150,7 +152,7 @@ short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
         out[2 * e] = act ? silu_acc(acc.x) : acc.x;
         out[2 * e + 1] = act ? silu_acc(acc.y) : acc.y;
       }
-      V::store(y + ((size_t)b * T + t) * C + c, out);
+      V::store(yt, out);
 #pragma unroll
       for (int j = 0; j + 1 < K - 1; ++j)
 #pragma unroll

@@ -88,61 +88,76 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
   }
   // Token t closes row s = t - (K - 1) of dxe: dxe[s] takes dpre[s .. t].
   const int tend = t1 + K - 1, tload = min(T, tend);
+  const size_t step = (size_t)kAhead * C;
+  const Tin* xt = x + (row0 + t0) * C + c;   // the next rows to load
+  const Tin* gt = dy + (row0 + t0) * C + c;
+  Tin* ot = dx + (row0 + t0) * C + c;        // the row of token tb
   Raw2<Tin> xr[kAhead], gr[kAhead];
   auto fetch = [&](int tb) {
-    const Tin* xp = x + (row0 + tb) * C + c;
-    const Tin* gp = dy + (row0 + tb) * C + c;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       xr[i].u = {};
       gr[i].u = {};
       if (tb + i < tload) {
-        xr[i] = ldr(xp + (size_t)i * C);
-        gr[i] = ldr(gp + (size_t)i * C);
+        xr[i] = ldr(xt + (size_t)i * C);
+        gr[i] = ldr(gt + (size_t)i * C);
       }
     }
+    xt += step;
+    gt += step;
+  };
+  // One token: dpre into the sums (own: a token of this tile) and the row it closes.
+  auto token = [&](float2 xv, float2 d, bool own) {
+    float2 pre = fma2(wk[K - 1], xv, bs);
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) pre = fma2(wk[j], win[j], pre);
+    if (act) {
+      const float2 sg = make_float2(fast_sigmoid(pre.x), fast_sigmoid(pre.y));
+      const float2 q = fma2(sg, make_float2(-1.f, -1.f), one);
+      d = mul2(mul2(d, sg), fma2(pre, q, one));
+    }
+    if (own) {
+      db = add2(db, d);
+      dw[K - 1] = fma2(d, xv, dw[K - 1]);
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) dw[j] = fma2(d, win[j], dw[j]);
+    }
+    // dxe[s] = w[0] dpre[t] + w[1] dpre[t - 1] + ...
+    float2 out = mul2(wk[0], d);
+#pragma unroll
+    for (int j = 1; j < K; ++j) out = fma2(wk[j], dwin[K - 1 - j], out);
+#pragma unroll
+    for (int j = 0; j + 1 < K - 1; ++j) {
+      win[j] = win[j + 1];
+      dwin[j] = dwin[j + 1];
+    }
+    if constexpr (K > 1) {
+      win[K - 2] = xv;
+      dwin[K - 2] = d;
+    }
+    return out;
   };
   fetch(t0);
-  for (int tb = t0; tb < tend; tb += kAhead) {
-    float2 xv[kAhead], gv[kAhead];
+  for (int tb = t0; tb < tend; tb += kAhead, ot += step) {
+    float2 xv[kAhead], gv[kAhead];   // (gradients past the last token are zero)
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       xv[i] = xr[i].get();
       gv[i] = gr[i].get();
     }
     if (tb + kAhead < tend) fetch(tb + kAhead);
+    if (tb >= t0 + K - 1 && tb + kAhead <= t1) {
+      // inside the tile: every token its own, every row closed one of dx
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        st2(ot + (i - (K - 1)) * (ptrdiff_t)C, token(xv[i], gv[i], true));
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int t = tb + i;
       if (t >= tend) break;
-      float2 pre = fma2(wk[K - 1], xv[i], bs);
-#pragma unroll
-      for (int j = 0; j < K - 1; ++j) pre = fma2(wk[j], win[j], pre);
-      float2 d = gv[i];   // zero past the last token
-      if (act) {
-        const float2 sg = make_float2(fast_sigmoid(pre.x), fast_sigmoid(pre.y));
-        const float2 q = fma2(sg, make_float2(-1.f, -1.f), one);
-        d = mul2(mul2(d, sg), fma2(pre, q, one));
-      }
-      if (t < t1) {
-        db = add2(db, d);
-        dw[K - 1] = fma2(d, xv[i], dw[K - 1]);
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j) dw[j] = fma2(d, win[j], dw[j]);
-      }
-      // dxe[s] = w[0] dpre[t] + w[1] dpre[t - 1] + ...
-      float2 out = mul2(wk[0], d);
-#pragma unroll
-      for (int j = 1; j < K; ++j) out = fma2(wk[j], dwin[K - 1 - j], out);
-#pragma unroll
-      for (int j = 0; j + 1 < K - 1; ++j) {
-        win[j] = win[j + 1];
-        dwin[j] = dwin[j + 1];
-      }
-      if constexpr (K > 1) {
-        win[K - 2] = xv[i];
-        dwin[K - 2] = d;
-      }
+      float2 out = token(xv[i], gv[i], t < t1);
       const int s = t - (K - 1);
       if (s < t0 && blockIdx.y != 0) continue;
       // the final window's rows are the inputs s = T - (K - 1) .. T - 1
@@ -186,11 +201,11 @@ cudaError_t bwd_dispatch(const ShortConvBwdArgs& a, int TT, int tiles, cudaStrea
   return cudaGetLastError();
 }
 
-// Token tiles: enough warps to keep loads in flight on every SM (24 a SM),
+// Token tiles: enough warps to keep loads in flight on every SM (36 a SM),
 // tiles of 16 to 512 tokens (a tile reads 2 (K - 1) rows more than it owns).
 int conv_bwd_tile(int B, int T, int C) {
   const long long warps_per_row = (C + kVec * 32 - 1) / (kVec * 32);
-  const long long want = 24LL * 148;
+  const long long want = 36LL * 148;
   long long tt = (long long)B * T * warps_per_row / want;
   tt = (tt + 15) / 16 * 16;
   if (tt < 16) tt = 16;
