@@ -44,7 +44,7 @@ enum GluMode : int {
 //   kDx   A = dg, du [M, K], B(n, k) = W[k, n]  (two passes over k);
 //   kDw   A(m, k) = dg[k, m], B(n, k) = x[k, n].
 template <typename T, int MODE, int TM>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __restrict__ B0,
                 const T* __restrict__ B1, T* __restrict__ O0, T* __restrict__ O1,
                 T* __restrict__ O2, int M, int N, int K, bool vec) {
@@ -52,7 +52,7 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
   constexpr int BNH = MODE == kFwd ? BN / 2 : BN;   // output columns of a tile
   constexpr int LV = BM * kBK / 4 / kThreads;       // vectors of a tile per thread
   constexpr int LD = BM + 4;
-  __shared__ float As[2][kBK][LD], Bs[2][kBK][LD];
+  __shared__ __align__(16) float As[2][kBK][LD], Bs[2][kBK][LD];
   const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
   const long long m0 = (long long)blockIdx.y * BM, n0 = (long long)blockIdx.x * BNH;
   const int ksteps = (K + kBK - 1) / kBK;
@@ -101,11 +101,12 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
     }
   };
 
-  float acc[TM][TM];
+  // pairs of columns: two multiply-adds an instruction
+  float2 acc2[TM][TM / 2];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TM; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < TM / 2; ++j) acc2[i][j] = make_float2(0.f, 0.f);
 
   if (total > 0) {
     fetch(0);
@@ -117,18 +118,23 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
     if (s + 1 < total) fetch(s + 1);
 #pragma unroll
     for (int k = 0; k < kBK; ++k) {
-      float a[TM], b[TM];
+      float a[TM];
+      float2 b[TM / 2];
 #pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = As[buf][k][ty * TM + i];
+      for (int i = 0; i < TM; i += 4) {
+        const float4 v = load4(&As[buf][k][ty * TM + i]);
+        a[i] = v.x; a[i + 1] = v.y; a[i + 2] = v.z; a[i + 3] = v.w;
+      }
 #pragma unroll
-      for (int j = 0; j < H; ++j) {
-        b[j] = Bs[buf][k][tx * H + j];
-        b[H + j] = Bs[buf][k][BN / 2 + tx * H + j];
+      for (int j = 0; j < H; j += 2) {
+        b[j / 2] = *reinterpret_cast<const float2*>(&Bs[buf][k][tx * H + j]);
+        b[(H + j) / 2] = *reinterpret_cast<const float2*>(&Bs[buf][k][BN / 2 + tx * H + j]);
       }
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        for (int j = 0; j < TM / 2; ++j)
+          acc2[i][j] = fma2(make_float2(a[i], a[i]), b[j], acc2[i][j]);
     }
     if (s + 1 < total) put(buf ^ 1);
     __syncthreads();
@@ -138,12 +144,18 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
   for (int i = 0; i < TM; ++i) {
     const long long m = m0 + ty * TM + i;
     if (m >= M) continue;
+    float acc[TM];
+#pragma unroll
+    for (int j = 0; j < TM / 2; ++j) {
+      acc[2 * j] = acc2[i][j].x;
+      acc[2 * j + 1] = acc2[i][j].y;
+    }
 #pragma unroll
     for (int j = 0; j < H; ++j) {
       if (MODE == kFwd) {
         const long long n = n0 + tx * H + j;
         if (n >= N) continue;
-        const float g = acc[i][j], u = acc[i][H + j];
+        const float g = acc[j], u = acc[H + j];
         const float sg = 1.f / (1.f + expf(-g));
         O0[m * N + n] = from_f32<T>(g * sg * u);
         if (O1) {
@@ -155,7 +167,7 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const long long n = n0 + hf * (BN / 2) + tx * H + j;
-          if (n < N) O[m * N + n] = from_f32<T>(acc[i][hf * H + j]);
+          if (n < N) O[m * N + n] = from_f32<T>(acc[hf * H + j]);
         }
       }
     }
