@@ -143,7 +143,7 @@ def _declare(lib):
     lib.gdn_glu_fwd.restype = _i
     lib.gdn_glu_bwd.argtypes = [_vp] * 9 + [_i] * 4 + [_vp, _sz, _vp]
     lib.gdn_glu_bwd.restype = _i
-    lib.gdn_glu_bwd_workspace_bytes.argtypes = [_i] * 3
+    lib.gdn_glu_bwd_workspace_bytes.argtypes = [_i] * 4
     lib.gdn_glu_bwd_workspace_bytes.restype = _sz
     lib.gdn_selective_scan_fwd.argtypes = [_vp] * 12 + [_i] * 7 + [_vp, _sz, _vp]
     lib.gdn_selective_scan_fwd.restype = _i

@@ -177,9 +177,11 @@ int check_glu(const void* x, const void* wg, const void* wu, int M, int D, int I
   g_err[0] = '\0';
   if (M < 0 || D < 0 || I < 0) return fail(GDN_ERR_INVALID, "negative size M=%d D=%d I=%d", M, D, I);
   if (int rc = check_dtype(dtype)) return rc;
-  // (the CUDA-core form's grid: 65535 row tiles of 64)
-  if (M > 65535 * 64 || I > 65535 * 64 || D > 65535 * 64)
-    return fail(GDN_ERR_UNSUPPORTED, "M=%d, D=%d or I=%d exceeds %d", M, D, I, 65535 * 64);
+  // (the CUDA-core form's grid: 65535 row tiles of 64; the tensor-core form's row indexes)
+  const bool tc = dtype == GDN_DTYPE_BF16 && D % 8 == 0 && I % 8 == 0;
+  const int most = tc ? 1 << 30 : 65535 * 64;
+  if (M > most || I > most || D > most)
+    return fail(GDN_ERR_UNSUPPORTED, "M=%d, D=%d or I=%d exceeds %d", M, D, I, most);
   if ((long long)M * (D > I ? D : I) > (1LL << 40) || (long long)I * D > (1LL << 40))
     return fail(GDN_ERR_INVALID, "tensor too large (more than 2^40 elements)");
   if (D > 0 && ((M > 0 && !x) || (I > 0 && (!wg || !wu))))
@@ -849,9 +851,11 @@ int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, vo
   return cuda_status(gdn::launch_glu_fwd(a, (cudaStream_t)stream), "gdn_glu_fwd");
 }
 
-size_t gdn_glu_bwd_workspace_bytes(int M, int I, int dtype) {
-  if (M <= 0 || I <= 0) return 0;
-  return 2 * glu_half_bytes(M, I, dtype);
+size_t gdn_glu_bwd_workspace_bytes(int M, int D, int I, int dtype) {
+  if (M <= 0 || D < 0 || I <= 0) return 0;
+  const int parts = gdn::glu_dw_parts(M, D, I, dtype);
+  return 2 * glu_half_bytes(M, I, dtype) +
+         (parts > 1 ? (size_t)parts * 2 * I * D * sizeof(float) : 0);
 }
 
 int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void* g, const void* u,
@@ -869,13 +873,14 @@ int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void*
     for (const void* p : ptrs)
       if (!p || !aligned16(p))
         return fail(GDN_ERR_INVALID, "g, u and dh must be non-NULL and 16-byte aligned");
-    rc = check_workspace(workspace, ws_bytes, gdn_glu_bwd_workspace_bytes(M, I, dtype),
+    rc = check_workspace(workspace, ws_bytes, gdn_glu_bwd_workspace_bytes(M, D, I, dtype),
                          "gdn_glu_bwd_workspace_bytes");
     if (rc) return rc;
   }
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  gdn::GluBwdArgs a{x, w_gate, w_up, g, u, dh, ws, ws ? ws + glu_half_bytes(M, I, dtype) : nullptr,
-                    dx, dw_gate, dw_up, M, D, I, dtype};
+  const size_t half = glu_half_bytes(M, I, dtype);
+  gdn::GluBwdArgs a{x, w_gate, w_up, g, u, dh, ws, ws ? ws + half : nullptr, dx, dw_gate, dw_up,
+                    reinterpret_cast<float*>(ws ? ws + 2 * half : nullptr), M, D, I, dtype};
   return cuda_status(gdn::launch_glu_bwd(a, (cudaStream_t)stream), "gdn_glu_bwd");
 }
 

@@ -36,7 +36,7 @@ __device__ __forceinline__ void load_vec(const T* p, int n, bool vec, float (&v)
 enum GluMode : int {
   kFwd = 0,    // [g | u] = x [Wg | Wu]^T, h out (g, u out when asked for)
   kDx = 1,     // dx = dg Wg + du Wu
-  kDw = 2,     // dWg = dg^T x (blockIdx.z = 0), dWu = du^T x (blockIdx.z = 1)
+  kDw = 2,     // dWg = dg^T x (even blockIdx.z), dWu = du^T x (odd), over the K rows of part z / 2
 };
 
 // out [M, N] = sum_k A(m, k) B(n, k).  A and B per mode:
@@ -47,7 +47,7 @@ template <typename T, int MODE, int TM>
 __global__ void __launch_bounds__(kThreads, 2)
 glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __restrict__ B0,
                 const T* __restrict__ B1, T* __restrict__ O0, T* __restrict__ O1,
-                T* __restrict__ O2, int M, int N, int K, bool vec) {
+                T* __restrict__ O2, int M, int N, int K, int kpart, bool vec) {
   constexpr int BM = 16 * TM, BN = 16 * TM, H = TM / 2;
   constexpr int BNH = MODE == kFwd ? BN / 2 : BN;   // output columns of a tile
   constexpr int LV = BM * kBK / 4 / kThreads;       // vectors of a tile per thread
@@ -55,13 +55,16 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
   __shared__ __align__(16) float As[2][kBK][LD], Bs[2][kBK][LD];
   const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
   const long long m0 = (long long)blockIdx.y * BM, n0 = (long long)blockIdx.x * BNH;
-  const int ksteps = (K + kBK - 1) / kBK;
+  // kDw: this block's share of the contraction (kpart rows of it)
+  const int kbeg = MODE == kDw ? (int)(blockIdx.z / 2) * kpart : 0;
+  const int kend = MODE == kDw ? min(K, kbeg + kpart) : K;
+  const int ksteps = (kend - kbeg + kBK - 1) / kBK;
   const int total = MODE == kDx ? 2 * ksteps : ksteps;
   float ra[LV][4], rb[LV][4];
 
   auto fetch = [&](int s) {
-    const bool second = MODE == kDx ? s >= ksteps : (MODE == kDw ? blockIdx.z != 0 : false);
-    const int k0 = (MODE == kDx && second ? s - ksteps : s) * kBK;
+    const bool second = MODE == kDx ? s >= ksteps : (MODE == kDw ? blockIdx.z % 2 != 0 : false);
+    const int k0 = kbeg + (MODE == kDx && second ? s - ksteps : s) * kBK;
     const T* A = second ? A1 : A0;
     const T* B = MODE == kDx && second ? B1 : B0;
 #pragma unroll
@@ -79,9 +82,9 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
       if (MODE != kFwd) {  // rows over k: four consecutive columns of one row
         const int k = k0 + idx / (BM / 4), c = idx % (BM / 4) * 4;
         if (MODE == kDw)
-          load_vec(A + (long long)k * M + m0 + c, k < K ? (int)min(4LL, M - m0 - c) : 0, vec,
+          load_vec(A + (long long)k * M + m0 + c, k < kend ? (int)min(4LL, M - m0 - c) : 0, vec,
                    ra[i]);
-        load_vec(B + (long long)k * N + n0 + c, k < K ? (int)min(4LL, N - n0 - c) : 0, vec, rb[i]);
+        load_vec(B + (long long)k * N + n0 + c, k < kend ? (int)min(4LL, N - n0 - c) : 0, vec, rb[i]);
       }
     }
   };
@@ -163,7 +166,8 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
           O2[m * N + n] = from_f32<T>(u);
         }
       } else {
-        T* O = MODE == kDw && blockIdx.z ? O1 : O0;
+        T* O = MODE == kDw && blockIdx.z % 2 ? O1 : O0;
+        if (MODE == kDw) O += (long long)(blockIdx.z / 2) * 2 * M * N;   // (the parts' sums)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const long long n = n0 + hf * (BN / 2) + tx * H + j;
@@ -174,25 +178,30 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
   }
 }
 
+// Tiles of 128 do four times the products per shared-memory word of tiles of 64;
+// the small tiles only where the big ones leave SMs idle.
+bool big_tiles(int mode, int M, int N) {
+  const long long rows = mode == kFwd ? 64 : 128;
+  return (N + rows - 1) / rows * ((M + 127LL) / 128) * (mode == kDw ? 2 : 1) >= 148;
+}
+
 template <typename T, int MODE>
 cudaError_t launch_simt(const T* A0, const T* A1, const T* B0, const T* B1, T* O0, T* O1, T* O2,
-                        int M, int N, int K, cudaStream_t st) {
+                        int M, int N, int K, int parts, cudaStream_t st) {
   // 16-byte (fp32) or 8-byte (bf16) vectors need rows that are a multiple of four elements
   const bool vec = MODE == kDw ? (M % 4 == 0 && N % 4 == 0)
                                : (K % 4 == 0 && (MODE == kFwd || N % 4 == 0));
-  const int z = MODE == kDw ? 2 : 1;
+  const int z = MODE == kDw ? 2 * parts : 1;
+  const int kpart = ((K + parts - 1) / parts + kBK - 1) / kBK * kBK;
   const long long rows = MODE == kFwd ? 64 : 128;
-  const long long big = (N + rows - 1) / rows * ((M + 127LL) / 128) * z;
-  // Tiles of 128 do four times the products per shared-memory word of tiles of
-  // 64; the small tiles only where the big ones leave SMs idle.
-  if (big >= 148) {
+  if (big_tiles(MODE, M, N)) {
     const dim3 grid((unsigned)((N + rows - 1) / rows), (unsigned)((M + 127LL) / 128), z);
     glu_simt_kernel<T, MODE, 8><<<grid, kThreads, 0, st>>>(A0, A1, B0, B1, O0, O1, O2, M, N, K,
-                                                           vec);
+                                                           kpart, vec);
   } else {
     const dim3 grid((unsigned)((N + rows / 2 - 1) / (rows / 2)), (unsigned)((M + 63LL) / 64), z);
     glu_simt_kernel<T, MODE, 4><<<grid, kThreads, 0, st>>>(A0, A1, B0, B1, O0, O1, O2, M, N, K,
-                                                           vec);
+                                                           kpart, vec);
   }
   return cudaGetLastError();
 }
@@ -234,7 +243,7 @@ template <typename T>
 cudaError_t fwd_simt(const GluArgs& a, cudaStream_t st) {
   return launch_simt<T, kFwd>(static_cast<const T*>(a.x), nullptr, static_cast<const T*>(a.wg),
                               static_cast<const T*>(a.wu), static_cast<T*>(a.h),
-                              static_cast<T*>(a.g), static_cast<T*>(a.u), a.M, a.I, a.D, st);
+                              static_cast<T*>(a.g), static_cast<T*>(a.u), a.M, a.I, a.D, 1, st);
 }
 
 template <typename T>
@@ -259,14 +268,35 @@ cudaError_t bwd_products_simt(const GluBwdArgs& a, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   if (a.dx)
     e = launch_simt<T, kDx>(dg, du, wg, wu, static_cast<T*>(a.dx), nullptr, nullptr, a.M, a.D,
-                            a.I, st);
-  if (e == cudaSuccess && a.dwg)
-    e = launch_simt<T, kDw>(dg, du, x, nullptr, static_cast<T*>(a.dwg), static_cast<T*>(a.dwu),
-                            nullptr, a.I, a.D, a.M, st);
-  return e;
+                            a.I, 1, st);
+  if (e != cudaSuccess || !a.dwg) return e;
+  T *dwg = static_cast<T*>(a.dwg), *dwu = static_cast<T*>(a.dwu);
+  const int parts = glu_dw_parts(a.M, a.D, a.I, a.dtype);
+  const long long n = (long long)a.I * a.D;
+  if (parts > 1) {
+    dwg = reinterpret_cast<T*>(a.part);
+    dwu = dwg + n;
+  }
+  e = launch_simt<T, kDw>(dg, du, x, nullptr, dwg, dwu, nullptr, a.I, a.D, a.M, parts, st);
+  if (e != cudaSuccess || parts == 1) return e;
+  const SumSegments out{{static_cast<float*>(a.dwg), static_cast<float*>(a.dwu), nullptr},
+                        {n, n, 0}};
+  return launch_sum_partials(a.part, parts, 2 * n, out, st);
 }
 
 }  // namespace
+
+// The weights' gradients in fp32 contract over the tokens: few output tiles leave
+// SMs idle, and the tokens are cut into parts (of 512 or more) whose sums a second
+// kernel adds up (10000 x 128 x 330: 0.5 ms in one part).
+int glu_dw_parts(int M, int D, int I, int dtype) {
+  if (dtype != kFP32 || M < 1024 || big_tiles(kDw, I, D)) return 1;
+  const long long tiles = 2LL * ((I + 63) / 64) * ((D + 63) / 64);
+  if (tiles >= 148) return 1;
+  long long p = 296 / tiles;
+  if (p > M / 512) p = M / 512;
+  return p < 1 ? 1 : p > 16 ? 16 : (int)p;
+}
 
 cudaError_t launch_glu_fwd(const GluArgs& a, cudaStream_t st) {
   if (a.M == 0 || a.I == 0) return cudaSuccess;

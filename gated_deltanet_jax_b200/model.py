@@ -88,8 +88,9 @@ def _plain_linear(m: nn.Module, dtype) -> bool:
 class ShortConvolution(nn.Module):
     """Causal depthwise convolution over time, kernel K, then SiLU (model.py:15-40).
     ``weight`` [K, C] (the Flax depthwise kernel [K, 1, C] squeezed), optional bias.
-    On the GPU kernels (gdn_short_conv_fwd, gdn_short_conv_bwd) at the shapes they
-    take; torch's conv1d elsewhere."""
+    On the GPU kernel (gdn_short_conv_fwd) for inference without a bias, and with its
+    backward (gdn_short_conv_bwd) for training at the shapes they take; torch's
+    conv1d elsewhere."""
 
     def __init__(self, hidden_size: int, kernel_size: int, activation: Optional[str] = "silu",
                  use_bias: bool = False):
@@ -109,7 +110,7 @@ class ShortConvolution(nn.Module):
                                          activation="silu" if act else None)
             return y
         K, C = self.weight.shape
-        if (K <= 8 and C % (8 if x.dtype == torch.bfloat16 else 4) == 0
+        if (grad and K <= 8 and C % (8 if x.dtype == torch.bfloat16 else 4) == 0
                 and _kernel_call_ok(x, self.weight)):
             y, _ = ops.short_convolution(x, self.weight, bias=self.bias,
                                          activation="silu" if act else None)

@@ -677,7 +677,7 @@ class _GluFn(torch.autograd.Function):
         lib = _lib.load()
         dev = x.get_device()
         with _on_device(dev):
-            n = lib.gdn_glu_bwd_workspace_bytes(M, I, _DTYPES[x.dtype])
+            n = lib.gdn_glu_bwd_workspace_bytes(M, D, I, _DTYPES[x.dtype])
             ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
             rc = lib.gdn_glu_bwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(g), _ptr(u), _ptr(dh),
                                  _ptr(dx), _ptr(dwg), _ptr(dwu), M, D, I, _DTYPES[x.dtype],

@@ -416,7 +416,9 @@ int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
  * x [M, D], w_gate, w_up [I, D] (torch's [out, in]; the flax kernels
  * transposed), h [M, I], all bf16 or all fp32, products summed in fp32.  g and
  * u [M, I] (both or neither) receive the two projections for the backward, in
- * the same dtype.
+ * the same dtype.  Outputs overlap no input.  bf16 with D and I multiples of 8
+ * runs on the tensor cores (sizes up to 2^30), the rest on CUDA cores (up to
+ * 65535 * 64).
  */
 int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, void* g, void* u,
                 int M, int D, int I, int dtype, void* stream);
@@ -424,10 +426,10 @@ int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, vo
 /*
  * Its gradients from dh [M, I] and the forward's g and u: dx [M, D] (NULL: not
  * wanted), dw_gate and dw_up [I, D] (both or neither), in the inputs' dtype.
- * `workspace`: gdn_glu_bwd_workspace_bytes() bytes (the gradients of g and u,
- * in the inputs' dtype).
+ * `workspace`: gdn_glu_bwd_workspace_bytes() bytes (the gradients of g and u in
+ * the inputs' dtype; partial sums of the weights' where those need them).
  */
-size_t gdn_glu_bwd_workspace_bytes(int M, int I, int dtype);
+size_t gdn_glu_bwd_workspace_bytes(int M, int D, int I, int dtype);
 int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void* g, const void* u,
                 const void* dh, void* dx, void* dw_gate, void* dw_up, int M, int D, int I,
                 int dtype, void* workspace, size_t ws_bytes, void* stream);

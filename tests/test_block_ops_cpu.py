@@ -97,12 +97,14 @@ def test_glu_rejects_bad_arguments(lib):
     assert fwd(M=-1) == INVALID and fwd(dtype=5) == INVALID
     assert fwd(x=None) == INVALID and fwd(wg=BAD) == INVALID and fwd(h=BAD) == INVALID
     assert fwd(g=P) == INVALID                       # u missing
-    assert fwd(M=65535 * 64 + 1) == UNSUPPORTED
+    assert fwd(M=65535 * 64 + 1, dtype=FP32) == UNSUPPORTED
+    assert fwd(M=65535 * 64 + 1, D=60) == UNSUPPORTED      # no multiple of 8: CUDA cores
+    assert fwd(M=(1 << 30) + 1) == UNSUPPORTED
     assert fwd(M=0) == OK and fwd(I=0) == OK
 
     def bwd(ws=P, n=1 << 20, g=P, dh=P, dx=P, dwg=P, dwu=P, M=4, D=64, I=32, dtype=BF16):
         return lib.gdn_glu_bwd(P, P, P, g, P, dh, dx, dwg, dwu, M, D, I, dtype, ws, n, None)
-    need = lib.gdn_glu_bwd_workspace_bytes(4, 32, BF16)
+    need = lib.gdn_glu_bwd_workspace_bytes(4, 64, 32, BF16)
     assert need >= 2 * 4 * 32 * 2
     assert bwd(n=need - 1) == INVALID and bwd(ws=None) == INVALID and bwd(ws=BAD) == INVALID
     assert bwd(g=None) == INVALID and bwd(dh=BAD) == INVALID and bwd(dwu=None) == INVALID

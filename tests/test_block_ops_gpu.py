@@ -44,7 +44,7 @@ def _within(out, ref, tol, what):
 
 GLU = [(1, 64, 64), (1, 2048, 136), (2, 256, 96), (3, 40, 24), (7, 250, 66), (33, 128, 200),
        (64, 64, 128), (127, 72, 56), (128, 128, 128), (129, 192, 320), (257, 520, 264),
-       (300, 33, 17), (1000, 256, 768), (5, 1600, 4808), (37, 2048, 136), (2, 136, 9600)]
+       (300, 33, 17), (1000, 256, 768), (5, 1600, 4808), (37, 2048, 136), (2, 136, 9600), (4099, 72, 40)]
 
 
 def _glu_inputs(M, D, I, dtype, dev, seed):
