@@ -247,13 +247,34 @@ scan_chain_kernel(float* __restrict__ state, const float* __restrict__ sum,
   if (row >= rows) return;
   const float a2 = n < N ? A[(row % C) * N + n] * kLog2e : 0.f;
   float h = n < N && first ? first[row * N + n] : 0.f;
-  for (int s = 0; s < nchunk; ++s) {
-    const long long k = kReverse ? nchunk - 1 - s : s;
-    float* p = state + k * rows * NP + i;
-    const float loc = s + 1 < nchunk ? *p : 0.f;
-    const float dec = s + 1 < nchunk ? ex2(a2 * sum[k * rows + row]) : 0.f;
-    *p = h;
-    h = fmaf(dec, h, loc);
+  constexpr int kAt = 8;   // chunks whose loads are in flight under eight others' steps
+  float loc[kAt], dec[kAt];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int j = 0; j < kAt; ++j) {
+      const int s = s0 + j;
+      const long long k = kReverse ? nchunk - 1 - s : s;
+      const bool on = s + 1 < nchunk;
+      loc[j] = on ? state[k * rows * NP + i] : 0.f;
+      dec[j] = on ? sum[k * rows + row] : 0.f;
+    }
+  };
+  fetch(0);
+  for (int s0 = 0; s0 < nchunk; s0 += kAt) {
+    float l[kAt], d[kAt];
+#pragma unroll
+    for (int j = 0; j < kAt; ++j) {
+      l[j] = loc[j];
+      d[j] = ex2(a2 * dec[j]);
+    }
+    fetch(s0 + kAt);
+#pragma unroll
+    for (int j = 0; j < kAt; ++j) {
+      const int s = s0 + j;
+      if (s >= nchunk) break;
+      state[(kReverse ? nchunk - 1 - s : s) * rows * NP + i] = h;
+      h = fmaf(d[j], h, l[j]);
+    }
   }
 }
 

@@ -435,6 +435,7 @@ sum_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict_
   const int g = (int)(rg % G);
   const long long row = rg / G;
   float s = 0.f;
+#pragma unroll 8
   for (int t = 0; t < tiles; ++t)
     s += part[(((long long)g * tiles + t) * rows + row) * (2 * NP) + n];
   T* out = n < NP ? dB : dC;
