@@ -367,16 +367,17 @@ cudaError_t fwd_dispatch(const ScanArgs& a, cudaStream_t st) {
 }  // namespace
 
 // How a row is cut.  Whole rows are bound by one warp's walk until about three
-// blocks share an SM (2048 tokens, 16 states: 0.24 ms from 1 to 256 blocks, 0.31 at
-// 512), while a cut row costs 1.4 (forward) to 1.2 times the work; cutting into
-// two waves of blocks measured better than one (256 blocks: forward 0.21 against
-// 0.23, backward 0.59 against 0.70 and 0.98 ms whole; 8192 tokens, 512 blocks:
-// forward 1.42 against 1.22 ms whole, backward 4.3 against 4.6).
+// blocks share an SM (2048 tokens, 16 states: 0.24 ms forward from 1 to 256 blocks,
+// 0.31 at 512), while a cut row costs 1.4 (forward) to 1.2 times the work.  The
+// chunks make two waves of the forward's blocks (seven an SM) and four of the
+// backward's (four an SM), which measured best: at 256 blocks the forward takes
+// 0.21 ms cut, 0.24 whole, the backward 0.54 and 0.98; at 8192 tokens and 512 blocks
+// the forward 1.42 cut, 1.22 whole, the backward 3.9 and 4.6.
 ScanSplit scan_split(int B, int T, int C, int G, bool backward) {
   const long long blocks = (long long)((C / G + kScanCh - 1) / kScanCh) * G * B;
   ScanSplit s{1, T};
   if (T <= 0 || blocks <= 0 || blocks > (backward ? 512 : 384)) return s;
-  const long long want = (148LL * (backward ? 12 : 14) + blocks - 1) / blocks;
+  const long long want = (148LL * (backward ? 16 : 14) + blocks - 1) / blocks;
   long long tokens = (T + want - 1) / want;
   if (tokens < 128) tokens = 128;   // a chunk's launch and chaining against its walk
   tokens = (tokens + 31) / 32 * 32;

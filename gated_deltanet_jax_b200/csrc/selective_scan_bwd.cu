@@ -14,8 +14,9 @@
 // the states in registers, then the adjoint recurrence backwards.  Rows that
 // leave most SMs idle are cut as in the forward, the chunks' adjoint states
 // chained from the end.  Bound by issue slots and exponentials: two to three
-// exponentials and about a dozen multiply-adds a state and token, and seven
-// shuffles a token that sum dB and dC over a warp's 16 channels.  Sums over
+// exponentials and about a dozen multiply-adds a state and token, and the sums
+// of dB and dC over the block's channels, which go through shared memory half a
+// tile at a time (shuffles took 31 instructions a token for them, this takes 15).  Sums over
 // channels, rows and tokens leave as one partial per block and are added up in a
 // fixed order by further kernels: no atomics, the same bits on every run.
 #include "selective_scan_common.cuh"
@@ -24,50 +25,13 @@ namespace gdn {
 
 namespace {
 
-// Reduces NV values per lane over the eight channels of a warp (lane bits 2 to
-// 4), halving the values kept where it can; afterwards the lane holds
-// max(1, NV / 8) totals, value index first + i.
-template <int NV>
-struct ChanSum {
-  static constexpr int K1 = NV >= 2 ? NV / 2 : 1;
-  static constexpr int K2 = NV >= 4 ? NV / 4 : 1;
-  static constexpr int K3 = NV >= 8 ? NV / 8 : 1;
-  template <int NI, int NO>
-  __device__ __forceinline__ static void half(const float (&v)[NI], float (&o)[NO], int mask,
-                                              bool up) {
-    if constexpr (NI == 2 * NO) {
-#pragma unroll
-      for (int i = 0; i < NO; ++i) {
-        const float keep = up ? v[NO + i] : v[i], give = up ? v[i] : v[NO + i];
-        o[i] = keep + __shfl_xor_sync(0xffffffffu, give, mask);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NO; ++i) o[i] = v[i] + __shfl_xor_sync(0xffffffffu, v[i], mask);
-    }
-  }
-  __device__ __forceinline__ static void run(const float (&v)[NV], float (&o)[K3], int lane) {
-    float p[K1], q[K2];
-    half(v, p, 4, (lane & 4) != 0);
-    half(p, q, 8, (lane & 8) != 0);
-    half(q, o, 16, (lane & 16) != 0);
-  }
-  __device__ __forceinline__ static int first(int lane) {
-    int f = 0;
-    if (NV >= 2 && (lane & 4)) f += NV / 2;
-    if (NV >= 4 && (lane & 8)) f += NV / 4;
-    if (NV >= 8 && (lane & 16)) f += NV / 8;
-    return f;
-  }
-};
-
 constexpr int kBwdThreads = 64;   // 16 slots of four lanes, two channels a lane
-constexpr int kBwdWarps = kBwdThreads / 32;
+constexpr int kBwdSlots = kBwdThreads / kScanLanes;
 
 // kLocal: the first pass of a cut row (chunks 1 ..: the adjoint from zero over
 // the chunk and the steps' sum out, no gradients).
 template <typename T, int NL, bool kLocal>
-__global__ void __launch_bounds__(kBwdThreads, NL <= 4 ? 6 : 4)
+__global__ void __launch_bounds__(kBwdThreads, 4)
 scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, int nchunk,
                 float* __restrict__ pBC, float* __restrict__ pP) {
   constexpr int CK = scan_tile<NL>(), SUB = CK / 2;
@@ -80,14 +44,16 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
   __shared__ __align__(16) float sG[CK][kScanCh];         // dyp
   __shared__ __align__(16) float sB[CK][NP], sC[CK][NP];
   __shared__ __align__(16) float sPar[2][kScanCh];        // dt_bias, D
-  // x, sigmoid(dt + bias), dy silu'(z); sum C h, sum r B, sum r a h A; a warp's dB and dC
+  // x, sigmoid(dt + bias), dy silu'(z); sum C h, sum r B, sum r a h A
   __shared__ __align__(16) float sK[kLocal ? 1 : 3][CK][kScanCh];
   __shared__ __align__(16) float sO[kLocal ? 1 : 3][CK][kScanCh + 8];
-  __shared__ __align__(16) float sRed[kLocal ? 1 : kBwdWarps][CK][2 * NP];
+  // the lanes' dB and dC of half a tile, in vectors of VW
+  constexpr int VW = NL >= 2 ? 4 : 2, PARTS = 2 * NL / VW;
+  __shared__ __align__(16) float sV[kLocal ? 1 : SUB][PARTS][kBwdThreads][VW];
   __shared__ __align__(16) float sSum[2][kBwdThreads / 8][kScanCh];
 
   const ScanArgs& f = a.fwd;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int Cg = f.C / f.G;
   const int grp = blockIdx.x / tiles_per_group;
   const int cl0 = (blockIdx.x % tiles_per_group) * kScanCh;
@@ -318,20 +284,18 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
             rb[c][j] = sb.x + sb.y;
             fa[c][j] = sa.x + sa.y;
           }
-          float v[2 * NL];
+          if constexpr (NL == 1) {
+            *reinterpret_cast<float2*>(sV[tl][0][tid]) = make_float2(dBv[0].x, dCv[0].x);
+          } else if constexpr (NL == 2) {
+            store4(sV[tl][0][tid], make_float4(dBv[0].x, dBv[0].y, dCv[0].x, dCv[0].y));
+          } else {
 #pragma unroll
-          for (int i = 0; i < NL; ++i) {
-            v[i] = pair_at(dBv[i / 2], i & 1);
-            v[NL + i] = pair_at(dCv[i / 2], i & 1);
-          }
-          using CS = ChanSum<2 * NL>;
-          float tot[CS::K3];
-          CS::run(v, tot, lane);
-          const int first = CS::first(lane);
-#pragma unroll
-          for (int i = 0; i < CS::K3; ++i) {
-            const int w = first + i;   // < NL: dB of state q NL + w, else dC
-            sRed[warp][t][w < NL ? q * NL + w : NP + q * NL + w - NL] = tot[i];
+            for (int i = 0; i < NL / 4; ++i) {
+              store4(sV[tl][i][tid], make_float4(dBv[2 * i].x, dBv[2 * i].y, dBv[2 * i + 1].x,
+                                                 dBv[2 * i + 1].y));
+              store4(sV[tl][NL / 4 + i][tid], make_float4(dCv[2 * i].x, dCv[2 * i].y,
+                                                          dCv[2 * i + 1].x, dCv[2 * i + 1].y));
+            }
           }
         }
         const int t = base + g0 + q;
@@ -348,17 +312,38 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
         s1 = quad_sum4(fa[1][0], fa[1][1], fa[1][2], fa[1][3], lane);
         if (q < QT) *reinterpret_cast<float2*>(&sO[2][t][chl]) = make_float2(s0, s1);
       }
-    }
-    __syncthreads();
-    // the block's dB and dC of the tile
-    for (int i = tid; i < CK * 2 * NP; i += kBwdThreads) {
-      const int tl = i / (2 * NP), n = i % (2 * NP);
-      if (t0 + tl < tend) {
-        float sum = 0.f;
+      __syncthreads();
+      // The half's dB and dC: a thread sums one vector of one token over the 16 slots,
+      // from a slot of its own on, so that the threads' reads fall on other banks.
+      if (tid < SUB * PARTS * kScanLanes) {
+        const int qu = tid % kScanLanes, part = tid / kScanLanes % PARTS;
+        const int tl = tid / (kScanLanes * PARTS), t = t0 + base + tl;
+        float sum[VW] = {};
 #pragma unroll
-        for (int w = 0; w < kBwdWarps; ++w) sum += sRed[w][tl][n];
-        pBC[(((size_t)blockIdx.x * f.B + b) * f.T + t0 + tl) * (2 * NP) + n] = sum;
+        for (int i = 0; i < kBwdSlots; ++i) {
+          const int sl = (i + tid / kScanLanes) % kBwdSlots;
+          const float* v = sV[tl][part][sl * kScanLanes + qu];
+          if constexpr (VW == 4) {
+            const float4 w = load4(v);
+            sum[0] += w.x; sum[1] += w.y; sum[2] += w.z; sum[3] += w.w;
+          } else {
+            const float2 w = *reinterpret_cast<const float2*>(v);
+            sum[0] += w.x; sum[1] += w.y;
+          }
+        }
+        if (t < tend) {
+          float* o = pBC + (((size_t)blockIdx.x * f.B + b) * f.T + t) * (2 * NP) + qu * NL;
+          if constexpr (NL >= 4) {
+            constexpr int H = PARTS / 2;
+            store4(o + (part < H ? part * 4 : NP + (part - H) * 4),
+                   make_float4(sum[0], sum[1], sum[2], sum[3]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < VW; ++e) o[e < NL ? e : NP + e - NL] = sum[e];
+          }
+        }
       }
+      __syncthreads();
     }
     // dx, ddt, dz
     if (stages) {
