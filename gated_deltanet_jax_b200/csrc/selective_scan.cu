@@ -8,13 +8,19 @@
 // What it has to move is x, dt, z and y once (8 bytes a token and channel in
 // bf16); what it has to compute is one exponential and four multiply-adds per
 // state, which at N = 16 takes longer than the bytes (16 exponentials a clock
-// and SM: 0.24 ms for 8 x 2048 x 4096 against 0.08 ms for its bytes).  Four lanes
-// share a channel, each with a quarter of its states in registers as pairs (two
-// multiply-adds an instruction).  A block owns 32 channels of one row and walks
-// tiles of 32 tokens: every thread forms delta and delta x of eight (token,
-// channel) pairs into shared memory with the next tile's loads in flight, all
-// lanes then run the recurrence over the tile, and four tokens' read-outs at a
-// time are summed over the four lanes in three shuffles.
+// and SM: 0.30 ms with the gates' for 8 x 2048 x 4096 against 0.08 ms for its
+// bytes).  Four lanes share a channel, each with a quarter of its states in
+// registers as pairs (two multiply-adds an instruction), and a lane serves two
+// channels with each row of B and C that it reads: a 16-byte read takes four
+// shared-memory cycles of a warp whatever its lanes share, and with one channel a
+// lane those cycles (87 % busy) set the time.  A block owns 32 channels of one row
+// and walks tiles of 32 tokens: every thread forms delta and delta x of its share
+// into shared memory with the next tile's loads in flight, all lanes then run the
+// recurrence over the tile, and four tokens' read-outs at a time are summed over
+// the four lanes in three shuffles.  0.50 ms at that size: the exponential pipe 60 %
+// busy, issue slots 58 %, shared memory 54 %, 7 blocks (14 warps) an SM.  Part of
+// the exponentials on the multiply-add pipes, more warps of fewer registers, and
+// the read-out or the reads moved ahead by hand each measured slower.
 //
 // Few rows and a long axis: the recurrence is linear, so a row is cut into
 // chunks.  A first pass runs each from a zero state (no read-out) and keeps its

@@ -6,9 +6,8 @@
 
 namespace gdn {
 
-constexpr int kScanThreads = 128;
-constexpr int kScanLanes = 4;                            // lanes of a channel
-constexpr int kScanCh = kScanThreads / kScanLanes;       // channels of a block
+constexpr int kScanLanes = 4;   // lanes of a channel
+constexpr int kScanCh = 32;     // channels of a block
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -49,12 +48,6 @@ __device__ __forceinline__ float softplus_sig(float v, float& sig) {
   const float r = fast_rcp(1.f + e);
   sig = v >= 0.f ? r : e * r;
   return softplus_e(v, e);
-}
-
-// One element, zero where `ok` is false.
-template <typename T>
-__device__ __forceinline__ float load1(const T* p, bool ok) {
-  return ok ? to_f32(*p) : 0.f;
 }
 
 // Four consecutive elements as they lie in memory (a load in flight holds two
@@ -126,31 +119,6 @@ __device__ __forceinline__ float quad_sum4(float v0, float v1, float v2, float v
   k1 += __shfl_xor_sync(0xffffffffu, g1, 2);
   const float k = odd ? k1 : k0, g = odd ? k0 : k1;
   return k + __shfl_xor_sync(0xffffffffu, g, 1);
-}
-
-// NL fp32 values to / from memory in 16-byte vectors where NL allows.
-template <int NL>
-__device__ __forceinline__ void store_states(float* p, const float (&v)[NL]) {
-  if constexpr (NL % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < NL; i += 4) store4(p + i, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) p[i] = v[i];
-  }
-}
-template <int NL>
-__device__ __forceinline__ void load_states(const float* p, float (&v)[NL]) {
-  if constexpr (NL % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < NL; i += 4) {
-      const float4 q = load4(p + i);
-      v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) v[i] = p[i];
-  }
 }
 
 // A lane's states as pairs (NL = 1: one state and an idle second).
