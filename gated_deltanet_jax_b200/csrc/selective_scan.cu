@@ -326,8 +326,63 @@ scan_step_kernel(const ScanArgs a) {
   }
 }
 
+// The same at 16 states where four channels in a row share a group: four lanes
+// take four channels together, each forming the step and the gate of one (four
+// lanes a channel form them four times over, and issue slots, 71 % of them in use,
+// then hold the loads back: 12.2 us for 64 x 4096 channels).
+template <typename T>
+__global__ void __launch_bounds__(256)
+scan_step4_kernel(const ScanArgs a) {
+  constexpr int N = 16;
+  const int lane = threadIdx.x & 31, q = lane & 3, b = blockIdx.y;
+  const long long cl = (long long)blockIdx.x * 256 + threadIdx.x;   // this lane's channel
+  const bool chan = cl < a.C;
+  const int c = chan ? (int)cl : a.C - 1;
+  const int cq = c - q >= 0 ? c - q : 0;     // the four lanes' first channel
+  const int grp = cq / (a.C / a.G);
+  const bool quad = cl - q < a.C;            // C is a multiple of four: all four or none
+  const size_t row = (size_t)b * a.C;
+  const size_t st = (row + cq) * N + 4 * q;
+  float4 h[4], A[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    h[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (quad && a.h0) h[j] = load4_stream(a.h0 + st + j * N);
+  }
+  const float x = to_f32(static_cast<const T*>(a.x)[row + c]);
+  float d = to_f32(static_cast<const T*>(a.dt)[row + c]) + (a.dt_bias ? a.dt_bias[c] : 0.f);
+  const float zv = a.z ? to_f32(static_cast<const T*>(a.z)[row + c]) : 0.f;
+  const float Dv = a.D ? a.D[c] : 0.f;
+  const size_t bc = ((size_t)b * a.G + grp) * N + 4 * q;
+  const float4 B = load4(static_cast<const T*>(a.Bm) + bc);
+  const float4 Cv = load4(static_cast<const T*>(a.Cm) + bc);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) A[j] = load4(a.A + (size_t)(quad ? cq + j : 0) * N + 4 * q);
+  if (a.softplus) d = softplus_fast(d);
+  const float u = d * x;
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float dj = __shfl_sync(0xffffffffu, d, (lane & ~3) | j) * kLog2e;
+    const float uj = __shfl_sync(0xffffffffu, u, (lane & ~3) | j);
+    h[j].x = fmaf(ex2(dj * A[j].x), h[j].x, uj * B.x);
+    h[j].y = fmaf(ex2(dj * A[j].y), h[j].y, uj * B.y);
+    h[j].z = fmaf(ex2(dj * A[j].z), h[j].z, uj * B.z);
+    h[j].w = fmaf(ex2(dj * A[j].w), h[j].w, uj * B.w);
+    if (quad && a.hT) store4_stream(a.hT + st + j * N, h[j]);
+    y[j] = fmaf(Cv.x, h[j].x, fmaf(Cv.y, h[j].y, fmaf(Cv.z, h[j].z, Cv.w * h[j].w)));
+  }
+  float o = fmaf(Dv, x, quad_sum4(y[0], y[1], y[2], y[3], lane));
+  if (a.z) o *= zv * fast_sigmoid(zv);
+  if (chan) static_cast<T*>(a.y)[row + c] = from_f32<T>(o);
+}
+
 template <typename T, int L>
 cudaError_t launch_step(const ScanArgs& a, cudaStream_t st) {
+  if (L == 4 && a.C / a.G % 4 == 0) {
+    scan_step4_kernel<T><<<dim3((unsigned)((a.C + 255LL) / 256), a.B), 256, 0, st>>>(a);
+    return cudaGetLastError();
+  }
   const long long blocks = ((long long)a.C * L + 255) / 256;
   scan_step_kernel<T, L><<<dim3((unsigned)blocks, a.B), 256, 0, st>>>(a);
   return cudaGetLastError();
