@@ -56,7 +56,8 @@ inline int device_sm_count() {
 //   GDN_CHUNK_KERNEL=fused   the one-launch tensor-core chunk kernel (no workspace)
 //   GDN_CHUNK_TC_PAIR=0 / 1  its unpaired / paired form
 //   GDN_RECURRENT_KERNEL=token  the token loop for whole sequences
-//   GDN_DECODE_PDL=0         decode steps without programmatic dependent launch
+//   GDN_DECODE_PDL=0         decode steps and the gated linear unit of few tokens without
+//                            programmatic dependent launch
 //   GDN_BWD_PREP=warp        the backward's warp-level per-chunk preparation
 //   GDN_BWD_FWDPASS=warp     the backward's forward pass on its warp-level state kernel
 //   GDN_BWD_REVPASS=warp     the backward's reverse pass on its warp-level state kernel
