@@ -868,6 +868,8 @@ int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void*
   const void* outs[3] = {dx, dw_gate, dw_up};
   for (const void* p : outs)
     if (p && !aligned16(p)) return fail(GDN_ERR_INVALID, "the gradients must be 16-byte aligned");
+  if ((dx && (dx == x || dx == dh)) || (dw_gate && (dw_gate == w_gate || dw_up == w_up)))
+    return fail(GDN_ERR_INVALID, "the gradients may not be the inputs: later products read them");
   if (M > 0 && I > 0) {
     const void* ptrs[3] = {g, u, dh};
     for (const void* p : ptrs)
@@ -934,7 +936,14 @@ int gdn_selective_scan_bwd(const void* x, const void* dt, const float* A, const 
                            int softplus, int dtype, void* workspace, size_t ws_bytes,
                            void* stream) {
   int rc = check_scan(x, dt, A, Bm, Cm, D, z, dt_bias, nullptr, B, T, C, N, G, softplus, dtype);
-  if (rc || C == 0) return rc;
+  if (rc) return rc;
+  if (C == 0) {
+    // no channel reads B or C
+    const size_t bytes = (size_t)B * T * G * N * (dtype == GDN_DTYPE_BF16 ? 2 : 4);
+    if (bytes && dB) rc = carry(dB, nullptr, bytes, stream, "gdn_selective_scan_bwd");
+    if (!rc && bytes && dC) rc = carry(dC, nullptr, bytes, stream, "gdn_selective_scan_bwd");
+    return rc;
+  }
   const void* ptrs[11] = {checkpoints, dy, dhT, dx, ddt, dA, dB, dC, dD, dz, ddt_bias};
   for (const void* p : ptrs)
     if (!aligned16(p)) return fail(GDN_ERR_INVALID, "the gradients must be 16-byte aligned");

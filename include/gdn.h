@@ -425,7 +425,8 @@ int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, vo
 
 /*
  * Its gradients from dh [M, I] and the forward's g and u: dx [M, D] (NULL: not
- * wanted), dw_gate and dw_up [I, D] (both or neither), in the inputs' dtype.
+ * wanted), dw_gate and dw_up [I, D] (both or neither), in the inputs' dtype;
+ * outputs overlap no input.
  * `workspace`: gdn_glu_bwd_workspace_bytes() bytes (the gradients of g and u in
  * the inputs' dtype; partial sums of the weights' where those need them).
  */
@@ -463,7 +464,7 @@ int gdn_selective_scan_fwd(const void* x, const void* dt, const float* A, const 
  * ddt_bias [C] and dh0 [B, C, N] (NULL: not wanted) in fp32.  dD, dz and
  * ddt_bias are given exactly when D, z and dt_bias are.  `checkpoints`: as the
  * forward wrote them.  `workspace`: gdn_selective_scan_bwd_workspace_bytes()
- * bytes.  All sums run in a fixed order.
+ * bytes.  Outputs overlap no input.  All sums run in a fixed order.
  */
 size_t gdn_selective_scan_bwd_workspace_bytes(int B, int T, int C, int N, int G);
 int gdn_selective_scan_bwd(const void* x, const void* dt, const float* A, const void* Bm,

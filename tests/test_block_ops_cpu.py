@@ -85,7 +85,7 @@ def test_glu_reference_gradients_match_differences():
 
 # ---- refusals of the C entry points (before any CUDA call) ----
 
-P = ctypes.c_void_p(16)
+P, Q = ctypes.c_void_p(16), ctypes.c_void_p(32)
 BAD = ctypes.c_void_p(24)
 BF16, FP32 = _lib.GDN_DTYPE_BF16, _lib.GDN_DTYPE_FP32
 INVALID, UNSUPPORTED, OK = _lib.GDN_ERR_INVALID, _lib.GDN_ERR_UNSUPPORTED, _lib.GDN_OK
@@ -102,13 +102,14 @@ def test_glu_rejects_bad_arguments(lib):
     assert fwd(M=(1 << 30) + 1) == UNSUPPORTED
     assert fwd(M=0) == OK and fwd(I=0) == OK
 
-    def bwd(ws=P, n=1 << 20, g=P, dh=P, dx=P, dwg=P, dwu=P, M=4, D=64, I=32, dtype=BF16):
+    def bwd(ws=P, n=1 << 20, g=P, dh=P, dx=Q, dwg=Q, dwu=Q, M=4, D=64, I=32, dtype=BF16):
         return lib.gdn_glu_bwd(P, P, P, g, P, dh, dx, dwg, dwu, M, D, I, dtype, ws, n, None)
     need = lib.gdn_glu_bwd_workspace_bytes(4, 64, 32, BF16)
     assert need >= 2 * 4 * 32 * 2
     assert bwd(n=need - 1) == INVALID and bwd(ws=None) == INVALID and bwd(ws=BAD) == INVALID
     assert bwd(g=None) == INVALID and bwd(dh=BAD) == INVALID and bwd(dwu=None) == INVALID
     assert bwd(dx=BAD) == INVALID and bwd(D=-1) == INVALID
+    assert bwd(dx=P) == INVALID                      # x itself
 
 
 def test_scan_rejects_bad_arguments(lib):

@@ -284,6 +284,13 @@ def test_scan_empty_layouts_and_types(cuda):
     y1, s1 = selective_scan(**dict(none, A=A), output_final_state=True)
     assert y1.shape == (0, 9, 32) and s1.shape == (0, 32, 16)
     assert float(torch.autograd.grad(y1.sum(), [A])[0].abs().max()) == 0.0
+    # no channels: nothing reads B and C
+    Bg, Cg = (s[k].clone().requires_grad_(True) for k in ("B", "C"))
+    y2, s2 = selective_scan(s["x"][..., :0], s["dt"][..., :0], s["A"][:0], Bg, Cg,
+                            output_final_state=True)
+    assert y2.shape == (2, 9, 0) and s2.shape == (2, 0, 16)
+    gB, gC = torch.autograd.grad(y2.sum() + s2.sum(), [Bg, Cg])
+    assert float(gB.abs().max()) == 0.0 and float(gC.abs().max()) == 0.0
     # parameters in bf16 give their gradients in bf16; a state alone has gradients too
     Ab = s["A"].bfloat16().requires_grad_(True)
     h0 = s["initial_state"].clone().requires_grad_(True)
