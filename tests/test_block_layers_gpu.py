@@ -276,3 +276,75 @@ def test_retained_graph_and_accumulation(cuda):
     loss.backward()
     for q, f in zip(m.parameters(), first):
         assert torch.equal(q.grad, f + f)
+
+
+# ---------------------------------------------------------------------------
+# Offsets past 32 bits: the last rows of tensors of more than 2^31 elements
+# against the same rows computed on their own (the same kernels in the same
+# order: bf16 results equal up to one rounding)
+# ---------------------------------------------------------------------------
+
+def _same(a, b):
+    assert a.shape == b.shape and torch.isfinite(a.float()).all()
+    assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=1e-3)
+
+
+@pytest.fixture
+def roomy(cuda):
+    free, _ = torch.cuda.mem_get_info()
+    if free < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    yield cuda
+    torch.cuda.empty_cache()
+
+
+def test_conv_past_32_bit_offsets(roomy):
+    T, C, tail = 270_000, 8192, 500                      # 2.2e9 elements
+    x = torch.randn(1, T, C, device=roomy, dtype=torch.bfloat16)
+    dy = torch.randn(1, T, C, device=roomy, dtype=torch.bfloat16)
+    w = torch.randn(4, C, device=roomy) * 0.5
+    xg = x.requires_grad_(True)
+    y, s = short_convolution(xg, w, output_final_state=True)
+    (dx,) = torch.autograd.grad(y, [xg], dy)
+    x = x.detach()
+    win = x[:, T - tail - 3:T - tail].contiguous()
+    xt = x[:, -tail:].contiguous().requires_grad_(True)
+    yt, st = short_convolution(xt, w, conv_state=win, output_final_state=True)
+    (dxt,) = torch.autograd.grad(yt, [xt], dy[:, -tail:].contiguous())
+    _same(y[:, -tail:], yt)
+    assert torch.equal(s, st)
+    _same(dx[:, -tail:], dxt)
+    # in place over the whole axis: one tile of all tokens
+    S = torch.zeros(1, 3, C, device=roomy, dtype=torch.bfloat16)
+    with torch.no_grad():
+        y2, _ = short_convolution(x, w, conv_state=S, final_state_out=S)
+    assert torch.equal(y2[:, -tail:], y[:, -tail:]) and torch.equal(S, s)
+
+
+def test_scan_past_32_bit_offsets(roomy):
+    T, C, head = 270_000, 8192, 250_000                  # the head ends below 2^31
+    mk = lambda *s: torch.randn(*s, device=roomy, dtype=torch.bfloat16)   # noqa: E731
+    s = dict(x=mk(1, T, C), dt=mk(1, T, C), B=mk(1, T, 4), C=mk(1, T, 4))
+    A = -torch.rand(C, 4, device=roomy) - 0.05
+    y, st = selective_scan(A=A, **s, output_final_state=True)
+    cut = {k: v[:, :head].contiguous() for k, v in s.items()}
+    _, mid = selective_scan(A=A, **cut, output_final_state=True)
+    cut = {k: v[:, head:].contiguous() for k, v in s.items()}
+    yt, stt = selective_scan(A=A, **cut, initial_state=mid, output_final_state=True)
+    _same(y[:, head:], yt)
+    assert torch.allclose(st, stt, rtol=1e-4, atol=1e-4)
+
+
+def test_glu_past_32_bit_offsets(roomy):
+    M, D, I, tail = 400_000, 64, 5632, 512               # h has 2.25e9 elements
+    x = torch.randn(M, D, device=roomy, dtype=torch.bfloat16).requires_grad_(True)
+    wg, wu = (torch.randn(I, D, device=roomy, dtype=torch.bfloat16) * 0.125 for _ in range(2))
+    h = gated_linear_unit(x, wg, wu)
+    dh = torch.randn(M, I, device=roomy, dtype=torch.bfloat16)
+    (dx,) = torch.autograd.grad(h, [x], dh)
+    xt = x.detach()[-tail:].clone().requires_grad_(True)
+    ht = gated_linear_unit(xt, wg, wu)
+    (dxt,) = torch.autograd.grad(ht, [xt], dh[-tail:].clone())
+    _same(h[-tail:], ht)
+    _same(dx[-tail:], dxt)
+    assert _lib.load().gdn_device_error(0) == 0
