@@ -408,23 +408,31 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
   }
 }
 
-// dB, dC [rows, G, N] from the blocks' partials [tiles][rows][2 NP].
+// dB, dC [rows, G, N] from the blocks' partials [tiles][rows][2 NP]: four states a
+// thread, 16-byte reads with eight in flight.
 template <typename T>
 __global__ void __launch_bounds__(256)
 sum_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC,
               long long rows, int G, int N, int NP, int tiles) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;   // row, group, 2 NP
-  const int n = (int)(i % (2 * NP));
-  const long long rg = i / (2 * NP);
-  if (rg >= rows * G || n % NP >= N) return;
+  const int per = NP / 2;                                          // vectors of a row and group
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;   // row, group, vector
+  const int n = (int)(i % per) * 4;
+  const long long rg = i / per;
+  if (rg >= rows * G) return;
   const int g = (int)(rg % G);
-  const long long row = rg / G;
-  float s = 0.f;
+  const long long row = rg / G, step = rows * 2 * NP;
+  const float* p = part + ((long long)g * tiles * rows + row) * (2 * NP) + n;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int t = 0; t < tiles; ++t)
-    s += part[(((long long)g * tiles + t) * rows + row) * (2 * NP) + n];
-  T* out = n < NP ? dB : dC;
-  out[rg * N + n % NP] = from_f32<T>(s);
+  for (int t = 0; t < tiles; ++t) {
+    const float4 v = load4(p + t * step);
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  T* out = (n < NP ? dB : dC) + rg * N;
+  const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n % NP + e < N) out[n % NP + e] = from_f32<T>(v[e]);
 }
 
 template <typename T, int NL>
@@ -475,7 +483,7 @@ cudaError_t bwd_dispatch(const ScanBwdArgs& args, cudaStream_t st) {
   else if (f.N <= 32) e = bwd_form<T, 8>(a, tpg, vec, lay.sp, pBC, pP, st);
   else e = bwd_form<T, 16>(a, tpg, vec, lay.sp, pBC, pP, st);
   if (e != cudaSuccess) return e;
-  const long long n = rows * f.G * 2 * NP;
+  const long long n = rows * f.G * (NP / 2);
   if (n > 0) {
     const long long blocks = (n + 255) / 256;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;

@@ -482,7 +482,8 @@ _NO_SWITCH = contextlib.nullcontext()
 def _on_device(index: int):
     """``torch.cuda.device`` where it is not the current one already (single-token
     calls are bound by their host work)."""
-    return _NO_SWITCH if torch.cuda.current_device() == index else torch.cuda.device(index)
+    # (the raw query: its caller holds a CUDA tensor, so CUDA is initialised)
+    return _NO_SWITCH if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def _stream(index: int) -> int:
@@ -492,10 +493,9 @@ def _stream(index: int) -> int:
 
 def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """Contiguous and 16-byte aligned, as the kernels read and write."""
-    if t is None:
-        return None
-    if not t.is_contiguous():
-        t = t.contiguous()
+    if t is None or (t.is_contiguous() and not t.data_ptr() & 15):
+        return t
+    t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -515,12 +515,13 @@ def _on(t, dev):
 
 def _check_input(name, t, dev, dtype):
     """A CUDA tensor on the same device and of the same dtype as the first input."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, not on {dev}")
-    if t.dtype != dtype:
+    if isinstance(t, torch.Tensor):
+        if t.dtype is dtype and t.device == dev:
+            return
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, not on {dev}")
         raise TypeError(f"{name} must be {dtype} like the other inputs; got {t.dtype}")
+    raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
 
 
 def _cuda_input(name, t):
