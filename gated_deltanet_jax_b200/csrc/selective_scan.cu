@@ -182,7 +182,7 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
           float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
           for (int i = 0; i < P; ++i) {
-            const float2 e = mul2(d2, A2[c][i]);
+            const float2 e = decay_arg(d2, A2[c][i]);
             h[c][i] = fma2(make_float2(ex2(e.x), ex2(e.y)), h[c][i], mul2(u2, B2[i]));
             if (!kLocal) acc = i ? fma2(C2[i], h[c][i], acc) : mul2(C2[i], h[c][i]);
           }
@@ -271,7 +271,7 @@ scan_chain_kernel(float* __restrict__ state, const float* __restrict__ sum,
 #pragma unroll
     for (int j = 0; j < kAt; ++j) {
       l[j] = loc[j];
-      d[j] = ex2(a2 * dec[j]);
+      d[j] = ex2(fmaf(a2, dec[j], kDecayBias));
     }
     fetch(s0 + kAt);
 #pragma unroll
@@ -308,10 +308,10 @@ scan_step_kernel(const ScanArgs a) {
   float d = to_f32(static_cast<const T*>(a.dt)[row]) + (a.dt_bias ? a.dt_bias[c] : 0.f);
   if (a.softplus) d = softplus_fast(d);
   const float u = d * x, d2 = d * kLog2e;
-  h.x = fmaf(ex2(d2 * A.x), h.x, u * B.x);
-  h.y = fmaf(ex2(d2 * A.y), h.y, u * B.y);
-  h.z = fmaf(ex2(d2 * A.z), h.z, u * B.z);
-  h.w = fmaf(ex2(d2 * A.w), h.w, u * B.w);
+  h.x = fmaf(ex2(fmaf(d2, A.x, kDecayBias)), h.x, u * B.x);
+  h.y = fmaf(ex2(fmaf(d2, A.y, kDecayBias)), h.y, u * B.y);
+  h.z = fmaf(ex2(fmaf(d2, A.z, kDecayBias)), h.z, u * B.z);
+  h.w = fmaf(ex2(fmaf(d2, A.w, kDecayBias)), h.w, u * B.w);
   if (a.hT && chan) store4_stream(a.hT + st, h);
   float y = fmaf(Cv.x, h.x, fmaf(Cv.y, h.y, fmaf(Cv.z, h.z, Cv.w * h.w)));
 #pragma unroll
@@ -365,10 +365,10 @@ scan_step4_kernel(const ScanArgs a) {
   for (int j = 0; j < 4; ++j) {
     const float dj = __shfl_sync(0xffffffffu, d, (lane & ~3) | j) * kLog2e;
     const float uj = __shfl_sync(0xffffffffu, u, (lane & ~3) | j);
-    h[j].x = fmaf(ex2(dj * A[j].x), h[j].x, uj * B.x);
-    h[j].y = fmaf(ex2(dj * A[j].y), h[j].y, uj * B.y);
-    h[j].z = fmaf(ex2(dj * A[j].z), h[j].z, uj * B.z);
-    h[j].w = fmaf(ex2(dj * A[j].w), h[j].w, uj * B.w);
+    h[j].x = fmaf(ex2(fmaf(dj, A[j].x, kDecayBias)), h[j].x, uj * B.x);
+    h[j].y = fmaf(ex2(fmaf(dj, A[j].y, kDecayBias)), h[j].y, uj * B.y);
+    h[j].z = fmaf(ex2(fmaf(dj, A[j].z, kDecayBias)), h[j].z, uj * B.z);
+    h[j].w = fmaf(ex2(fmaf(dj, A[j].w, kDecayBias)), h[j].w, uj * B.w);
     if (quad && a.hT) store4_stream(a.hT + st + j * N, h[j]);
     y[j] = fmaf(Cv.x, h[j].x, fmaf(Cv.y, h[j].y, fmaf(Cv.z, h[j].z, Cv.w * h[j].w)));
   }

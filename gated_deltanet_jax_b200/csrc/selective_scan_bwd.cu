@@ -191,7 +191,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
           const float dd = c ? du.z : du.x, gg = c ? g.y : g.x;
 #pragma unroll
           for (int i = 0; i < P; ++i) {
-            const float2 e = mul2(make_float2(dd, dd), A2[c][i]);
+            const float2 e = decay_arg(make_float2(dd, dd), A2[c][i]);
             ar[c][i] = mul2(make_float2(ex2(e.x), ex2(e.y)),
                             fma2(C2[i], make_float2(gg, gg), ar[c][i]));
           }
@@ -221,7 +221,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
           const float2 u2 = c ? make_float2(du.w, du.w) : make_float2(du.y, du.y);
 #pragma unroll
           for (int i = 0; i < P; ++i) {
-            const float2 e = mul2(d2, A2[c][i]);
+            const float2 e = decay_arg(d2, A2[c][i]);
             s[c][i] = fma2(make_float2(ex2(e.x), ex2(e.y)), s[c][i], mul2(u2, B2[i]));
           }
         }
@@ -277,7 +277,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
               sb = i ? fma2(r, B2[i], sb) : mul2(r, B2[i]);
               // (kept from the walk above, the factors spilled: 1.24 against 0.83 ms
               // for the training pass of 4 x 2048 x 2048)
-              const float2 e = mul2(d2, A2[c][i]);
+              const float2 e = decay_arg(d2, A2[c][i]);
               const float2 dk = make_float2(ex2_again(e.x), ex2_again(e.y));
               ar[c][i] = mul2(dk, r);
               const float2 fl = mul2(ar[c][i], hp);
