@@ -853,9 +853,7 @@ int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, vo
 
 size_t gdn_glu_bwd_workspace_bytes(int M, int D, int I, int dtype) {
   if (M <= 0 || D < 0 || I <= 0) return 0;
-  const int parts = gdn::glu_dw_parts(M, D, I, dtype);
-  return 2 * glu_half_bytes(M, I, dtype) +
-         (parts > 1 ? (size_t)parts * 2 * I * D * sizeof(float) : 0);
+  return 2 * glu_half_bytes(M, I, dtype) + gdn::glu_part_floats(M, D, I, dtype) * sizeof(float);
 }
 
 int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void* g, const void* u,

@@ -332,10 +332,9 @@ struct GluArgs {
   int M, D, I, dtype;
 };
 cudaError_t launch_glu_fwd(const GluArgs& a, cudaStream_t st);
-// Its gradients from g, u and dh [M,I]; dg, du [M,I] are scratch, and part is of
-// 2 I D floats for each of glu_dw_parts() where those are more than one.  dx [M,D]
-// or NULL; dwg, dwu [I,D] or both NULL.
-int glu_dw_parts(int M, int D, int I, int dtype);
+// Its gradients from g, u and dh [M,I]; dg, du [M,I] and part (glu_part_floats()
+// floats) are scratch.  dx [M,D] or NULL; dwg, dwu [I,D] or both NULL.
+size_t glu_part_floats(int M, int D, int I, int dtype);
 struct GluBwdArgs {
   const void* x;
   const void* wg;

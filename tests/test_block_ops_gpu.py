@@ -89,6 +89,36 @@ def test_glu_gradients(cuda, dtype, M, D, I):
     assert _lib.load().gdn_device_error(0) == 0
 
 
+# Few tokens on the CUDA cores (one to sixteen at once, widths off a vector and off a
+# warp's 128 elements, a last column on its own), each tile, and contractions in parts.
+CUDA_CORES = [(1, 129, 7), (1, 300, 1), (2, 7, 9), (3, 1000, 33), (4, 128, 10), (5, 254, 31),
+              (8, 131, 6), (9, 300, 5), (16, 6, 50), (17, 2050, 33), (40, 512, 90), (50, 90, 700),
+              (20, 41, 3001), (64, 130, 1100), (130, 250, 1030), (700, 260, 300), (5001, 30, 22),
+              (513, 1024, 130), (1100, 130, 2100)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("M,D,I", CUDA_CORES)
+def test_glu_cuda_core_forms(cuda, dtype, M, D, I):
+    test_glu_gradients(cuda, dtype, M, D, I)
+
+
+def test_glu_cuda_core_padding_is_not_read(cuda):
+    """Infinities in the rows and columns after a call's tensors do not reach it."""
+    for M, D, I in [(3, 132, 6), (9, 130, 5), (70, 36, 33), (300, 260, 70)]:
+        x, wg, wu, dy = _glu_inputs(M, D, I, "fp32", cuda, M)
+        leaves = []
+        for t in (x, wg, wu):
+            flat = torch.full((t.numel() + 4096,), float("inf"), device=cuda)
+            flat[:t.numel()] = t.reshape(-1)
+            leaves.append(flat[:t.numel()].view(t.shape).requires_grad_(True))
+        h = gated_linear_unit(*leaves)
+        ref = gated_linear_unit(x, wg, wu)
+        assert torch.equal(h, ref)
+        for t in torch.autograd.grad(h, leaves, dy):
+            assert bool(torch.isfinite(t).all())
+
+
 def test_glu_shapes_strides_and_partial_gradients(cuda):
     x, wg, wu, dy = _glu_inputs(24, 64, 96, "bf16", cuda, 5)
     h = gated_linear_unit(x, wg, wu)
