@@ -119,6 +119,34 @@ def test_glu_cuda_core_padding_is_not_read(cuda):
             assert bool(torch.isfinite(t).all())
 
 
+@pytest.mark.parametrize("std", [0.05, 1.0, 4.0, 30.0])
+def test_conv_bf16_silu_keeps_the_bits_of_the_exact_division(cuda, std):
+    """The bf16 convolution forms its SiLU with fast instructions where they cannot
+    change the rounded result: every output has the bits of the fp32 call (an exact
+    division) on the same values, rounded to bf16."""
+    g = _gen(int(std * 100))
+    for K, bias in ((4, True), (3, False), (1, True)):
+        x = _randn(g, 3, 700, 512, std=std).to(torch.bfloat16).to(cuda)
+        w = _randn(g, K, 512).to(torch.float32).to(cuda)
+        b = _randn(g, 512).to(torch.float32).to(cuda) if bias else None
+        y, _ = short_convolution(x, w, bias=b)
+        ref, _ = short_convolution(x.float(), w, bias=b)
+        assert torch.equal(y, ref.to(torch.bfloat16))
+
+
+def test_conv_bf16_silu_special_values(cuda):
+    """Zeros, the ends of the range, subnormals, infinities and NaN."""
+    v = torch.tensor([0.0, -0.0, 1e-38, -1e-38, 1e-40, -1e-40, 3e38, -3e38, -8.0, -7.97, -8.06,
+                      -88.0, -100.0, -200.0, 88.0, 200.0, float("inf"), -float("inf"),
+                      float("nan"), 1.0], device=cuda).to(torch.bfloat16)
+    for shift in range(4):                        # each value beside every other kind
+        x = v.roll(shift).repeat(2).view(1, 1, -1).contiguous()
+        w = torch.ones(1, x.shape[2], device=cuda)
+        y, _ = short_convolution(x, w)
+        ref, _ = short_convolution(x.float(), w)
+        assert torch.equal(y.view(torch.int16), ref.to(torch.bfloat16).view(torch.int16))
+
+
 def test_glu_shapes_strides_and_partial_gradients(cuda):
     x, wg, wu, dy = _glu_inputs(24, 64, 96, "bf16", cuda, 5)
     h = gated_linear_unit(x, wg, wu)
