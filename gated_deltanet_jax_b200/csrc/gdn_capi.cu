@@ -6,6 +6,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include <algorithm>
 #include <atomic>
 
 #include "gdn.h"
@@ -798,7 +799,9 @@ int gdn_short_conv_fwd_bias(const void* x, const float* weight, const float* bia
 
 size_t gdn_short_conv_bwd_workspace_bytes(int B, int T, int C, int K) {
   if (K < 1 || K > gdn::kShortConvMaxK) return 0;
-  return gdn::short_conv_bwd_workspace_bytes(B, T, C, K);
+  // (either dtype's)
+  return std::max(gdn::short_conv_bwd_workspace_bytes(B, T, C, K, GDN_DTYPE_BF16),
+                  gdn::short_conv_bwd_workspace_bytes(B, T, C, K, GDN_DTYPE_FP32));
 }
 
 int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
@@ -828,7 +831,8 @@ int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
     return fail(GDN_ERR_INVALID, "x, dy and dx must be non-NULL and 16-byte aligned");
   if (dx == x || dx == dy)
     return fail(GDN_ERR_INVALID, "dx may not be x or dy: a token's gradient reads its neighbours");
-  rc = check_workspace(workspace, ws_bytes, gdn::short_conv_bwd_workspace_bytes(B, T, C, K),
+  rc = check_workspace(workspace, ws_bytes,
+                       gdn::short_conv_bwd_workspace_bytes(B, T, C, K, dtype),
                        "gdn_short_conv_bwd_workspace_bytes");
   if (rc) return rc;
   gdn::ShortConvBwdArgs a{x, weight, bias, state_in, dy, dstate_out, dx, dweight, dbias,

@@ -304,7 +304,7 @@ struct ShortConvBwdArgs {
   float* part;
   int B, T, C, K, act, dtype;
 };
-size_t short_conv_bwd_workspace_bytes(int B, int T, int C, int K);
+size_t short_conv_bwd_workspace_bytes(int B, int T, int C, int K, int dtype);
 cudaError_t launch_short_conv_bwd(const ShortConvBwdArgs& a, cudaStream_t st);
 // Sums `parts` rows of `stride` floats, in a fixed order; the row's columns go to
 // consecutive segments of n[k] values (n adding up to stride; dst NULL: dropped).

@@ -10,13 +10,15 @@
 // In bytes HBM-bound: x and dy are read once and dx is written once (pre is formed
 // again from x; it is not kept between the passes).  A thread owns two channels
 // (the two halves of every multiply-add instruction) and walks a tile of tokens
-// with x and dpre in sliding register windows, four tokens' loads in flight under
-// four others' work; a tile reads K - 1 rows before it and K - 1 after it again,
-// and inside it nothing is checked.  8 x 2048 x 4096 in bf16: 107 us (3.8 TB/s), 57 % of
-// the issue slots; with four channels a thread 275 us (registers left too few
-// warps), with every row's edges checked 155 us.  The sums over tokens stay in
-// registers (fp32) and leave as one partial row per tile, which a second kernel
-// adds up in a fixed order: no atomics, the same bits on every run.
+// with x and dpre in sliding register windows; it copies its own words of the next
+// twelve tokens to shared memory ahead of their use (in registers four tokens ahead
+// fitted, and 83 registers: 110 us); a tile reads K - 1 rows before it and K - 1
+// after it again, and inside it nothing is checked.  8 x 2048 x 4096 in bf16: 101 us
+// with the sums below (4.0 TB/s), about 60 % of the issue slots; with four channels a
+// thread 275 us (registers left too few warps), with every row's edges checked 155 us.
+// The sums over tokens stay in registers (fp32) and leave as one partial row per tile,
+// which a second kernel adds up in a fixed order: no atomics, the same bits on every
+// run.
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 
@@ -26,7 +28,13 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kVec = 2;        // channels of a thread: a warp reads 128 bytes of bf16 a row
-constexpr int kAhead = 4;      // tokens whose loads are in flight while four others are worked on
+constexpr int kAhead = 4;      // tokens of a group
+constexpr int kGroups = 4;     // groups in flight or worked on, in shared memory
+
+// Blocks of an SM: by registers in bf16 (72 of them at K = 4), by shared memory in fp32.
+constexpr int bwd_blocks(int K, int bytes) {
+  return K > 6 ? 3 : K > 4 ? 4 : bytes == 2 ? 7 : 6;
+}
 
 // Two channels as they lie in memory.
 template <typename T>
@@ -49,6 +57,19 @@ __device__ __forceinline__ Raw2<T> ldr(const T* p) {
   r.u = *reinterpret_cast<const decltype(r.u)*>(p);
   return r;
 }
+// A thread's own copy of them to shared memory; nothing is read and zeros are written
+// without `on` (p is then any valid address).
+template <typename T>
+__device__ __forceinline__ void copy2(Raw2<T>* dst, const T* p, bool on) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  const int n = on ? (int)sizeof(Raw2<T>) : 0;
+  if constexpr (sizeof(Raw2<T>) == 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(p), "r"(n)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d), "l"(p), "r"(n)
+                 : "memory");
+}
 __device__ __forceinline__ void st2(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
 __device__ __forceinline__ void st2(__nv_bfloat16* p, float2 v) {
   *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v.x, v.y);
@@ -57,7 +78,7 @@ __device__ __forceinline__ void st2(__nv_bfloat16* p, float2 v) {
 // Block (channel group, token tile, row b).  part [B * tiles][K + 1][C]: this
 // tile's sums for dw[0 .. K - 1] and dbias.
 template <typename Tin, int K>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, bwd_blocks(K, sizeof(Tin)))
 short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
                       const float* __restrict__ bias, const Tin* __restrict__ state_in,
                       const Tin* __restrict__ dy, const Tin* __restrict__ dstate_out,
@@ -95,17 +116,17 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
   const Tin* xt = x + (row0 + t0) * C + c;   // the next rows to load
   const Tin* gt = dy + (row0 + t0) * C + c;
   Tin* ot = dx + (row0 + t0) * C + c;        // the row of token tb
-  Raw2<Tin> xr[kAhead], gr[kAhead];
-  auto fetch = [&](int tb) {
+  __shared__ Raw2<Tin> ring[kGroups][kAhead][2][kThreads];
+  Raw2<Tin>* mine = &ring[0][0][0][threadIdx.x];
+  auto fetch = [&](int tb, int slot) {
+    Raw2<Tin>* r = mine + slot * (kAhead * 2 * kThreads);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      xr[i].u = {};
-      gr[i].u = {};
-      if (tb + i < tload) {
-        xr[i] = ldr(xt + (size_t)i * C);
-        gr[i] = ldr(gt + (size_t)i * C);
-      }
+      const bool on = tb + i < tload;
+      copy2(r + 2 * i * kThreads, on ? xt + (size_t)i * C : x, on);
+      copy2(r + (2 * i + 1) * kThreads, on ? gt + (size_t)i * C : x, on);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
     xt += step;
     gt += step;
   };
@@ -140,15 +161,21 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
     }
     return out;
   };
-  fetch(t0);
+#pragma unroll
+  for (int g = 0; g < kGroups - 1; ++g) fetch(t0 + g * kAhead, g);
+  int slot = 0;
   for (int tb = t0; tb < tend; tb += kAhead, ot += step) {
+    // (a thread reads what it copied itself: no barrier)
+    asm volatile("cp.async.wait_group %0;" ::"n"(kGroups - 2) : "memory");
     float2 xv[kAhead], gv[kAhead];   // (gradients past the last token are zero)
+    const Raw2<Tin>* r = mine + slot * (kAhead * 2 * kThreads);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      xv[i] = xr[i].get();
-      gv[i] = gr[i].get();
+      xv[i] = r[2 * i * kThreads].get();
+      gv[i] = r[(2 * i + 1) * kThreads].get();
     }
-    if (tb + kAhead < tend) fetch(tb + kAhead);
+    fetch(tb + (kGroups - 1) * kAhead, slot == 0 ? kGroups - 1 : slot - 1);
+    slot = slot + 1 == kGroups ? 0 : slot + 1;
     if (tb >= t0 + K - 1 && tb + kAhead <= t1) {
       // inside the tile: every token its own, every row closed one of dx
 #pragma unroll
@@ -173,6 +200,7 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
         st2(dstate_in + ((size_t)b * (K - 1) + (K - 1) + s) * C + c, out);
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");   // (zeros past the last token)
   float* pr = part + ((size_t)b * gridDim.y + blockIdx.y) * (K + 1) * C + c;
 #pragma unroll
   for (int j = 0; j < K; ++j) st2(pr + (size_t)j * C, dw[j]);
@@ -204,30 +232,34 @@ cudaError_t bwd_dispatch(const ShortConvBwdArgs& a, int TT, int tiles, cudaStrea
   return cudaGetLastError();
 }
 
-// Token tiles: enough warps to keep loads in flight on every SM (36 a SM),
-// tiles of 16 to 512 tokens (a tile reads 2 (K - 1) rows more than it owns).
-int conv_bwd_tile(int B, int T, int C) {
-  const long long warps_per_row = (C + kVec * 32 - 1) / (kVec * 32);
-  const long long want = 36LL * 148;
-  long long tt = (long long)B * T * warps_per_row / want;
-  tt = (tt + 15) / 16 * 16;
+// Token tiles such that the blocks fill the SMs a whole number of times, of at most 256
+// tokens where eight times allow it (a tile reads 2 (K - 1) rows more than it owns).
+// 8 x 2048 x 4096: 256 tokens, one wave, 101 us; 208 tokens 105, 352 tokens 118.
+int conv_bwd_tile(int B, int T, int C, int K, int dtype) {
+  const long long per = (long long)((C / kVec + kThreads - 1) / kThreads) * B;
+  const long long slots = 148LL * bwd_blocks(K, dtype == kBF16 ? 2 : 4);
+  long long tt = T;
+  for (int n = 1; per > 0 && n <= 8; ++n) {
+    const long long tiles = n * slots / per;
+    if (tiles > 0) tt = (T + tiles - 1) / tiles;
+    if (tiles > 0 && tt <= 256) break;
+  }
   if (tt < 16) tt = 16;
-  if (tt > 512) tt = 512;
   if ((T + tt - 1) / tt > 65535) tt = ((long long)T + 65534) / 65535;
   return (int)tt;
 }
 
 }  // namespace
 
-size_t short_conv_bwd_workspace_bytes(int B, int T, int C, int K) {
+size_t short_conv_bwd_workspace_bytes(int B, int T, int C, int K, int dtype) {
   if (B <= 0 || T <= 0 || C <= 0) return 0;
-  const int TT = conv_bwd_tile(B, T, C);
+  const int TT = conv_bwd_tile(B, T, C, K, dtype);
   return (size_t)B * ((T + TT - 1) / TT) * (K + 1) * C * sizeof(float);
 }
 
 cudaError_t launch_short_conv_bwd(const ShortConvBwdArgs& a, cudaStream_t st) {
   if (!short_conv_supported(a.C, a.K, a.dtype) || a.B > 65535) return cudaErrorInvalidValue;
-  const int TT = conv_bwd_tile(a.B, a.T, a.C);
+  const int TT = conv_bwd_tile(a.B, a.T, a.C, a.K, a.dtype);
   const int tiles = (a.T + TT - 1) / TT;
   cudaError_t e = a.dtype == kBF16 ? bwd_dispatch<__nv_bfloat16>(a, TT, tiles, st)
                                    : bwd_dispatch<float>(a, TT, tiles, st);

@@ -434,6 +434,13 @@ def test_conv_gradients(cuda, dtype, B, T, C, K, full):
             _within(t, ref[k], tol, k)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,C,K", [(64, 70, 4160, 4), (40, 150, 2048, 3), (60, 41, 4104, 8)])
+def test_conv_gradients_of_long_tiles(cuda, dtype, B, T, C, K):
+    """Rows that are one or two tiles each, walked past the copies in flight."""
+    test_conv_gradients(cuda, dtype, B, T, C, K, True)
+
+
 def test_conv_layouts_empty_and_refusals(cuda):
     g = _gen(4)
     x, w = _randn(g, 2, 20, 64).bfloat16().to(cuda), _randn(g, 4, 64).to(cuda)
