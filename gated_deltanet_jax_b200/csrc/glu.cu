@@ -13,7 +13,7 @@
 // tile of x: half of a tile's columns come from Wg and half from Wu, so that a
 // thread ends with g and u of the same elements.  Few tokens have a kernel of
 // their own, bound by the weights' bytes up to four of them (2048 x 5632 in fp32: one
-// token 147 us on the tiles, 10.5 here, partly from L2).
+// token 16 us from HBM, 10.5 with part of them in L2, where the tiles took 147).
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 
@@ -381,7 +381,7 @@ __device__ __forceinline__ void lane_sums(float2* v, int lane) {
 }
 
 // Few tokens on the CUDA cores: a warp owns two columns of the result, that is four
-// weight rows, and walks them 128 elements a step with the next step's loads in
+// weight rows, and walks them 128 elements a step with the next steps' loads in
 // flight; every 16 bytes of x (in L1, the SM's warps walk it together) serve the four
 // rows.  Even and odd elements are summed apart (two multiply-adds an instruction),
 // then the 32 lanes' sums are added up by halves in a fixed order, which leaves g and
@@ -413,21 +413,30 @@ glu_rows_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* __re
     }
   };
   const int full = K / 128 * 128;
-  float4 wn[4];
+  // Steps whose weights are in flight (from HBM, 2048 x 5632 and 4096 x 4096: one token 16.3
+  // and 24.5 us, with one step ahead 18.2 and 27.9; four tokens 20.5 and 27.3, 24.8 and 51.4).
+  constexpr int kAhead = MB <= 2 ? 2 : MB == 4 ? 4 : 1;
+  float4 wn[kAhead][4];
   if (full > 0) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) wn[r] = load_four<T, kVec, true>(w[r], 4);
+    for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        wn[s][r] = load_four<T, kVec, true>(w[r] + min(s * 128, full - 128), 4);
   }
+#pragma unroll kAhead
   for (int k = 0; k < full; k += 128) {
     float4 wv[4], xv[MB];
 #pragma unroll
     for (int m = 0; m < MB; ++m)
       xv[m] = load_four<T, kVec, true>(xr + (long long)min(m, mlast) * K + k, 4);
-    const int next = k + 128 < full ? k + 128 : k;
+    const int next = min(k + kAhead * 128, full - 128);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      wv[r] = wn[r];
-      wn[r] = load_four<T, kVec, true>(w[r] + next, 4);
+      wv[r] = wn[0][r];
+#pragma unroll
+      for (int s = 0; s + 1 < kAhead; ++s) wn[s][r] = wn[s + 1][r];
+      wn[kAhead - 1][r] = load_four<T, kVec, true>(w[r] + next, 4);
     }
 #pragma unroll
     for (int m = 0; m < MB; ++m) add(m, xv[m], wv);
