@@ -356,6 +356,7 @@ cudaError_t launch_glu_bwd(const GluBwdArgs& a, cudaStream_t st);
 bool glu_tc_supported(int M, int D, int I, int dtype);
 cudaError_t launch_glu_tc_fwd(const GluArgs& a, cudaStream_t st);
 cudaError_t launch_glu_tc_bwd(const GluBwdArgs& a, cudaStream_t st);
+size_t glu_tc_part_floats(int M, int D, int I);
 int device_error_glu_tc(bool clear);
 
 // Selective state-space scan (selective_scan.cu): x, dt, z, y [B,T,C], B, C

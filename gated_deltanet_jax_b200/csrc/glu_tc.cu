@@ -65,6 +65,9 @@ struct GluShape {
   int kblocks;            // 64-wide steps along the contraction (kDx: of each half)
   int keep;               // kFwd: g and u are stored
   int rows, cols;         // of the output
+  // kDx: the contraction's parts and their steps.  With more than one, part p's sums
+  // leave in fp32 for rows 256 tiles_m p .. of out[1], of parts 256 tiles_m rows.
+  int parts = 1, part_steps = 0;
 };
 
 template <int KIND>
@@ -103,9 +106,20 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
   const int npairs = gridDim.x / 2, pair = blockIdx.x / 2;
   const int tm = KIND == kDw ? 2 * sh.tiles_m : sh.tiles_m;
   const long long tiles = (long long)tm * sh.tiles_n;
+  const long long items = KIND == kDx ? tiles * sh.parts : tiles;
   const int ksteps = KIND == kDx ? 2 * sh.kblocks : sh.kblocks;
   // Panels of kPanel row tiles; within a panel, row tiles run fastest.
-  auto decode = [&](long long t, int& m, int& n) {
+  // k0 .. k1: the item's steps.
+  auto decode = [&](long long t, int& m, int& n, int& part, int& k0, int& k1) {
+    part = 0;
+    k0 = 0;
+    k1 = ksteps;
+    if (KIND == kDx) {
+      part = (int)(t / tiles);
+      t -= part * tiles;
+      k0 = part * sh.part_steps;
+      k1 = min(ksteps, k0 + sh.part_steps);
+    }
     const long long per = (long long)kPanel * sh.tiles_n;
     const int p = (int)(t / per);
     const int rows = min(kPanel, tm - p * kPanel);
@@ -118,13 +132,13 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
     if (lane == 0) {
       bool ok = true;
       uint32_t it = 0;
-      for (long long t = pair; ok && t < tiles; t += npairs) {
-        int m, n;
-        decode(t, m, n);
+      for (long long t = pair; ok && t < items; t += npairs) {
+        int m, n, part, k0, k1;
+        decode(t, m, n, part, k0, k1);
         const int half = KIND == kDw && m >= sh.tiles_m;
         if (half) m -= sh.tiles_m;
         const int row = m * kTile + (int)rank * 128;
-        for (int k = 0; k < ksteps; ++k, ++it) {
+        for (int k = k0; k < k1; ++k, ++it) {
           const int s = it % kStages;
           ok = mbar_wait(&empty[s], ((it / kStages) & 1) ^ 1);
           if (!ok) break;
@@ -167,11 +181,13 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
       const uint32_t sbase = smem_u32(sm);
       bool ok = true;
       uint32_t it = 0, j = 0;
-      for (long long t = pair; ok && t < tiles; t += npairs, ++j) {
+      for (long long t = pair; ok && t < items; t += npairs, ++j) {
         const uint32_t acc = tmem + (j & 1) * 256;
+        int m, n, part, k0, k1;
+        decode(t, m, n, part, k0, k1);
         ok = mbar_wait_cluster(&tempty[j & 1], ((j >> 1) & 1) ^ 1);
         tc_fence_after();
-        for (int k = 0; ok && k < ksteps; ++k, ++it) {
+        for (int k = k0; ok && k < k1; ++k, ++it) {
           const int s = it % kStages;
           ok = mbar_wait_cluster(&full[s], (it / kStages) & 1);
           if (!ok) break;
@@ -183,7 +199,7 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
                                             : umma_desc(a + q * 32, 16, 1024, kSW128);
             const uint64_t bd = KIND == kFwd ? umma_desc(b + q * 32, 16, 1024, kSW128)
                                              : umma_desc(b + q * 2048, 8192, 1024, kSW128);
-            mma_bf16_pair(acc, ad, bd, idesc, (k | q) != 0);
+            mma_bf16_pair(acc, ad, bd, idesc, k > k0 || q != 0);
           }
           mma_commit_pair(&empty[s]);
         }
@@ -227,9 +243,9 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
     };
     uint32_t j = 0;
     bool ok = true;
-    for (long long t = pair; ok && t < tiles; t += npairs, ++j) {
-      int m, n;
-      decode(t, m, n);
+    for (long long t = pair; ok && t < items; t += npairs, ++j) {
+      int m, n, part, k0, k1;
+      decode(t, m, n, part, k0, k1);
       const int second = KIND == kDw && m >= sh.tiles_m;
       if (second) m -= sh.tiles_m;
       const int r0 = m * kTile + (int)rank * 128;
@@ -271,6 +287,20 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
             if (w == 1) release();
             end_box(&maps.out[1 + w], c0, r0, box);
           }
+        }
+      } else if (KIND == kDx && sh.parts > 1) {
+#pragma unroll 1
+        for (int w = 0; w < 4; ++w) {
+          unsigned char* box = begin_box();
+          float v[32];
+          tmem_ld32(acc + half * 128 + w * 32, v);
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float4*>(box + sw128(row, c)) =
+                make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+          if (w == 3) release();
+          end_box(&maps.out[1], n * kTile + half * 128 + w * 32, part * sh.tiles_m * kTile + r0,
+                  box);
         }
       } else {
 #pragma unroll 1
@@ -460,17 +490,19 @@ glu_few_kernel(const __grid_constant__ FewMaps maps, const FewShape sh,
   }
 }
 
-// [rows, cols] bf16 row-major, boxes of 64 columns x `box_rows`, 128-byte swizzle.
-bool make_map(CUtensorMap* m, const void* base, long long rows, long long cols, int box_rows) {
+// [rows, cols] bf16 row-major, boxes of 64 columns x `box_rows` (fp32: of 32 columns),
+// 128-byte swizzle.
+bool make_map(CUtensorMap* m, const void* base, long long rows, long long cols, int box_rows,
+              bool fp32 = false) {
   auto fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint64_t strides[1] = {(cuuint64_t)cols * (fp32 ? 4 : 2)};
+  cuuint32_t box[2] = {fp32 ? 32u : 64u, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
-            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return fn(m, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -481,11 +513,42 @@ cudaError_t launch_kind(const GluMaps& maps, const GluShape& sh, cudaStream_t st
   static std::atomic<int> slot[kMaxDevices] = {};
   const cudaError_t e = ensure_smem(glu_tc_kernel<KIND>, kSmemBytes, slot);
   if (e != cudaSuccess) return e;
-  const long long tiles = (long long)sh.tiles_m * sh.tiles_n * (KIND == kDw ? 2 : 1);
+  const long long tiles = (long long)sh.tiles_m * sh.tiles_n * (KIND == kDw ? 2 : sh.parts);
   const int pairs = device_sm_count() / 2;
   const int grid = 2 * (int)(tiles < pairs ? tiles : pairs);
   glu_tc_kernel<KIND><<<grid, kTcThreads, kSmemBytes, st>>>(maps, sh);
   return cudaGetLastError();
+}
+
+// dx's parts added up in their order: n vectors of four, `stride` of them a part.
+__global__ void __launch_bounds__(256)
+glu_dx_sum_kernel(const float* __restrict__ part, int parts, long long n, long long stride,
+                  __nv_bfloat16* __restrict__ dx) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float4 s = load4(part + 4 * i);
+#pragma unroll 4
+  for (int p = 1; p < parts; ++p) {
+    const float4 v = load4(part + 4 * (p * stride + i));
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  store4(dx + 4 * i, s);
+}
+
+// Parts of dx's contraction, where its output tiles are at most half the pairs of SMs (a
+// tile walks 2 I / 64 steps alone): each of 8 steps or more, at most 16.  The whole
+// backward of 2048 x 5632: 16 tokens 74 -> 40 us, 256 81 -> 46, 1000 105 -> 88.
+int tc_dx_parts(int M, int D, int I, int* steps) {
+  const int ksteps = 2 * ceil_div(I, kBK), pairs = 74;
+  const long long tiles = (long long)ceil_div(M, kTile) * ceil_div(D, kTile);
+  *steps = ksteps;
+  if (tiles <= 0 || 2 * tiles > pairs) return 1;
+  int parts = (int)(pairs / tiles);
+  if (parts > 16) parts = 16;
+  if (parts > ksteps / 8) parts = ksteps / 8;
+  if (parts <= 1) return 1;
+  *steps = ceil_div(ksteps, parts);
+  return ceil_div(ksteps, *steps);
 }
 
 cudaError_t launch_few(const GluArgs& a, cudaStream_t st) {
@@ -563,6 +626,12 @@ cudaError_t launch_glu_tc_fwd(const GluArgs& a, cudaStream_t st) {
   return launch_kind<kFwd>(m, sh, st);
 }
 
+size_t glu_tc_part_floats(int M, int D, int I) {
+  int steps;
+  const int parts = tc_dx_parts(M, D, I, &steps);
+  return parts > 1 ? (size_t)parts * ceil_div(M, kTile) * kTile * D : 0;
+}
+
 cudaError_t launch_glu_tc_bwd(const GluBwdArgs& a, cudaStream_t st) {
   GluMaps m;
   if (a.dx) {
@@ -571,9 +640,20 @@ cudaError_t launch_glu_tc_bwd(const GluBwdArgs& a, cudaStream_t st) {
         !make_map(&m.out[0], a.dx, a.M, a.D, 128))
       return cudaErrorInvalidValue;
     m.out[1] = m.out[2] = m.out[0];
-    const GluShape sh{ceil_div(a.M, kTile), ceil_div(a.D, kTile), ceil_div(a.I, kBK), 0,
-                      a.M, a.D};
-    const cudaError_t e = launch_kind<kDx>(m, sh, st);
+    GluShape sh{ceil_div(a.M, kTile), ceil_div(a.D, kTile), ceil_div(a.I, kBK), 0, a.M, a.D};
+    sh.parts = tc_dx_parts(a.M, a.D, a.I, &sh.part_steps);
+    const int padded = sh.tiles_m * kTile;   // rows of a part
+    if (sh.parts > 1) {
+      sh.rows = sh.parts * padded;
+      if (!make_map(&m.out[1], a.part, sh.rows, a.D, 128, true)) return cudaErrorInvalidValue;
+    }
+    cudaError_t e = launch_kind<kDx>(m, sh, st);
+    if (e == cudaSuccess && sh.parts > 1) {
+      const long long n = (long long)a.M * a.D / 4;
+      glu_dx_sum_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(
+          a.part, sh.parts, n, (long long)padded * a.D / 4, static_cast<__nv_bfloat16*>(a.dx));
+      e = cudaGetLastError();
+    }
     if (e != cudaSuccess) return e;
   }
   if (a.dwg) {
