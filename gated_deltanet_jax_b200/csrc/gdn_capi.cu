@@ -179,8 +179,7 @@ int check_glu(const void* x, const void* wg, const void* wu, int M, int D, int I
   if (M < 0 || D < 0 || I < 0) return fail(GDN_ERR_INVALID, "negative size M=%d D=%d I=%d", M, D, I);
   if (int rc = check_dtype(dtype)) return rc;
   // (the CUDA-core form's grid: 65535 row tiles of 64; the tensor-core form's row indexes)
-  const bool tc = dtype == GDN_DTYPE_BF16 && D % 8 == 0 && I % 8 == 0;
-  const int most = tc ? 1 << 30 : 65535 * 64;
+  const int most = gdn::glu_tc_widths(D, I, dtype) ? 1 << 30 : 65535 * 64;
   if (M > most || I > most || D > most)
     return fail(GDN_ERR_UNSUPPORTED, "M=%d, D=%d or I=%d exceeds %d", M, D, I, most);
   if ((long long)M * (D > I ? D : I) > (1LL << 40) || (long long)I * D > (1LL << 40))

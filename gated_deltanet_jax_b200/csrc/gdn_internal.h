@@ -352,7 +352,8 @@ struct GluBwdArgs {
 };
 cudaError_t launch_glu_bwd(const GluBwdArgs& a, cudaStream_t st);
 // Their products on tcgen05 (glu_tc.cu): bf16, D and I multiples of 8 (a row's
-// bytes a multiple of 16, as TMA needs).  The backward's reads dg and du.
+// bytes a multiple of 16, as TMA needs), D up to 131072.  The backward's reads dg and du.
+bool glu_tc_widths(int D, int I, int dtype);
 bool glu_tc_supported(int M, int D, int I, int dtype);
 cudaError_t launch_glu_tc_fwd(const GluArgs& a, cudaStream_t st);
 cudaError_t launch_glu_tc_bwd(const GluBwdArgs& a, cudaStream_t st);

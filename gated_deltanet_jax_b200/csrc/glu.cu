@@ -547,9 +547,10 @@ cudaError_t bwd_products_simt(const GluBwdArgs& a, cudaStream_t st) {
 }  // namespace
 
 // A product with few output tiles leaves SMs idle; its contraction is cut into parts (in
-// fp32, and dx on the tensor cores), whose sums a second kernel adds up in a fixed order.
+// fp32, and dx on the tensor cores, whose accumulators also take no more than 32768 terms
+// each), whose sums a second kernel adds up in a fixed order.
 size_t glu_part_floats(int M, int D, int I, int dtype) {
-  if (dtype == kBF16 && D % 8 == 0 && I % 8 == 0) return glu_tc_part_floats(M, D, I);
+  if (glu_tc_widths(D, I, dtype)) return glu_tc_part_floats(M, D, I);
   if (dtype != kFP32) return 0;
   const size_t dx = simt_plan(kDx, M, D, I, true).parts, dw = simt_plan(kDw, I, D, M, true).parts;
   const size_t a = dx > 1 ? dx * M * D : 0, b = dw > 1 ? dw * 2 * I * D : 0;

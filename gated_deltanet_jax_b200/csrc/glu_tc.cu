@@ -29,6 +29,8 @@
 // value: together they take a gradient's error in the norm from 1.7e-3 (its own
 // rounding) to 3.1e-3.  Keeping g and u in fp32 would double what a training step
 // keeps of them.
+#include <algorithm>
+
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
 #include "ptx.cuh"
@@ -65,10 +67,17 @@ struct GluShape {
   int kblocks;            // 64-wide steps along the contraction (kDx: of each half)
   int keep;               // kFwd: g and u are stored
   int rows, cols;         // of the output
-  // kDx: the contraction's parts and their steps.  With more than one, part p's sums
-  // leave in fp32 for rows 256 tiles_m p .. of out[1], of parts 256 tiles_m rows.
+  // kDx, kDw: the contraction's parts and their steps.  With more than one, part p's sums
+  // leave in fp32 for rows 256 tiles_m p .. (kDw: 512 tiles_m p, dWg's before dWu's) of out[2].
   int parts = 1, part_steps = 0;
 };
+
+// The most 64-wide steps that one accumulator takes.  A sum in TMEM does not round to
+// nearest: over terms of one sign it came out too small by 0.7e-4 after 16384 of them, 3.5e-4
+// after 65536, 1.6e-3 after 262144 and 2.6 % after 4 million.  Longer contractions are cut into
+// parts of 32768 terms, added up in fp32: at 2048 x 5632 the weights' gradients of 65536 tokens
+// then write and read 0.37 GB more beside 2 ms of products.
+constexpr int kMaxSteps = 512;
 
 template <int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
@@ -106,7 +115,7 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
   const int npairs = gridDim.x / 2, pair = blockIdx.x / 2;
   const int tm = KIND == kDw ? 2 * sh.tiles_m : sh.tiles_m;
   const long long tiles = (long long)tm * sh.tiles_n;
-  const long long items = KIND == kDx ? tiles * sh.parts : tiles;
+  const long long items = KIND == kFwd ? tiles : tiles * sh.parts;
   const int ksteps = KIND == kDx ? 2 * sh.kblocks : sh.kblocks;
   // Panels of kPanel row tiles; within a panel, row tiles run fastest.
   // k0 .. k1: the item's steps.
@@ -114,7 +123,7 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
     part = 0;
     k0 = 0;
     k1 = ksteps;
-    if (KIND == kDx) {
+    if (KIND != kFwd) {
       part = (int)(t / tiles);
       t -= part * tiles;
       k0 = part * sh.part_steps;
@@ -288,7 +297,7 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
             end_box(&maps.out[1 + w], c0, r0, box);
           }
         }
-      } else if (KIND == kDx && sh.parts > 1) {
+      } else if (sh.parts > 1) {
 #pragma unroll 1
         for (int w = 0; w < 4; ++w) {
           unsigned char* box = begin_box();
@@ -299,8 +308,8 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
             *reinterpret_cast<float4*>(box + sw128(row, c)) =
                 make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
           if (w == 3) release();
-          end_box(&maps.out[1], n * kTile + half * 128 + w * 32, part * sh.tiles_m * kTile + r0,
-                  box);
+          end_box(&maps.out[2], n * kTile + half * 128 + w * 32,
+                  (KIND == kDw ? 2 * part + second : part) * sh.tiles_m * kTile + r0, box);
         }
       } else {
 #pragma unroll 1
@@ -513,17 +522,17 @@ cudaError_t launch_kind(const GluMaps& maps, const GluShape& sh, cudaStream_t st
   static std::atomic<int> slot[kMaxDevices] = {};
   const cudaError_t e = ensure_smem(glu_tc_kernel<KIND>, kSmemBytes, slot);
   if (e != cudaSuccess) return e;
-  const long long tiles = (long long)sh.tiles_m * sh.tiles_n * (KIND == kDw ? 2 : sh.parts);
+  const long long tiles = (long long)sh.tiles_m * sh.tiles_n * sh.parts * (KIND == kDw ? 2 : 1);
   const int pairs = device_sm_count() / 2;
   const int grid = 2 * (int)(tiles < pairs ? tiles : pairs);
   glu_tc_kernel<KIND><<<grid, kTcThreads, kSmemBytes, st>>>(maps, sh);
   return cudaGetLastError();
 }
 
-// dx's parts added up in their order: n vectors of four, `stride` of them a part.
+// The parts added up in their order: n vectors of four, `stride` of them a part.
 __global__ void __launch_bounds__(256)
-glu_dx_sum_kernel(const float* __restrict__ part, int parts, long long n, long long stride,
-                  __nv_bfloat16* __restrict__ dx) {
+glu_part_sum_kernel(const float* __restrict__ part, int parts, long long n, long long stride,
+                    __nv_bfloat16* __restrict__ out) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   float4 s = load4(part + 4 * i);
@@ -532,23 +541,34 @@ glu_dx_sum_kernel(const float* __restrict__ part, int parts, long long n, long l
     const float4 v = load4(part + 4 * (p * stride + i));
     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
-  store4(dx + 4 * i, s);
+  store4(out + 4 * i, s);
 }
 
-// Parts of dx's contraction, where its output tiles are at most half the pairs of SMs (a
-// tile walks 2 I / 64 steps alone): each of 8 steps or more, at most 16.  The whole
-// backward of 2048 x 5632: 16 tokens 74 -> 40 us, 256 81 -> 46, 1000 105 -> 88.
+cudaError_t sum_parts(const float* part, int parts, long long n, long long stride, void* out,
+                      cudaStream_t st) {
+  glu_part_sum_kernel<<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>(
+      part, parts, n / 4, stride / 4, static_cast<__nv_bfloat16*>(out));
+  return cudaGetLastError();
+}
+
+// Parts of dx's contraction: of kMaxSteps at most, and where its output tiles are at most
+// half the pairs of SMs (a tile walks 2 I / 64 steps alone) up to 16 of 8 steps or more.  The
+// whole backward of 2048 x 5632: 16 tokens 74 -> 40 us, 256 81 -> 46, 1000 105 -> 88.
 int tc_dx_parts(int M, int D, int I, int* steps) {
   const int ksteps = 2 * ceil_div(I, kBK), pairs = 74;
   const long long tiles = (long long)ceil_div(M, kTile) * ceil_div(D, kTile);
-  *steps = ksteps;
-  if (tiles <= 0 || 2 * tiles > pairs) return 1;
-  int parts = (int)(pairs / tiles);
-  if (parts > 16) parts = 16;
-  if (parts > ksteps / 8) parts = ksteps / 8;
-  if (parts <= 1) return 1;
-  *steps = ceil_div(ksteps, parts);
-  return ceil_div(ksteps, *steps);
+  int parts = ceil_div(ksteps, kMaxSteps);
+  if (tiles > 0 && 2 * tiles <= pairs)
+    parts = std::max(parts, (int)std::min(std::min(pairs / tiles, 16LL), ksteps / 8LL));
+  *steps = parts > 1 ? ceil_div(ksteps, parts) : ksteps;
+  return parts > 1 ? ceil_div(ksteps, *steps) : 1;
+}
+
+// Parts of the weights' gradients' contraction over M tokens.
+int tc_dw_parts(int M, int* steps) {
+  const int ksteps = ceil_div(M, kBK), parts = ceil_div(ksteps, kMaxSteps);
+  *steps = parts > 1 ? ceil_div(ksteps, parts) : ksteps;
+  return parts > 1 ? ceil_div(ksteps, *steps) : 1;
 }
 
 cudaError_t launch_few(const GluArgs& a, cudaStream_t st) {
@@ -605,9 +625,15 @@ cudaError_t launch_few(const GluArgs& a, cudaStream_t st) {
 
 GDN_DEVICE_ERROR_ACCESSOR(device_error_glu_tc)
 
+// The forward's contraction is not cut (its sums never reach HBM), so D ends where an
+// accumulator would take 2048 steps (0.7e-3 short at most, by the figures at kMaxSteps);
+// wider inputs run on the CUDA cores, whose sums round to nearest.
+bool glu_tc_widths(int D, int I, int dtype) {
+  return dtype == kBF16 && D % 8 == 0 && I % 8 == 0 && D <= 4 * kMaxSteps * kBK;
+}
+
 bool glu_tc_supported(int M, int D, int I, int dtype) {
-  return dtype == kBF16 && M > 0 && D > 0 && I > 0 && D % 8 == 0 && I % 8 == 0 &&
-         encode_fn() != nullptr;
+  return M > 0 && D > 0 && I > 0 && glu_tc_widths(D, I, dtype) && encode_fn() != nullptr;
 }
 
 cudaError_t launch_glu_tc_fwd(const GluArgs& a, cudaStream_t st) {
@@ -628,8 +654,9 @@ cudaError_t launch_glu_tc_fwd(const GluArgs& a, cudaStream_t st) {
 
 size_t glu_tc_part_floats(int M, int D, int I) {
   int steps;
-  const int parts = tc_dx_parts(M, D, I, &steps);
-  return parts > 1 ? (size_t)parts * ceil_div(M, kTile) * kTile * D : 0;
+  const int dx = tc_dx_parts(M, D, I, &steps), dw = tc_dw_parts(M, &steps);
+  return std::max(dx > 1 ? (size_t)dx * ceil_div(M, kTile) * kTile * D : 0,
+                  dw > 1 ? (size_t)dw * 2 * ceil_div(I, kTile) * kTile * D : 0);
 }
 
 cudaError_t launch_glu_tc_bwd(const GluBwdArgs& a, cudaStream_t st) {
@@ -645,15 +672,11 @@ cudaError_t launch_glu_tc_bwd(const GluBwdArgs& a, cudaStream_t st) {
     const int padded = sh.tiles_m * kTile;   // rows of a part
     if (sh.parts > 1) {
       sh.rows = sh.parts * padded;
-      if (!make_map(&m.out[1], a.part, sh.rows, a.D, 128, true)) return cudaErrorInvalidValue;
+      if (!make_map(&m.out[2], a.part, sh.rows, a.D, 128, true)) return cudaErrorInvalidValue;
     }
     cudaError_t e = launch_kind<kDx>(m, sh, st);
-    if (e == cudaSuccess && sh.parts > 1) {
-      const long long n = (long long)a.M * a.D / 4;
-      glu_dx_sum_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(
-          a.part, sh.parts, n, (long long)padded * a.D / 4, static_cast<__nv_bfloat16*>(a.dx));
-      e = cudaGetLastError();
-    }
+    if (e == cudaSuccess && sh.parts > 1)
+      e = sum_parts(a.part, sh.parts, (long long)a.M * a.D, (long long)padded * a.D, a.dx, st);
     if (e != cudaSuccess) return e;
   }
   if (a.dwg) {
@@ -663,9 +686,20 @@ cudaError_t launch_glu_tc_bwd(const GluBwdArgs& a, cudaStream_t st) {
       return cudaErrorInvalidValue;
     m.b[1] = m.b[0];
     m.out[2] = m.out[1];
-    const GluShape sh{ceil_div(a.I, kTile), ceil_div(a.D, kTile), ceil_div(a.M, kBK), 0,
-                      a.I, a.D};
-    return launch_kind<kDw>(m, sh, st);
+    GluShape sh{ceil_div(a.I, kTile), ceil_div(a.D, kTile), ceil_div(a.M, kBK), 0, a.I, a.D};
+    sh.parts = tc_dw_parts(a.M, &sh.part_steps);
+    const long long seg = (long long)sh.tiles_m * kTile * a.D;   // a part's dWg, or its dWu
+    if (sh.parts > 1) {
+      sh.rows = sh.parts * 2 * sh.tiles_m * kTile;
+      if (!make_map(&m.out[2], a.part, sh.rows, a.D, 128, true)) return cudaErrorInvalidValue;
+    }
+    cudaError_t e = launch_kind<kDw>(m, sh, st);
+    const long long n = (long long)a.I * a.D;
+    if (e == cudaSuccess && sh.parts > 1)
+      e = sum_parts(a.part, sh.parts, n, 2 * seg, a.dwg, st);
+    if (e == cudaSuccess && sh.parts > 1)
+      e = sum_parts(a.part + seg, sh.parts, n, 2 * seg, a.dwu, st);
+    return e;
   }
   return cudaSuccess;
 }

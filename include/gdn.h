@@ -417,8 +417,8 @@ int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
  * transposed), h [M, I], all bf16 or all fp32, products summed in fp32.  g and
  * u [M, I] (both or neither) receive the two projections for the backward, in
  * the same dtype.  Outputs overlap no input.  bf16 with D and I multiples of 8
- * runs on the tensor cores (sizes up to 2^30), the rest on CUDA cores (up to
- * 65535 * 64).
+ * and D up to 131072 runs on the tensor cores (M and I up to 2^30), the rest on
+ * CUDA cores (sizes up to 65535 * 64).
  */
 int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, void* g, void* u,
                 int M, int D, int I, int dtype, void* stream);
@@ -428,7 +428,8 @@ int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, vo
  * wanted), dw_gate and dw_up [I, D] (both or neither), in the inputs' dtype;
  * outputs overlap no input.
  * `workspace`: gdn_glu_bwd_workspace_bytes() bytes (the gradients of g and u in
- * the inputs' dtype; partial sums of the weights' where those need them).
+ * the inputs' dtype; fp32 partial sums of dx, then of the weights' gradients,
+ * where a product's contraction is cut into parts).
  */
 size_t gdn_glu_bwd_workspace_bytes(int M, int D, int I, int dtype);
 int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void* g, const void* u,

@@ -1,0 +1,73 @@
+"""Faults that the block operators once had, each with the call that showed it, and
+the calls around them.  Tolerances: a stored bf16 value is off by at most 2^-8 of it,
+an fp32 one by 2^-24; an fp32 sum of n terms by n 2^-24 of the terms' magnitudes."""
+
+import pytest
+import torch
+
+from gated_deltanet_jax_b200 import _lib, gated_linear_unit
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(cuda, seed):
+    return torch.Generator(device=cuda).manual_seed(seed)
+
+
+# ---------------------------------------------------------------------------
+# gated linear unit: long contractions on the tensor cores
+# ---------------------------------------------------------------------------
+
+def _silu_grads(g, u, dh):
+    s = torch.sigmoid(g)
+    return dh * u * (s * (1 + g * (1 - s))), dh * (g * s)
+
+
+def _sum_error(out, ref, what):
+    """Sums of positive terms: each accumulator takes 32768 of them at most (2^-9), its
+    operands are rounded one by one to either side (below 1e-4 of a sum of so many), and
+    the result once."""
+    off = (out.double() - ref) / ref
+    assert float(off.mean().abs()) <= 2.0 ** -9 + 2e-4, (what, off.mean())
+    assert float(off.abs().max()) <= 2.0 ** -8 + 2.0 ** -9 + 2e-4, (what, off.abs().max())
+
+
+@pytest.mark.parametrize("M,D,I", [(32768, 64, 96), (32769, 72, 40), (100_000, 64, 96),
+                                   ((1 << 20) + 77, 64, 264)])
+def test_glu_weight_gradients_of_many_tokens(cuda, M, D, I):
+    """The weights' gradients are sums over the tokens, however many."""
+    gen = _gen(cuda, M)
+    rand = lambda *s: torch.rand(*s, device=cuda, generator=gen).bfloat16()   # noqa: E731
+    x, dh = rand(M, D), rand(M, I)
+    wg, wu = ((rand(I, D) * 0.02).requires_grad_(True) for _ in range(2))
+    dg, du = torch.autograd.grad(gated_linear_unit(x, wg, wu), [wg, wu], dh)
+    xd = x.double()
+    a, b = _silu_grads(xd @ wg.detach().double().T, xd @ wu.detach().double().T, dh.double())
+    _sum_error(dg, a.T @ xd, "dwg")
+    _sum_error(du, b.T @ xd, "dwu")
+    assert _lib.load().gdn_device_error(0) == 0
+
+
+@pytest.mark.parametrize("M,D,I", [(3, 64, 70_000), (300, 72, 40_000)])
+def test_glu_input_gradient_of_many_columns(cuda, M, D, I):
+    """dx is one sum over both projections' columns."""
+    gen = _gen(cuda, I)
+    rand = lambda *s: torch.rand(*s, device=cuda, generator=gen).bfloat16()   # noqa: E731
+    x, dh = rand(M, D).requires_grad_(True), rand(M, I)
+    wg, wu = rand(I, D) * 0.02, rand(I, D) * 0.02
+    (dx,) = torch.autograd.grad(gated_linear_unit(x, wg, wu), [x], dh)
+    xd, gd, ud = x.detach().double(), wg.double(), wu.double()
+    a, b = _silu_grads(xd @ gd.T, xd @ ud.T, dh.double())
+    _sum_error(dx, a @ gd + b @ ud, "dx")
+    assert _lib.load().gdn_device_error(0) == 0
+
+
+def test_glu_inputs_wider_than_the_tensor_core_form(cuda):
+    """D past 131072 runs on the CUDA cores."""
+    gen = _gen(cuda, 1)
+    D = 131072 + 8
+    x = torch.rand(3, D, device=cuda, generator=gen).bfloat16()
+    w = (torch.rand(2, 16, D, device=cuda, generator=gen) * 1e-5).bfloat16()
+    h = gated_linear_unit(x, w[0], w[1])
+    g, u = x.double() @ w[0].double().T, x.double() @ w[1].double().T
+    _sum_error(h, g * torch.sigmoid(g) * u, "h")
