@@ -828,8 +828,14 @@ int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
   }
   if (!x || !dy || !dx || !aligned16(x) || !aligned16(dy) || !aligned16(dx))
     return fail(GDN_ERR_INVALID, "x, dy and dx must be non-NULL and 16-byte aligned");
-  if (dx == x || dx == dy)
-    return fail(GDN_ERR_INVALID, "dx may not be x or dy: a token's gradient reads its neighbours");
+  // (a tile reads rows that its neighbours own, and the final window's gradient after the
+  // first one's has been written)
+  if (dx == x || dx == dy || dx == state_in || dx == dstate_out)
+    return fail(GDN_ERR_INVALID, "dx may not be x, dy or a window: later tokens read them");
+  if (dstate_in && (dstate_in == x || dstate_in == dy || dstate_in == state_in ||
+                    dstate_in == dstate_out || dstate_in == dx))
+    return fail(GDN_ERR_INVALID, "dstate_in may not be x, dy, dx or a window: later tokens read "
+                                 "them");
   rc = check_workspace(workspace, ws_bytes,
                        gdn::short_conv_bwd_workspace_bytes(B, T, C, K, dtype),
                        "gdn_short_conv_bwd_workspace_bytes");

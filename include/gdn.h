@@ -399,8 +399,9 @@ int gdn_short_conv_fwd_bias(const void* x, const float* weight, const float* bia
  * convolution with JAX).  dy [B, T, C] and dstate_out [B, K - 1, C] (NULL:
  * zero) are the gradients of y and of the final state, in x's dtype.  Written:
  * dx [B, T, C] and dstate_in [B, K - 1, C] (NULL: not wanted) in x's dtype,
- * dweight [K, C] and dbias [C] (NULL: not wanted) in fp32.  dx may not be x or
- * dy.  `workspace`: gdn_short_conv_bwd_workspace_bytes() bytes.  The sums over
+ * dweight [K, C] and dbias [C] (NULL: not wanted) in fp32.  dx and dstate_in
+ * overlap none of x, dy, state_in and dstate_out, nor each other (no form in
+ * place, unlike the forward's state).  `workspace`: gdn_short_conv_bwd_workspace_bytes() bytes.  The sums over
  * tokens run in a fixed order.
  */
 size_t gdn_short_conv_bwd_workspace_bytes(int B, int T, int C, int K);
