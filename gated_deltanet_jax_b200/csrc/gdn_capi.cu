@@ -877,19 +877,26 @@ int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void*
     if (p && !aligned16(p)) return fail(GDN_ERR_INVALID, "the gradients must be 16-byte aligned");
   if ((dx && (dx == x || dx == dh)) || (dw_gate && (dw_gate == w_gate || dw_up == w_up)))
     return fail(GDN_ERR_INVALID, "the gradients may not be the inputs: later products read them");
-  if (M > 0 && I > 0) {
-    const void* ptrs[3] = {g, u, dh};
-    for (const void* p : ptrs)
-      if (!p || !aligned16(p))
-        return fail(GDN_ERR_INVALID, "g, u and dh must be non-NULL and 16-byte aligned");
-    rc = check_workspace(workspace, ws_bytes, gdn_glu_bwd_workspace_bytes(M, D, I, dtype),
-                         "gdn_glu_bwd_workspace_bytes");
-    if (rc) return rc;
+  if (M == 0 || D == 0 || I == 0) {
+    // no output depends on the inputs that are left
+    const size_t e = dtype == GDN_DTYPE_BF16 ? 2 : 4;
+    const size_t nx = (size_t)M * D * e, nw = (size_t)I * D * e;
+    if (dx && nx) rc = carry(dx, nullptr, nx, stream, "gdn_glu_bwd");
+    if (!rc && dw_gate && nw) rc = carry(dw_gate, nullptr, nw, stream, "gdn_glu_bwd");
+    if (!rc && dw_up && nw) rc = carry(dw_up, nullptr, nw, stream, "gdn_glu_bwd");
+    return rc;
   }
+  const void* ptrs[3] = {g, u, dh};
+  for (const void* p : ptrs)
+    if (!p || !aligned16(p))
+      return fail(GDN_ERR_INVALID, "g, u and dh must be non-NULL and 16-byte aligned");
+  rc = check_workspace(workspace, ws_bytes, gdn_glu_bwd_workspace_bytes(M, D, I, dtype),
+                       "gdn_glu_bwd_workspace_bytes");
+  if (rc) return rc;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const size_t half = glu_half_bytes(M, I, dtype);
-  gdn::GluBwdArgs a{x, w_gate, w_up, g, u, dh, ws, ws ? ws + half : nullptr, dx, dw_gate, dw_up,
-                    reinterpret_cast<float*>(ws ? ws + 2 * half : nullptr), M, D, I, dtype};
+  gdn::GluBwdArgs a{x, w_gate, w_up, g, u, dh, ws, ws + half, dx, dw_gate, dw_up,
+                    reinterpret_cast<float*>(ws + 2 * half), M, D, I, dtype};
   return cuda_status(gdn::launch_glu_bwd(a, (cudaStream_t)stream), "gdn_glu_bwd");
 }
 

@@ -333,7 +333,7 @@ struct GluArgs {
 };
 cudaError_t launch_glu_fwd(const GluArgs& a, cudaStream_t st);
 // Its gradients from g, u and dh [M,I]; dg, du [M,I] and part (glu_part_floats()
-// floats) are scratch.  dx [M,D] or NULL; dwg, dwu [I,D] or both NULL.
+// floats) are scratch.  dx [M,D] or NULL; dwg, dwu [I,D] or both NULL.  No size is zero.
 size_t glu_part_floats(int M, int D, int I, int dtype);
 struct GluBwdArgs {
   const void* x;

@@ -523,7 +523,7 @@ cudaError_t bwd_products_simt(const GluBwdArgs& a, cudaStream_t st) {
           *wu = static_cast<const T*>(a.wu), *dg = static_cast<const T*>(a.dg),
           *du = static_cast<const T*>(a.du);
   cudaError_t e = cudaSuccess;
-  if (a.dx && a.M > 0) {
+  if (a.dx) {
     const SimtPlan p = simt_plan(kDx, a.M, a.D, a.I, a.dtype == kFP32);
     const long long n = (long long)a.M * a.D;
     T* dx = p.parts > 1 ? reinterpret_cast<T*>(a.part) : static_cast<T*>(a.dx);
@@ -564,12 +564,8 @@ cudaError_t launch_glu_fwd(const GluArgs& a, cudaStream_t st) {
 }
 
 cudaError_t launch_glu_bwd(const GluBwdArgs& a, cudaStream_t st) {
-  if (a.M > 0 && a.I > 0) {
-    const cudaError_t e =
-        a.dtype == kBF16 ? act_bwd<__nv_bfloat16>(a, st) : act_bwd<float>(a, st);
-    if (e != cudaSuccess) return e;
-  }
-  if (a.D == 0) return cudaSuccess;
+  const cudaError_t e = a.dtype == kBF16 ? act_bwd<__nv_bfloat16>(a, st) : act_bwd<float>(a, st);
+  if (e != cudaSuccess) return e;
   if (glu_tc_supported(a.M, a.D, a.I, a.dtype)) return launch_glu_tc_bwd(a, st);
   return a.dtype == kBF16 ? bwd_products_simt<__nv_bfloat16>(a, st)
                           : bwd_products_simt<float>(a, st);

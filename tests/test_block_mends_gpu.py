@@ -71,3 +71,24 @@ def test_glu_inputs_wider_than_the_tensor_core_form(cuda):
     h = gated_linear_unit(x, w[0], w[1])
     g, u = x.double() @ w[0].double().T, x.double() @ w[1].double().T
     _sum_error(h, g * torch.sigmoid(g) * u, "h")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,D,I", [(0, 64, 40), (5, 64, 0), (0, 64, 0), (5, 0, 40), (0, 33, 7),
+                                   (5, 33, 0), (0, 64, 5_000_000)])
+def test_glu_backward_of_empty_sizes(cuda, dtype, M, D, I):
+    """Through the C entry point, with every pointer given: what depends on nothing is
+    zero, and nothing else is written."""
+    lib = _lib.load()
+    n = max(M * D, I * D, 1)
+    bufs = [torch.full((n + 64,), 3.0, device=cuda, dtype=dtype) for _ in range(9)]
+    x, wg, wu, g, u, dh, dx, dwg, dwu = (t.data_ptr() for t in bufs)
+    kind = {torch.bfloat16: _lib.GDN_DTYPE_BF16, torch.float32: _lib.GDN_DTYPE_FP32}[dtype]
+    if I > 65535 * 64 and dtype == torch.float32:
+        I = 4_000_000
+    st = torch.cuda.current_stream().cuda_stream
+    rc = lib.gdn_glu_bwd(x, wg, wu, g, u, dh, dx, dwg, dwu, M, D, I, kind, None, 0, st)
+    assert rc == _lib.GDN_OK, lib.gdn_last_error()
+    for t, k in zip(bufs[6:], (M * D, I * D, I * D)):
+        assert float(t[:k].abs().sum()) == 0.0 and bool((t[k:] == 3.0).all())
+    assert all(bool((t == 3.0).all()) for t in bufs[:6])
