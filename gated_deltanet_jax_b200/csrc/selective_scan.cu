@@ -28,6 +28,8 @@
 // a second kernel chains the chunks' entering states, and the main pass starts
 // every chunk from its own.  The exponentials are computed twice, so only rows
 // that leave most SMs idle are cut.
+#include <type_traits>
+
 #include "selective_scan_common.cuh"
 
 namespace gdn {
@@ -41,7 +43,10 @@ constexpr int kRows = kTT / kSRows;                         // staging rows per 
 
 // kLocal: the first pass of a cut row (from zero; the end state and the steps'
 // sum out, no y).  chunk / nchunk: tokens of a chunk and their number (grid z).
-template <typename T, int NL, bool kLocal>
+// kTail: the row ends inside a tile.  The factors of the tokens past its end are not
+// formed: with A = -inf a step of zero would make them NaN.  (A form of its own, so that
+// whole tiles do not carry it: 8 x 2048 x 4096 in bf16 514 us with it, 500 without.)
+template <typename T, int NL, bool kLocal, bool kTail>
 __global__ void __launch_bounds__(kFwdThreads, NL > 8 ? 4 : 7)
 scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int nchunk) {
   constexpr int NP = NL * kScanLanes;
@@ -129,8 +134,7 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
       for (int e = 0; e < 4; ++e) {
         d[e] += bias[e];
         if (a.softplus) d[e] = softplus_fast(d[e]);
-        if (t0 + tl >= tend) d[e] = 0.f;   // past the end: the state stays
-        if (kLocal) dsum[e] += d[e];
+        if (kLocal) dsum[e] += d[e];   // (its chunks are whole tiles)
       }
       float* du = reinterpret_cast<float*>(&sDU[tl][sc]);
       store4(du, make_float4(d[0], d[0] * xf[0], d[1], d[1] * xf[1]));
@@ -160,8 +164,10 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
       }
     }
     if (t0 + kTT < tend) fetch(t0 + kTT);
-#pragma unroll 1
-    for (int g = 0; g < kTT; g += 4) {
+    // Four tokens from g on; kRagged: the row ends among them.
+    const int left = kTail ? min(kTT, tend - t0) : kTT;
+    auto group = [&](int g, auto ragged) {
+      constexpr bool kRagged = decltype(ragged)::value;
       if (!kLocal && a.ckpt && g % CK == 0 && t0 + g < a.T) {
         float* ck = a.ckpt + (((size_t)b * a.nck + (t0 + g) / CK) * a.C + c0 + chl) * NP + q * NL;
 #pragma unroll
@@ -171,6 +177,10 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
       float ys[2][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        if (kRagged && g + j >= left) {
+          ys[0][j] = ys[1][j] = 0.f;
+          continue;
+        }
         const float4 du = load4(reinterpret_cast<const float*>(&sDU[g + j][chl]));
         float2 B2[P], C2[P];
         load_pairs<NL>(&sB[g + j][q * NL], B2);
@@ -196,7 +206,11 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
         v.y += quad_sum4(ys[1][0], ys[1][1], ys[1][2], ys[1][3], lane);
         *yp = v;
       }
-    }
+    };
+    const int whole = left / 4 * 4;
+#pragma unroll 1
+    for (int g = 0; g < whole; g += 4) group(g, std::false_type{});
+    if (kTail && whole < left) group(whole, std::true_type{});
     __syncthreads();
     if (!kLocal) {
 #pragma unroll
@@ -392,13 +406,19 @@ template <typename T, int NL>
 cudaError_t launch_fwd(const ScanArgs& a, int tpg, int vec, const ScanSplit& sp, cudaStream_t st) {
   const dim3 grid((unsigned)(tpg * a.G), a.B, sp.chunks);
   if (sp.chunks > 1) {
-    scan_fwd_kernel<T, NL, true><<<dim3(grid.x, grid.y, sp.chunks - 1), kFwdThreads, 0, st>>>(
-        a, tpg, vec, sp.tokens, sp.chunks);
+    scan_fwd_kernel<T, NL, true, false>
+        <<<dim3(grid.x, grid.y, sp.chunks - 1), kFwdThreads, 0, st>>>(a, tpg, vec, sp.tokens,
+                                                                      sp.chunks);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = launch_scan_chain(a, a.h0, sp.chunks, false, st);
     if (e != cudaSuccess) return e;
   }
-  scan_fwd_kernel<T, NL, false><<<grid, kFwdThreads, 0, st>>>(a, tpg, vec, sp.tokens, sp.chunks);
+  if (a.T % kTT)
+    scan_fwd_kernel<T, NL, false, true><<<grid, kFwdThreads, 0, st>>>(a, tpg, vec, sp.tokens,
+                                                                      sp.chunks);
+  else
+    scan_fwd_kernel<T, NL, false, false><<<grid, kFwdThreads, 0, st>>>(a, tpg, vec, sp.tokens,
+                                                                       sp.chunks);
   return cudaGetLastError();
 }
 

@@ -23,6 +23,8 @@
 // first pass 89 (exponential pipe 79 %).  The sums of dB and dC over the block's
 // channels go through shared memory half a tile at a time (shuffles took 31
 // instructions a token for them, this takes 15: 425 to 394 us).
+#include <type_traits>
+
 #include "selective_scan_common.cuh"
 
 namespace gdn {
@@ -33,8 +35,11 @@ constexpr int kBwdThreads = 64;   // 16 slots of four lanes, two channels a lane
 constexpr int kBwdSlots = kBwdThreads / kScanLanes;
 
 // kLocal: the first pass of a cut row (chunks 1 ..: the adjoint from zero over
-// the chunk and the steps' sum out, no gradients).
-template <typename T, int NL, bool kLocal>
+// the chunk and the steps' sum out, no gradients).  kTail: the row ends inside a
+// tile.  The factors of the tokens past its end are not formed: with A = -inf a step of
+// zero would make them NaN.  (A form of its own: 4 x 2048 x 2048 with 16 states 538 us
+// with it, 511 without.)
+template <typename T, int NL, bool kLocal, bool kTail>
 __global__ void __launch_bounds__(kBwdThreads, 4)
 scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, int nchunk,
                 float* __restrict__ pBC, float* __restrict__ pP) {
@@ -181,7 +186,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
     if (k > 0) fetch(t0 - CK);
     if (kLocal) {
 #pragma unroll 4
-      for (int t = CK - 1; t >= 0; --t) {
+      for (int t = (kTail ? min(CK, tend - t0) : CK) - 1; t >= 0; --t) {
         const float4 du = load4(reinterpret_cast<const float*>(&sDU[t][chl]));
         const float2 g = *reinterpret_cast<const float2*>(&sG[t][chl]);
         float2 C2[P];
@@ -201,9 +206,11 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
       continue;
     }
     // Halves of the tile, the later one first, each with its states in registers.
+    // kRagged: the row ends in this one.
     const float* ck = f.ckpt + (((size_t)b * f.nck + t0 / CK) * f.C + c0 + chl) * NP + q * NL;
-#pragma unroll 1
-    for (int hf = 1; hf >= 0; --hf) {
+    const int left = kTail ? tend - t0 : CK;
+    auto half = [&](int hf, auto ragged) {
+      constexpr bool kRagged = decltype(ragged)::value;
       float2 hs[2][P], h[SUB][2][P];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -241,7 +248,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
           for (int i = 0; i < P; ++i) s[c][i] = hs[c][i];
 #pragma unroll
         for (int t = 0; t < SUB; ++t) {
-          advance(base + t, s);
+          if (!kRagged || base + t < left) advance(base + t, s);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -256,6 +263,7 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
 #pragma unroll
         for (int j = QT - 1; j >= 0; --j) {
           const int tl = g0 + j, t = base + tl;
+          if (kRagged && t >= left) continue;
           const float4 du = load4(reinterpret_cast<const float*>(&sDU[t][chl]));
           const float2 gg = *reinterpret_cast<const float2*>(&sG[t][chl]);
           float2 B2[P], C2[P], dBv[P], dCv[P];
@@ -348,6 +356,11 @@ scan_bwd_kernel(const ScanBwdArgs a, int tiles_per_group, int vec, int chunk, in
         }
       }
       __syncthreads();
+    };
+#pragma unroll 1
+    for (int hf = 1; hf >= 0; --hf) {
+      if (hf * SUB + SUB <= left) half(hf, std::false_type{});
+      else if (kTail && hf * SUB < left) half(hf, std::true_type{});
     }
     // dx, ddt, dz
     if (stages) {
@@ -439,20 +452,28 @@ sum_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict_
     if (n % NP + e < N) out[n % NP + e] = from_f32<T>(v[e]);
 }
 
-template <typename T, int NL>
+template <typename T, int NL, bool kTail>
 cudaError_t bwd_form(const ScanBwdArgs& a, int tpg, int vec, const ScanSplit& sp, float* pBC,
                      float* pP, cudaStream_t st) {
   const dim3 grid((unsigned)(tpg * a.fwd.G), a.fwd.B, sp.chunks);
   if (sp.chunks > 1) {
-    scan_bwd_kernel<T, NL, true><<<dim3(grid.x, grid.y, sp.chunks - 1), kBwdThreads, 0, st>>>(
-        a, tpg, vec, sp.tokens, sp.chunks, nullptr, nullptr);
+    scan_bwd_kernel<T, NL, true, kTail>
+        <<<dim3(grid.x, grid.y, sp.chunks - 1), kBwdThreads, 0, st>>>(
+            a, tpg, vec, sp.tokens, sp.chunks, nullptr, nullptr);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = launch_scan_chain(a.fwd, a.dhT, sp.chunks, true, st);
     if (e != cudaSuccess) return e;
   }
-  scan_bwd_kernel<T, NL, false><<<grid, kBwdThreads, 0, st>>>(a, tpg, vec, sp.tokens, sp.chunks,
-                                                              pBC, pP);
+  scan_bwd_kernel<T, NL, false, kTail><<<grid, kBwdThreads, 0, st>>>(a, tpg, vec, sp.tokens,
+                                                                     sp.chunks, pBC, pP);
   return cudaGetLastError();
+}
+
+template <typename T, int NL>
+cudaError_t bwd_form(const ScanBwdArgs& a, int tpg, int vec, const ScanSplit& sp, float* pBC,
+                     float* pP, cudaStream_t st) {
+  return a.fwd.T % scan_tile<NL>() ? bwd_form<T, NL, true>(a, tpg, vec, sp, pBC, pP, st)
+                                   : bwd_form<T, NL, false>(a, tpg, vec, sp, pBC, pP, st);
 }
 
 // The workspace's parts, in floats from its start.

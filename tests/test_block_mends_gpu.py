@@ -5,7 +5,8 @@ an fp32 one by 2^-24; an fp32 sum of n terms by n 2^-24 of the terms' magnitudes
 import pytest
 import torch
 
-from gated_deltanet_jax_b200 import _lib, gated_linear_unit
+from gated_deltanet_jax_b200 import _lib, gated_linear_unit, selective_scan
+from test_block_ops_gpu import GRAD, HALF, _f64, _names, _scan_inputs, _scan_ref, _scan_tol
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +93,43 @@ def test_glu_backward_of_empty_sizes(cuda, dtype, M, D, I):
     for t, k in zip(bufs[6:], (M * D, I * D, I * D)):
         assert float(t[:k].abs().sum()) == 0.0 and bool((t[k:] == 3.0).all())
     assert all(bool((t == 3.0).all()) for t in bufs[:6])
+
+
+# ---------------------------------------------------------------------------
+# selective scan: states without memory, growing states
+# ---------------------------------------------------------------------------
+
+def _close(out, ref, tol, what):
+    """Within the tolerance, and NaN where the reference is."""
+    out = _f64(out)
+    assert torch.equal(out.isnan(), ref.isnan()), what
+    off = torch.where(ref.isnan(), torch.zeros_like(ref), (out - ref).abs() - tol.nan_to_num(0.0))
+    assert bool((off <= 0).all()), (what, off.max())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("case", [(2, 1, 36, 16, 1, True), (2, 1, 20, 24, 2, True),
+                                  (1, 2, 33, 16, 1, True), (2, 15, 40, 4, 1, True),
+                                  (2, 16, 40, 8, 1, False), (1, 17, 40, 16, 1, True),
+                                  (1, 20, 24, 32, 2, True), (1, 22, 24, 64, 1, True),
+                                  (2, 32, 40, 16, 1, True), (3, 33, 40, 16, 1, True),
+                                  (1, 300, 34, 12, 2, False), (1, 701, 40, 16, 1, True)])
+def test_scan_states_without_memory(cuda, dtype, case):
+    """A = -inf: a decay of zero at every length, whatever tile it ends in."""
+    b, T, ch, N, G, full = case
+    s, dy, dhT = _scan_inputs(*case, dtype, cuda, T + N)
+    s["A"][1::5, ::3] = -float("inf")
+    y, st = selective_scan(**s, output_final_state=True)          # (one token: the step kernels)
+    ref, mag = _scan_ref(s, True, dy, dhT), _scan_ref(s, True, dy, dhT, absval=True)
+    assert bool(ref["state"].isfinite().all()) and bool(ref["y"].isfinite().all())
+    _close(y, ref["y"], _scan_tol(ref, mag, "y", T, 0, 0, HALF[dtype]), "y")
+    _close(st, ref["state"], _scan_tol(ref, mag, "state", T, 0, 0, HALF["fp32"]), "state")
+    names = _names(s)
+    for k in names:
+        s[k].requires_grad_(True)
+    out = selective_scan(**s, output_final_state=True)
+    _close(out[1], ref["state"], _scan_tol(ref, mag, "state", T, 0, 0, HALF["fp32"]), "state")
+    for k, g in zip(names, torch.autograd.grad(out, [s[k] for k in names], (dy, dhT))):
+        key = GRAD.get(k, "d" + k)
+        half = HALF["bf16"] if g.dtype == torch.bfloat16 else HALF["fp32"]
+        _close(g, ref[key], _scan_tol(ref, mag, key, 2 * T, ch, b * T, half), key)
