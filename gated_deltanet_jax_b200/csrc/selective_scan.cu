@@ -255,7 +255,9 @@ scan_fwd_kernel(const ScanArgs a, int tiles_per_group, int vec, int chunk, int n
 // Chains a cut row's chunks: state [chunk][rows = B C][NP] holds each chunk's end
 // from zero (the last chunk's is not read) and takes the state entering it.
 // kReverse: from the last chunk to the first (the backward's adjoint states),
-// the sum of steps being that of the chunk the state leaves through.
+// the sum of steps being that of the chunk the state leaves through.  A chunk's decay may
+// leave fp32's range where the state does not (A > 0 and a state of zero or near it, or a
+// large one that shrinks): it enters as its square root, twice, and not at all at zero.
 template <bool kReverse>
 __global__ void __launch_bounds__(256)
 scan_chain_kernel(float* __restrict__ state, const float* __restrict__ sum,
@@ -265,7 +267,7 @@ scan_chain_kernel(float* __restrict__ state, const float* __restrict__ sum,
   const long long row = i / NP;
   const int n = (int)(i % NP);
   if (row >= rows) return;
-  const float a2 = n < N ? A[(row % C) * N + n] * kLog2e : 0.f;
+  const float a2 = n < N ? A[(row % C) * N + n] * (0.5f * kLog2e) : 0.f;
   float h = n < N && first ? first[row * N + n] : 0.f;
   constexpr int kAt = 8;   // chunks whose loads are in flight under eight others' steps
   float loc[kAt], dec[kAt];
@@ -293,7 +295,7 @@ scan_chain_kernel(float* __restrict__ state, const float* __restrict__ sum,
       const int s = s0 + j;
       if (s >= nchunk) break;
       state[(kReverse ? nchunk - 1 - s : s) * rows * NP + i] = h;
-      h = fmaf(d[j], h, l[j]);
+      h = h == 0.f ? l[j] : fmaf(d[j], d[j] * h, l[j]);
     }
   }
 }

@@ -133,3 +133,36 @@ def test_scan_states_without_memory(cuda, dtype, case):
         key = GRAD.get(k, "d" + k)
         half = HALF["bf16"] if g.dtype == torch.bfloat16 else HALF["fp32"]
         _close(g, ref[key], _scan_tol(ref, mag, key, 2 * T, ch, b * T, half), key)
+
+
+@pytest.mark.parametrize("zero_start", [True, False])
+def test_scan_growing_states_in_cut_rows(cuda, zero_start):
+    """A > 0 with a chunk's factor (e^128) past fp32's range, where no state is: states
+    of zero until the last token, and a tiny one that grows and shrinks again."""
+    T, ch, N = 1024, 32, 16
+    s, dy, dhT = _scan_inputs(1, T, ch, N, 1, True, "fp32", cuda, 3)
+    s.update(dt=torch.zeros_like(s["dt"]), dt_bias=None, A=torch.ones_like(s["A"]))
+    assert _lib.load().gdn_selective_scan_workspace_bytes(1, T, ch, N, 1) > 0     # it is cut
+    s["A"][:, 1::2] = 0.5
+    s["x"][:, :-1] = 0.0
+    if zero_start:
+        s["initial_state"] = None
+        s["dt"] += 1.0
+        dy, dhT = dy.clone(), torch.zeros_like(dhT)
+        dy[:, 1:] = 0.0                                 # (the adjoint states likewise)
+    else:
+        s["dt"][:, 128:256] = 1.0
+        s["A"][ch // 2:] *= -1.0
+        s["initial_state"][:, :ch // 2] *= 1e-30
+        s["initial_state"][:, ch // 2:] *= 1e30
+        dy, dhT = dy * 1e-36, dhT * 1e-30
+    names = _names(s)
+    for k in names:
+        s[k].requires_grad_(True)
+    y, st = selective_scan(**s, dt_softplus=False, output_final_state=True)
+    grads = torch.autograd.grad((y, st), [s[k] for k in names], (dy, dhT))
+    ref, mag = _scan_ref(s, False, dy, dhT), _scan_ref(s, False, dy, dhT, absval=True)
+    for k, t, n, rows in ([("y", y, T, 0), ("state", st, T, 0)]
+                          + [(GRAD.get(k, "d" + k), g, 2 * T, T) for k, g in zip(names, grads)]):
+        assert float(mag[k].max()) < 1e38                # nothing leaves fp32's range
+        _close(t, ref[k], _scan_tol(ref, mag, k, n, ch, rows, HALF["fp32"]) + 1e-36, k)
