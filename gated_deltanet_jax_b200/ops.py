@@ -543,41 +543,128 @@ def _conv_state(t, name, shape, dtype, dev):
     return t
 
 
+def _alias(t, connect):
+    """``t`` as a point to differentiate at: with ``connect`` still a function of what t
+    came from, else on its own."""
+    if t is None:
+        return None
+    return t.view_as(t) if connect and t.requires_grad else t.detach().requires_grad_(True)
+
+
+def _formula_grads(formula, ts, cots):
+    """Gradients of ``formula(*ts)`` (a tuple) for the cotangents ``cots`` through torch's
+    own operations: where the kernels cannot run (batched cotangents)."""
+    connect = torch.is_grad_enabled()
+    with torch.enable_grad():
+        a = [_alias(t, connect) for t in ts]
+        live = [(o, c) for o, c in zip(formula(*a), cots) if c is not None]
+        wrt = [t for t in a if t is not None]
+        got = iter(torch.autograd.grad([o for o, _ in live], wrt, [c for _, c in live],
+                                       create_graph=connect, allow_unused=True))
+    return tuple(None if t is None else next(got) for t in a)
+
+
+def _formula_second(formula, ts, cots, dds):
+    """The gradients of that: for cotangents ``dds`` of the gradients by ``ts``, the
+    gradients by ``cots`` and by ``ts``, themselves differentiable when grad mode is on."""
+    connect = torch.is_grad_enabled()
+    by = [i for i, d in enumerate(dds) if d is not None and ts[i] is not None]
+    if not by or all(d is None for d in cots):
+        return (None,) * (len(cots) + len(ts))
+    with torch.enable_grad():
+        a, c = [_alias(t, connect) for t in ts], [_alias(t, connect) for t in cots]
+        live = [(o, d) for o, d in zip(formula(*a), c) if d is not None]
+        first = torch.autograd.grad([o for o, _ in live], [a[i] for i in by],
+                                    [d for _, d in live], create_graph=True, allow_unused=True)
+        pairs = [(f, dds[i]) for f, i in zip(first, by) if f is not None and f.requires_grad]
+        both = c + a
+        wrt = [t for t in both if t is not None]
+        got = iter(torch.autograd.grad([f for f, _ in pairs], wrt, [d for _, d in pairs],
+                                       create_graph=connect, allow_unused=True) if pairs
+                   else [None] * len(wrt))
+    return tuple(None if t is None else next(got) for t in both)
+
+
+def _batched(*ts) -> bool:
+    """Tensors that stand for a batch of them and have no data pointer
+    (``torch.autograd.grad(is_grads_batched=True)``)."""
+    ft = torch._C._functorch
+    return any(t is not None and (ft.is_legacy_batchedtensor(t) or ft.is_batchedtensor(t))
+               for t in ts)
+
+
+def _conv_formula(act):
+    """The short convolution in torch's operations, fp32 inside."""
+    def formula(x, w, bias, st):
+        (B, T, C), K = x.shape, w.shape[0]
+        xe = torch.cat([x.new_zeros(B, K - 1, C) if st is None else st, x], 1)
+        pre = sum(w[j] * xe[:, j:j + T].to(w.dtype) for j in range(K))
+        pre = pre if bias is None else pre + bias
+        y = torch.nn.functional.silu(pre) if act else pre
+        return y.to(x.dtype), xe[:, T:]
+    return formula
+
+
+def _short_conv_bwd(dy, ds, x, w, bias, st, act):
+    """gdn_short_conv_bwd: (dx, dw, dbias, dstate), the last two None without theirs."""
+    B, T, C = x.shape
+    K = w.shape[0]
+    dy = torch.zeros_like(x) if dy is None else _aligned(dy)
+    ds = _aligned(ds)
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    db = None if bias is None else torch.empty_like(bias)
+    dst = None if st is None else torch.empty_like(st)
+    lib = _lib.load()
+    dev = x.get_device()
+    with _on_device(dev):
+        n = lib.gdn_short_conv_bwd_workspace_bytes(B, T, C, K)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
+        rc = lib.gdn_short_conv_bwd(
+            _ptr(x), _ptr(w), _ptr(bias), _ptr(st), _ptr(dy), _ptr(ds), _ptr(dx), _ptr(dw),
+            _ptr(db), _ptr(dst), B, T, C, K, act, _DTYPES[x.dtype], _ptr(ws), n,
+            _stream(dev))
+    _lib.check(rc, "gdn_short_conv_bwd")
+    return dx, dw, db, dst
+
+
+# The autograd functions take aligned inputs (weights in fp32 where the kernels want them
+# so): what is saved for the backward is then the inputs themselves, and with
+# create_graph=True the gradients' own graph reaches them.
+
 class _ShortConvFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, conv_state, act):
-        x = _aligned(x)
-        w32, b32, st = _aligned32(w), _aligned32(bias), _aligned(conv_state)
         s_out = x.new_empty((x.shape[0], w.shape[0] - 1, x.shape[2]))
-        y = _short_conv_fwd(x, w32, b32, st, s_out, act)
+        y = _short_conv_fwd(x, w, bias, conv_state, s_out, act)
         ctx.act = act
-        ctx.w_dtype, ctx.b_dtype = w.dtype, None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, w32, b32, st)
+        ctx.save_for_backward(x, w, bias, conv_state)
         return y, s_out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, ds):
-        x, w, bias, st = ctx.saved_tensors
-        B, T, C = x.shape
-        K = w.shape[0]
-        dy = torch.zeros_like(x) if dy is None else _aligned(dy)
-        ds = _aligned(ds)
-        dx, dw = torch.empty_like(x), torch.empty_like(w)
-        db = None if bias is None else torch.empty_like(bias)
-        dst = None if st is None else torch.empty_like(st)
-        lib = _lib.load()
-        dev = x.get_device()
-        with _on_device(dev):
-            n = lib.gdn_short_conv_bwd_workspace_bytes(B, T, C, K)
-            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
-            rc = lib.gdn_short_conv_bwd(
-                _ptr(x), _ptr(w), _ptr(bias), _ptr(st), _ptr(dy), _ptr(ds), _ptr(dx), _ptr(dw),
-                _ptr(db), _ptr(dst), B, T, C, K, ctx.act, _DTYPES[x.dtype], _ptr(ws), n,
-                _stream(dev))
-        _lib.check(rc, "gdn_short_conv_bwd")
-        return (dx, dw.to(ctx.w_dtype), None if db is None else db.to(ctx.b_dtype), dst, None)
+        ts = ctx.saved_tensors
+        if _batched(dy, ds):
+            return _formula_grads(_conv_formula(ctx.act), ts, (dy, ds)) + (None,)
+        run = _ShortConvBwdFn.apply if torch.is_grad_enabled() else _short_conv_bwd
+        return tuple(run(dy, ds, *ts, ctx.act)) + (None,)
+
+
+class _ShortConvBwdFn(torch.autograd.Function):
+    """The backward as a function of its own (create_graph=True): the kernel's gradients,
+    whose derivatives are formed by torch's operations."""
+
+    @staticmethod
+    def forward(ctx, dy, ds, x, w, bias, conv_state, act):
+        ctx.act = act
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(dy, ds, x, w, bias, conv_state)
+        return _short_conv_bwd(dy, ds, x, w, bias, conv_state, act)
+
+    @staticmethod
+    def backward(ctx, *dds):
+        dy, ds, *ts = ctx.saved_tensors
+        return _formula_second(_conv_formula(ctx.act), ts, (dy, ds), dds) + (None,)
 
 
 def _short_conv_fwd(x, w, bias, s_in, s_out, act):
@@ -610,7 +697,8 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
     ``final_state_out`` (which may be ``conv_state``, updated in place) is
     given, else None.  The reference's call is ``short_convolution(x, w)`` (no
     state).  Differentiable in x, weight, bias and conv_state, through y and
-    the returned state (without ``final_state_out``; gdn_short_conv_bwd).
+    the returned state (without ``final_state_out``; gdn_short_conv_bwd), twice too
+    (second derivatives run on torch's operations).
     """
     _cuda_input("x", x)
     if x.dim() != 3:
@@ -635,7 +723,7 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
     if _wants_grad(x, w, bias, conv_state):
         if final_state_out is not None:
             raise NotImplementedError("the backward does not cover final_state_out")
-        y, s_out = _ShortConvFn.apply(x, w, bias, s_in, act)
+        y, s_out = _ShortConvFn.apply(_aligned(x), _aligned32(w), _aligned32(bias), s_in, act)
         return y, s_out if output_final_state else None
     if s_out is None and output_final_state:
         s_out = torch.empty(shape, dtype=x.dtype, device=dev)
@@ -658,33 +746,64 @@ def _glu_fwd(x, wg, wu, keep):
     return h, g, u
 
 
+def _glu_formula(x, wg, wu):
+    """The gated linear unit in torch's operations: products in the inputs' type, the
+    activation in fp32, as the kernels round."""
+    lin = torch.nn.functional.linear
+    g, u = lin(x, wg), lin(x, wu)
+    if x.dtype == torch.bfloat16:
+        g, u = g.float(), u.float()
+    return ((torch.nn.functional.silu(g) * u).to(x.dtype),)
+
+
+def _glu_bwd(dh, x, wg, wu, g, u, need_x, need_w):
+    """gdn_glu_bwd: (dx, dwg, dwu), None where not needed."""
+    (M, D), I = x.shape, wg.shape[0]
+    dh = _aligned(dh)
+    dx = torch.empty_like(x) if need_x else None
+    dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_w else (None, None)
+    lib = _lib.load()
+    dev = x.get_device()
+    with _on_device(dev):
+        n = lib.gdn_glu_bwd_workspace_bytes(M, D, I, _DTYPES[x.dtype])
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
+        rc = lib.gdn_glu_bwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(g), _ptr(u), _ptr(dh),
+                             _ptr(dx), _ptr(dwg), _ptr(dwu), M, D, I, _DTYPES[x.dtype],
+                             _ptr(ws), n, _stream(dev))
+    _lib.check(rc, "gdn_glu_bwd")
+    return dx, dwg, dwu
+
+
 class _GluFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu):
-        x, wg, wu = _aligned(x), _aligned(wg), _aligned(wu)
         h, g, u = _glu_fwd(x, wg, wu, True)
         ctx.save_for_backward(x, wg, wu, g, u)
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         x, wg, wu, g, u = ctx.saved_tensors
-        (M, D), I = x.shape, wg.shape[0]
-        need_x, need_w = ctx.needs_input_grad[0], any(ctx.needs_input_grad[1:])
-        dh = _aligned(dh)
-        dx = torch.empty_like(x) if need_x else None
-        dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_w else (None, None)
-        lib = _lib.load()
-        dev = x.get_device()
-        with _on_device(dev):
-            n = lib.gdn_glu_bwd_workspace_bytes(M, D, I, _DTYPES[x.dtype])
-            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
-            rc = lib.gdn_glu_bwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(g), _ptr(u), _ptr(dh),
-                                 _ptr(dx), _ptr(dwg), _ptr(dwu), M, D, I, _DTYPES[x.dtype],
-                                 _ptr(ws), n, _stream(dev))
-        _lib.check(rc, "gdn_glu_bwd")
-        return dx, dwg, dwu
+        if _batched(dh):
+            return _formula_grads(_glu_formula, (x, wg, wu), (dh,))
+        run = _GluBwdFn.apply if torch.is_grad_enabled() else _glu_bwd
+        return tuple(run(dh, x, wg, wu, g, u, ctx.needs_input_grad[0],
+                         any(ctx.needs_input_grad[1:])))
+
+
+class _GluBwdFn(torch.autograd.Function):
+    """The backward as a function of its own, as _ShortConvBwdFn."""
+
+    @staticmethod
+    def forward(ctx, dh, x, wg, wu, g, u, need_x, need_w):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(dh, x, wg, wu)
+        return _glu_bwd(dh, x, wg, wu, g, u, need_x, need_w)
+
+    @staticmethod
+    def backward(ctx, *dds):
+        dh, *ts = ctx.saved_tensors
+        return _formula_second(_glu_formula, ts, (dh,), dds) + (None,) * 4
 
 
 def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") -> torch.Tensor:
@@ -695,8 +814,9 @@ def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") ->
     x ``[...,D]``, gate_weight and up_weight ``[I,D]`` (torch's Linear layout)
     in one dtype, bfloat16 or float32, on a CUDA device; returns ``[...,I]``.
     ``activation``: ``'silu'`` / ``'swish'``.  Differentiable in all three
-    (gdn_glu_bwd, from the two projections kept in x's dtype).  bfloat16 widths D
-    and I that are multiples of 8 run on the tensor cores, others on CUDA cores.
+    (gdn_glu_bwd, from the two projections kept in x's dtype), twice too (second
+    derivatives run on torch's operations).  bfloat16 widths D and I that are multiples of
+    8 run on the tensor cores, others on CUDA cores.
     """
     _cuda_input("x", x)
     if activation not in ("silu", "swish"):
@@ -712,7 +832,7 @@ def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") ->
                          f"{tuple(gate_weight.shape)}, {tuple(up_weight.shape)}")
     x2 = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), D)
     if _wants_grad(x, gate_weight, up_weight):
-        h = _GluFn.apply(x2, gate_weight, up_weight)
+        h = _GluFn.apply(_aligned(x2), _aligned(gate_weight), _aligned(up_weight))
     else:
         h, _, _ = _glu_fwd(_aligned(x2), _aligned(gate_weight), _aligned(up_weight), False)
     return h if x2 is x else h.reshape(*x.shape[:-1], gate_weight.shape[0])
@@ -741,12 +861,34 @@ def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, keep):
     return y, ck
 
 
+def _scan_bwd(dy, dhT, x, dt, A, B, C, D, z, dt_bias, ck, has_h0, softplus):
+    """gdn_selective_scan_bwd: the gradients of x, dt, A, B, C, D, z, dt_bias and the
+    initial state, None without theirs."""
+    b, T, ch = x.shape
+    G, N = B.shape[2], A.shape[1]
+    dev = x.get_device()
+    dy = torch.zeros_like(x) if dy is None else _aligned(dy)
+    dhT = _aligned32(dhT)
+    like = lambda t: None if t is None else torch.empty_like(t)  # noqa: E731
+    dx, ddt, dA, dB, dC = like(x), like(dt), like(A), like(B), like(C)
+    dD, dz, dbias = like(D), like(z), like(dt_bias)
+    dh0 = torch.empty((b, ch, N), dtype=torch.float32, device=dev) if has_h0 else None
+    lib = _lib.load()
+    with _on_device(dev):
+        n = lib.gdn_selective_scan_bwd_workspace_bytes(b, T, ch, N, G)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+        rc = lib.gdn_selective_scan_bwd(
+            _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
+            _ptr(ck), _ptr(dy), _ptr(dhT), _ptr(dx), _ptr(ddt), _ptr(dA), _ptr(dB), _ptr(dC),
+            _ptr(dD), _ptr(dz), _ptr(dbias), _ptr(dh0), b, T, ch, N, G, softplus,
+            _DTYPES[x.dtype], _ptr(ws), n, _stream(dev))
+    _lib.check(rc, "gdn_selective_scan_bwd")
+    return dx, ddt, dA, dB, dC, dD, dz, dbias, dh0
+
+
 class _SelectiveScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, h0, softplus):
-        x, dt, B, C, z = _aligned(x), _aligned(dt), _aligned(B), _aligned(C), _aligned(z)
-        ctx.dtypes = [None if t is None else t.dtype for t in (A, D, dt_bias, h0)]
-        A, D, dt_bias, h0 = (_aligned32(t) for t in (A, D, dt_bias, h0))
         hT = torch.empty((x.shape[0], x.shape[2], A.shape[1]), dtype=torch.float32,
                          device=x.device)
         y, ck = _scan_fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, True)
@@ -756,31 +898,24 @@ class _SelectiveScanFn(torch.autograd.Function):
         return y, hT
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dhT):
-        x, dt, A, B, C, D, z, dt_bias, ck = ctx.saved_tensors
-        b, T, ch = x.shape
-        G, N = B.shape[2], A.shape[1]
-        dev = x.get_device()
-        dy = torch.zeros_like(x) if dy is None else _aligned(dy)
-        dhT = _aligned32(dhT)
-        like = lambda t: None if t is None else torch.empty_like(t)  # noqa: E731
-        dx, ddt, dA, dB, dC = like(x), like(dt), like(A), like(B), like(C)
-        dD, dz, dbias = like(D), like(z), like(dt_bias)
-        dh0 = torch.empty((b, ch, N), dtype=torch.float32, device=dev) if ctx.has_h0 else None
-        lib = _lib.load()
-        with _on_device(dev):
-            n = lib.gdn_selective_scan_bwd_workspace_bytes(b, T, ch, N, G)
-            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
-            rc = lib.gdn_selective_scan_bwd(
-                _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
-                _ptr(ck), _ptr(dy), _ptr(dhT), _ptr(dx), _ptr(ddt), _ptr(dA), _ptr(dB), _ptr(dC),
-                _ptr(dD), _ptr(dz), _ptr(dbias), _ptr(dh0), b, T, ch, N, G, ctx.softplus,
-                _DTYPES[x.dtype], _ptr(ws), n, _stream(dev))
-        _lib.check(rc, "gdn_selective_scan_bwd")
-        to = lambda t, d: None if t is None else t.to(d)  # noqa: E731
-        Ad, Dd, bd, hd = ctx.dtypes
-        return (dx, ddt, to(dA, Ad), dB, dC, to(dD, Dd), dz, to(dbias, bd), to(dh0, hd), None)
+        if _batched(dy, dhT):
+            raise NotImplementedError("selective_scan's backward takes no batched gradients")
+        run = _SelectiveScanBwdFn.apply if torch.is_grad_enabled() else _scan_bwd
+        return tuple(run(dy, dhT, *ctx.saved_tensors, ctx.has_h0, ctx.softplus)) + (None,)
+
+
+class _SelectiveScanBwdFn(torch.autograd.Function):
+    """The backward with create_graph=True: gradients that say so when they are
+    differentiated, instead of being taken as constants."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _scan_bwd(*args)
+
+    @staticmethod
+    def backward(ctx, *dds):
+        raise NotImplementedError("selective_scan has no second derivatives")
 
 
 def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus: bool = True,
@@ -803,7 +938,8 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
     ``output_final_state`` or ``final_state_out`` is given (decode:
     ``initial_state=S, final_state_out=S`` updates S in place), else None.
     Differentiable in every tensor, through y and the returned state (without
-    ``final_state_out``; gdn_selective_scan_bwd).  Its layer feeds x through
+    ``final_state_out``; gdn_selective_scan_bwd), once: second derivatives raise
+    NotImplementedError.  Its layer feeds x through
     :func:`short_convolution` first.
     """
     _cuda_input("x", x)
@@ -848,7 +984,9 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
     if _wants_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
         if final_state_out is not None:
             raise NotImplementedError("the backward does not cover final_state_out")
-        y, hT = _SelectiveScanFn.apply(x, dt, A, B, C, D, z, dt_bias, initial_state, softplus)
+        y, hT = _SelectiveScanFn.apply(
+            _aligned(x), _aligned(dt), _aligned32(A), _aligned(B), _aligned(C), _aligned32(D),
+            _aligned(z), _aligned32(dt_bias), _aligned32(initial_state), softplus)
         return y, hT if output_final_state else None
     hT = final_state_out
     if hT is not None:

@@ -4,8 +4,10 @@
 import ctypes
 
 import pytest
+import torch
 
-from gated_deltanet_jax_b200 import _build, _lib
+import block_refs as refs
+from gated_deltanet_jax_b200 import _build, _lib, ops
 
 BF16, FP32 = _lib.GDN_DTYPE_BF16, _lib.GDN_DTYPE_FP32
 INVALID = _lib.GDN_ERR_INVALID
@@ -36,3 +38,126 @@ def test_conv_backward_refuses_its_inputs_as_outputs(lib, out, other):
                                   a["dw"], None, a["dst"], 2, 1000, 64, 4, 1, BF16, _at(9), need,
                                   None) == INVALID
     assert b"may not be" in lib.gdn_last_error()
+
+
+# ---------------------------------------------------------------------------
+# second derivatives: the autograd functions with the library's calls replaced by
+# the 64-bit references
+# ---------------------------------------------------------------------------
+
+def _rand(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+
+
+@pytest.fixture
+def reference_calls(monkeypatch):
+    def conv_fwd(x, w, bias, s_in, s_out, act):
+        o = refs.conv_ref(x, w, bias, s_in, act=bool(act))
+        s_out.copy_(o["state"])
+        return o["y"]
+
+    def conv_bwd(dy, ds, x, w, bias, st, act):
+        o = refs.conv_ref(x, w, bias, st, act=bool(act),
+                          dy=torch.zeros_like(x) if dy is None else dy, dstate=ds)
+        return (o["dx"], o["dw"], None if bias is None else o["dbias"],
+                None if st is None else o["dstate"])
+
+    def glu_fwd(x, wg, wu, keep):
+        g, u = x @ wg.T, x @ wu.T
+        return refs.silu(g) * u, g, u
+
+    def glu_bwd(dh, x, wg, wu, g, u, need_x, need_w):
+        o = refs.glu_ref(x, wg, wu, dh)
+        return (o["dx"] if need_x else None,) + ((o["dwg"], o["dwu"]) if need_w else (None, None))
+    for name, fn in (("_short_conv_fwd", conv_fwd), ("_short_conv_bwd", conv_bwd),
+                     ("_glu_fwd", glu_fwd), ("_glu_bwd", glu_bwd)):
+        monkeypatch.setattr(ops, name, fn)
+
+
+@pytest.mark.parametrize("act", [1, 0])
+@pytest.mark.parametrize("full", [True, False])
+@pytest.mark.parametrize("T,K", [(5, 4), (2, 4), (3, 1), (0, 3)])
+def test_conv_second_derivatives(reference_calls, act, full, T, K):
+    x, w = _rand(2, T, 3, seed=1), _rand(K, 3, seed=2)
+    bias, st = (_rand(3, seed=3), _rand(2, K - 1, 3, seed=4)) if full else (None, None)
+    leaves = [t.requires_grad_(True) for t in (x, w, bias, st) if t is not None]
+
+    def fn(*a):
+        a = iter(a)
+        return ops._ShortConvFn.apply(*(None if t is None else next(a) for t in (x, w, bias, st)),
+                                      act)
+    assert torch.autograd.gradgradcheck(fn, leaves)
+
+
+@pytest.mark.parametrize("needs", [(True, True, True), (True, False, False), (False, True, False)])
+def test_glu_second_derivatives(reference_calls, needs):
+    ts = [_rand(*s, seed=i).requires_grad_(n) for i, (s, n) in enumerate(
+        zip([(4, 3), (2, 3), (2, 3)], needs))]
+    assert torch.autograd.gradgradcheck(ops._GluFn.apply, ts)
+
+
+def test_second_derivatives_are_taken_once(reference_calls):
+    """Where one input is a function of another, its share flows through it alone."""
+    x = _rand(1, 6, 3, seed=1).requires_grad_(True)
+
+    def penalty(conv):
+        (g,) = torch.autograd.grad(conv(x, torch.tanh(x[0, :4])).square().sum(), x,
+                                   create_graph=True)
+        return torch.autograd.grad(g.square().sum(), x)[0]
+    a = penalty(lambda v, w: ops._ShortConvFn.apply(v, w, None, None, 1)[0])
+    b = penalty(lambda v, w: refs.conv_ref(v, w)["y"])
+    assert torch.allclose(a, b, rtol=1e-9, atol=1e-12)
+    # a third derivative, and a sum whose incoming gradient is a constant
+    (g,) = torch.autograd.grad(ops._ShortConvFn.apply(x, x[0, :4], None, None, 1)[0].sum(), x,
+                               create_graph=True)
+    assert g.requires_grad
+    (h,) = torch.autograd.grad(g.square().sum(), x, create_graph=True)
+    assert torch.autograd.grad(h.sum(), x)[0].shape == x.shape
+
+
+def test_batched_gradients(reference_calls):
+    x, w = _rand(2, 5, 3, seed=1).requires_grad_(True), _rand(4, 3, seed=2).requires_grad_(True)
+    y, s = ops._ShortConvFn.apply(x, w, None, None, 1)
+    d = _rand(3, *y.shape, seed=5)
+    got = torch.autograd.grad(y, (x, w), d, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        for a, b in zip(got, torch.autograd.grad(y, (x, w), d[i], retain_graph=True)):
+            assert torch.allclose(a[i], b, rtol=1e-10, atol=1e-12)
+    ts = [_rand(*q, seed=i).requires_grad_(True) for i, q in enumerate([(4, 3), (2, 3), (2, 3)])]
+    h = ops._GluFn.apply(*ts)
+    d = _rand(3, *h.shape, seed=6)
+    got = torch.autograd.grad(h, ts, d, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        for a, b in zip(got, torch.autograd.grad(h, ts, d[i], retain_graph=True)):
+            assert torch.allclose(a[i], b, rtol=1e-10, atol=1e-12)
+
+
+def test_scan_says_that_it_has_no_second_derivatives(monkeypatch):
+    """Gradients with create_graph=True are as before; differentiating them raises."""
+    names = ["x", "dt", "A", "B", "C", "D", "z", "dt_bias"]
+
+    def fwd(x, dt, A, B, C, D, z, dt_bias, softplus, h0, hT, keep):
+        o = refs.scan_ref(x, dt, A, B, C, D, z, dt_bias, h0, softplus=bool(softplus))
+        hT.copy_(o["state"])
+        return o["y"], torch.zeros(1)
+
+    def bwd(dy, dhT, *a):
+        *ts, ck, has_h0, softplus = a
+        o = refs.scan_ref(*ts, softplus=bool(softplus), dy=dy, dhT=dhT)
+        return tuple(None if t is None else o["d" + ("dt_bias" if n == "dt_bias" else n)]
+                     for n, t in zip(names, ts)) + (None,)
+    monkeypatch.setattr(ops, "_scan_fwd", fwd)
+    monkeypatch.setattr(ops, "_scan_bwd", bwd)
+    ts = [_rand(1, 5, 4, seed=1), _rand(1, 5, 4, seed=2), -_rand(4, 2, seed=3).abs(),
+          _rand(1, 5, 1, 2, seed=4), _rand(1, 5, 1, 2, seed=5), _rand(4, seed=6),
+          _rand(1, 5, 4, seed=7), _rand(4, seed=8)]
+    ts = [t.requires_grad_(True) for t in ts]
+    y, _ = ops._SelectiveScanFn.apply(*ts, None, 1)
+    dy = torch.ones_like(y)
+    plain = torch.autograd.grad(y, ts, dy, retain_graph=True)
+    kept = torch.autograd.grad(y, ts, dy, create_graph=True)
+    assert all(torch.equal(a, b) and b.requires_grad for a, b in zip(plain, kept))
+    with pytest.raises(NotImplementedError, match="second"):
+        torch.autograd.grad(kept[0].square().sum(), ts)
+    with pytest.raises(NotImplementedError, match="batched"):
+        torch.autograd.grad(y, ts, dy[None].expand(2, *y.shape), is_grads_batched=True)

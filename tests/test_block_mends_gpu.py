@@ -4,8 +4,10 @@ an fp32 one by 2^-24; an fp32 sum of n terms by n 2^-24 of the terms' magnitudes
 
 import pytest
 import torch
+import torch.nn.functional as F
 
-from gated_deltanet_jax_b200 import _lib, gated_linear_unit, selective_scan
+from gated_deltanet_jax_b200 import (GatedDeltaNetConfig, GatedDeltaNetMLP, ShortConvolution, _lib,
+                                     gated_linear_unit, selective_scan, short_convolution)
 from test_block_ops_gpu import GRAD, HALF, _f64, _names, _scan_inputs, _scan_ref, _scan_tol
 
 pytestmark = pytest.mark.gpu
@@ -166,3 +168,122 @@ def test_scan_growing_states_in_cut_rows(cuda, zero_start):
                           + [(GRAD.get(k, "d" + k), g, 2 * T, T) for k, g in zip(names, grads)]):
         assert float(mag[k].max()) < 1e38                # nothing leaves fp32's range
         _close(t, ref[k], _scan_tol(ref, mag, k, n, ch, rows, HALF["fp32"]) + 1e-36, k)
+
+
+# ---------------------------------------------------------------------------
+# second derivatives and batched gradients
+# ---------------------------------------------------------------------------
+
+def _rel(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return float((a - b).norm() / b.norm())
+
+
+def _penalty(out, x, params, dy):
+    """Gradients of |d <out, dy> / dx|^2 by x and the parameters."""
+    (g,) = torch.autograd.grad(out, x, dy, create_graph=True)
+    return (g,) + torch.autograd.grad(g.double().square().sum(), [x] + params)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bias", [True, False])
+def test_short_convolution_module_second_derivatives(cuda, dtype, bias):
+    """Sums of 12 terms of order one: fp32 to 1e-5 of them; bf16 up to four roundings of
+    2^-8 on a path (y's and dx's gradients, weights, the result)."""
+    torch.manual_seed(0)
+    conv = ShortConvolution(64, 4, use_bias=bias).to(cuda, dtype)
+    x = torch.randn(2, 75, 64, device=cuda).to(dtype).requires_grad_(True)
+    y = conv(x)
+    dy = torch.randn_like(y)
+    (plain,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    params = list(conv.parameters())
+    got = _penalty(y, x, params, dy)
+    assert torch.equal(got[0], plain)                  # the kernel's gradient, with a graph
+    r = [t.detach().double().requires_grad_(True) for t in [x] + params]
+    xp = F.pad(r[0], (0, 0, 3, 0))
+    pre = sum(r[1][j] * xp[:, j:j + 75] for j in range(4)) + (r[2] if bias else 0)
+    for a, b in zip(got, _penalty(F.silu(pre), r[0], r[1:], dy.double())):
+        assert _rel(a, b) <= (1e-5 if dtype == torch.float32 else 4 * 2.0 ** -8)
+
+
+@pytest.mark.parametrize("shape", [(5, 64), (2, 130, 64)])
+def test_mlp_module_second_derivatives(cuda, shape):
+    """bf16 throughout: ten rounded tensors on the longest path (g, u, h, dh, dg, du, dx,
+    its gradient, two products of it), 2^-8 each at most."""
+    torch.manual_seed(0)
+    mlp = GatedDeltaNetMLP(GatedDeltaNetConfig(hidden_size=64)).to(cuda, torch.bfloat16)
+    x = torch.randn(*shape, device=cuda).bfloat16().requires_grad_(True)
+    y = mlp(x)
+    dy = torch.randn_like(y)
+    (plain,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    params = list(mlp.parameters())
+    got = _penalty(y, x, params, dy)
+    assert torch.equal(got[0], plain)
+    r = [t.detach().double().requires_grad_(True) for t in [x] + params]
+    z, wg, wu, wd = r
+    ref = (F.silu(z @ wg.T) * (z @ wu.T)) @ wd.T
+    for a, b in zip(got, _penalty(ref, z, r[1:], dy.double())):
+        assert _rel(a, b) <= 10 * 2.0 ** -8
+
+
+def test_sum_of_outputs_keeps_its_graph(cuda):
+    """The incoming gradient is a constant here, and the result still has a graph."""
+    torch.manual_seed(0)
+    conv = ShortConvolution(64, 4).to(cuda)
+    mlp = GatedDeltaNetMLP(GatedDeltaNetConfig(hidden_size=64)).to(cuda, torch.bfloat16)
+    for m, x in ((conv, torch.randn(2, 9, 64, device=cuda)),
+                 (mlp, torch.randn(9, 64, device=cuda).bfloat16())):
+        x.requires_grad_(True)
+        (g,) = torch.autograd.grad(m(x).sum(), x, create_graph=True)
+        assert g.requires_grad
+        assert float(torch.autograd.grad(g.float().square().sum(), x)[0].norm()) > 0
+
+
+def test_batched_gradients(cuda):
+    torch.manual_seed(0)
+    conv = ShortConvolution(64, 4).to(cuda)
+    x = torch.randn(2, 9, 64, device=cuda, requires_grad=True)
+    y = conv(x)
+    d = torch.randn(3, *y.shape, device=cuda)
+    got = torch.autograd.grad(y, (x, conv.weight), d, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        for a, b in zip(got, torch.autograd.grad(y, (x, conv.weight), d[i], retain_graph=True)):
+            assert _rel(a[i], b) <= 1e-5
+    w = [torch.randn(96, 64, device=cuda, requires_grad=True) for _ in range(2)]
+    v = torch.randn(7, 64, device=cuda, requires_grad=True)
+    h = gated_linear_unit(v, *w)
+    d = torch.randn(3, *h.shape, device=cuda)
+    got = torch.autograd.grad(h, [v] + w, d, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        for a, b in zip(got, torch.autograd.grad(h, [v] + w, d[i], retain_graph=True)):
+            assert _rel(a[i], b) <= 1e-5
+
+
+def test_scan_second_derivatives_raise(cuda):
+    s, dy, dhT = _scan_inputs(2, 20, 40, 16, 1, True, "bf16", cuda, 1)
+    names = _names(s)
+    for k in names:
+        s[k].requires_grad_(True)
+    out = selective_scan(**s, output_final_state=True)
+    leaves = [s[k] for k in names]
+    plain = torch.autograd.grad(out, leaves, (dy, dhT), retain_graph=True)
+    kept = torch.autograd.grad(out, leaves, (dy, dhT), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, kept))
+    with pytest.raises(NotImplementedError, match="second"):
+        torch.autograd.grad(kept[0].float().sum(), leaves)
+    with pytest.raises(NotImplementedError, match="batched"):
+        torch.autograd.grad(out[0], leaves, dy[None], is_grads_batched=True)
+
+
+def test_strided_and_unaligned_inputs_keep_their_gradients(cuda):
+    """Inputs that are copied for the kernels: gradients of the originals' layout and type."""
+    torch.manual_seed(0)
+    base = torch.randn(2, 21, 131, device=cuda).bfloat16().requires_grad_(True)
+    w = torch.randn(4, 64, device=cuda).bfloat16().requires_grad_(True)
+    y, _ = short_convolution(base[..., 3:67], w)
+    dy = torch.randn_like(y)
+    gx, gw = torch.autograd.grad(y, [base, w], dy)
+    x2, w2 = (t.detach().clone().requires_grad_(True) for t in (base[..., 3:67], w.float()))
+    hx, hw = torch.autograd.grad(short_convolution(x2, w2)[0], [x2, w2], dy)
+    assert torch.equal(gx[..., 3:67], hx) and float(gx[..., 67:].abs().max()) == 0.0
+    assert torch.equal(gw, hw.bfloat16())
