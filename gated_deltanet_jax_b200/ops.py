@@ -45,6 +45,7 @@ import contextlib
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -114,6 +115,12 @@ def _prepare(q, k, v, g, beta, initial_state, final_state_out, output_final_stat
 
 
 def _wants_grad(*ts) -> bool:
+    """Whether an input asks for a gradient; raises for tangents (forward mode), which no
+    kernel carries on: the output would come without one."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the kernels have no forward-mode derivatives")
     if not torch.is_grad_enabled():
         return False
     for t in ts:
@@ -1008,6 +1015,7 @@ def gated_rms_norm(o, gate=None, weight=None, eps: float = 1e-5, *,
     ``o * rsqrt(mean(o^2, -1) + eps) * weight``, times ``silu(gate)`` when a
     gate is given.  o ``[..., dv]`` bfloat16 or float32; gate like o or None;
     weight ``[dv]`` (None: ones).  ``out`` may be o (in place)."""
+    _wants_grad(o, gate, weight)   # (inference only; tangents raise)
     if not (isinstance(o, torch.Tensor) and o.is_cuda and o.dtype in _DTYPES):
         raise ValueError("o must be a bfloat16 or float32 CUDA tensor")
     dv = o.shape[-1]

@@ -161,3 +161,23 @@ def test_scan_says_that_it_has_no_second_derivatives(monkeypatch):
         torch.autograd.grad(kept[0].square().sum(), ts)
     with pytest.raises(NotImplementedError, match="batched"):
         torch.autograd.grad(y, ts, dy[None].expand(2, *y.shape), is_grads_batched=True)
+
+
+def test_tangents_are_refused():
+    """Forward mode: a dual tensor asks for no gradient, and its tangent would be lost."""
+    fw = torch.autograd.forward_ad
+    x = torch.randn(3)
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones(3))
+        assert not ops._wants_grad(x, None, 1.0)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward"):
+                ops._wants_grad(x, None, dual)
+        assert ops._wants_grad(x, x.clone().requires_grad_(True))
+    assert not ops._wants_grad(x)
+
+    def fn(v):
+        ops._wants_grad(v)
+        return v
+    with pytest.raises(NotImplementedError, match="forward"):
+        torch.func.jvp(fn, (x,), (torch.ones(3),))

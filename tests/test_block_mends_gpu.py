@@ -7,7 +7,9 @@ import torch
 import torch.nn.functional as F
 
 from gated_deltanet_jax_b200 import (GatedDeltaNetConfig, GatedDeltaNetMLP, ShortConvolution, _lib,
-                                     gated_linear_unit, selective_scan, short_convolution)
+                                     chunk_gated_delta_rule, fused_recurrent_gated_delta_rule,
+                                     gated_linear_unit, gated_rms_norm, selective_scan,
+                                     short_convolution)
 from test_block_ops_gpu import GRAD, HALF, _f64, _names, _scan_inputs, _scan_ref, _scan_tol
 
 pytestmark = pytest.mark.gpu
@@ -287,3 +289,34 @@ def test_strided_and_unaligned_inputs_keep_their_gradients(cuda):
     hx, hw = torch.autograd.grad(short_convolution(x2, w2)[0], [x2, w2], dy)
     assert torch.equal(gx[..., 3:67], hx) and float(gx[..., 67:].abs().max()) == 0.0
     assert torch.equal(gw, hw.bfloat16())
+
+
+# ---------------------------------------------------------------------------
+# forward mode
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_raises(cuda, grad):
+    """No operator gives an output without the tangent that it should have; the modules'
+    torch routes keep theirs."""
+    fw = torch.autograd.forward_ad
+    x = torch.randn(1, 9, 64, device=cuda)
+    w, A, B = torch.randn(64, 64, device=cuda), -torch.rand(64, 16, device=cuda), x[..., :16]
+    q, b = x.view(1, 9, 1, 64), x[..., :1]
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        d = fw.make_dual(x, torch.randn_like(x))
+        calls = [lambda: gated_linear_unit(d, w, w),
+                 lambda: selective_scan(x, d, A, B, B),
+                 lambda: selective_scan(x, x, A, d[..., :16], B),
+                 lambda: short_convolution(d, w[:4]), lambda: gated_rms_norm(d),
+                 lambda: chunk_gated_delta_rule(d.view(1, 9, 1, 64), q, q, b, b),
+                 lambda: fused_recurrent_gated_delta_rule(q, q, d.view(1, 9, 1, 64), b, b)]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()
+        gated_linear_unit(x, w, w)                      # no tangent: as always
+        conv = ShortConvolution(64, 4).to(cuda)
+        if grad:
+            assert fw.unpack_dual(conv(d)).tangent is not None
+        mlp = GatedDeltaNetMLP(GatedDeltaNetConfig(hidden_size=64)).to(cuda)
+        assert fw.unpack_dual(mlp(d)).tangent is not None
