@@ -704,8 +704,9 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
     ``final_state_out`` (which may be ``conv_state``, updated in place) is
     given, else None.  The reference's call is ``short_convolution(x, w)`` (no
     state).  Differentiable in x, weight, bias and conv_state, through y and
-    the returned state (without ``final_state_out``; gdn_short_conv_bwd), twice too
-    (second derivatives run on torch's operations).
+    the returned state (gdn_short_conv_bwd; with ``final_state_out`` in weight and bias
+    alone, of which the state is no function), twice too (second derivatives run on
+    torch's operations).
     """
     _cuda_input("x", x)
     if x.dim() != 3:
@@ -729,9 +730,16 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
             raise ValueError(f"bias must be [{C}]; got {tuple(bias.shape)}")
     if _wants_grad(x, w, bias, conv_state):
         if final_state_out is not None:
-            raise NotImplementedError("the backward does not cover final_state_out")
-        y, s_out = _ShortConvFn.apply(_aligned(x), _aligned32(w), _aligned32(bias), s_in, act)
-        return y, s_out if output_final_state else None
+            if _wants_grad(x, conv_state):
+                raise NotImplementedError("the backward does not cover final_state_out of an x or "
+                                          "conv_state that requires grad")
+            # the backward reads the window as it entered, which the call may overwrite
+            s_in = None if s_in is None else s_in.clone()
+        y, state = _ShortConvFn.apply(_aligned(x), _aligned32(w), _aligned32(bias), s_in, act)
+        if final_state_out is not None:
+            with torch.no_grad():
+                return y, s_out.copy_(state)
+        return y, state if output_final_state else None
     if s_out is None and output_final_state:
         s_out = torch.empty(shape, dtype=x.dtype, device=dev)
     y = _short_conv_fwd(_aligned(x), _aligned32(w), _aligned32(bias), s_in, s_out, act)

@@ -320,3 +320,38 @@ def test_forward_mode_raises(cuda, grad):
             assert fw.unpack_dual(conv(d)).tangent is not None
         mlp = GatedDeltaNetMLP(GatedDeltaNetConfig(hidden_size=64)).to(cuda)
         assert fw.unpack_dual(mlp(d)).tangent is not None
+
+
+# ---------------------------------------------------------------------------
+# short convolution: decoding over a module's parameters
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T", [1, 2, 40])
+def test_conv_decodes_in_place_over_parameters(cuda, T):
+    """Weights that require grad, outside no_grad, with the window updated in place: the
+    values of a call without gradients, and the weights' gradients of one out of place."""
+    gen = _gen(cuda, T)
+    rn = lambda *s: torch.randn(*s, device=cuda, generator=gen)   # noqa: E731
+    w, bias = torch.nn.Parameter(rn(4, 64)), torch.nn.Parameter(rn(64))
+    x = [rn(2, T, 64).bfloat16() for _ in range(3)]
+    dy = rn(2, T, 64).bfloat16()
+    start = rn(2, 3, 64).bfloat16()
+    S, P, state = start.clone(), start.clone(), start
+    ys, zs = [], []
+    for v in x:
+        y, out = short_convolution(v, w, bias=bias, conv_state=S, final_state_out=S)
+        assert out is S and not S.requires_grad
+        with torch.no_grad():
+            plain, _ = short_convolution(v, w, bias=bias, conv_state=P, final_state_out=P)
+        z, state = short_convolution(v, w, bias=bias, conv_state=state, output_final_state=True)
+        state = state.detach()
+        assert torch.equal(y, plain) and torch.equal(S, P) and torch.equal(S, state)
+        ys.append(y)
+        zs.append(z)
+    for y, z in zip(ys, zs):                           # (the windows have moved on since)
+        for a, b in zip(torch.autograd.grad(y, [w, bias], dy), torch.autograd.grad(z, [w, bias], dy)):
+            assert torch.equal(a, b)
+    for bad in (dict(x=x[0].clone().requires_grad_(True)),
+                dict(x=x[0], conv_state=start.clone().requires_grad_(True))):
+        with pytest.raises(NotImplementedError, match="final_state_out"):
+            short_convolution(bad.pop("x"), w, bias=bias, final_state_out=S, **bad)
