@@ -159,8 +159,9 @@ int check_short_conv(const float* weight, const float* bias, const void* state_i
   if (!gdn::short_conv_supported(C, K, dtype))
     return fail(GDN_ERR_UNSUPPORTED, "C=%d channels must be a multiple of %d for this dtype", C,
                 dtype == GDN_DTYPE_BF16 ? 8 : 4);
-  if (T > (1 << 30) || (long long)B * ((long long)T + K) * C > (1LL << 40))
-    return fail(GDN_ERR_INVALID, "tensor too large (T > 2^30 or B*T*C > 2^40)");
+  // (the kernels' token indexes run up to two dozen past T)
+  if (T > 0x7fffffff - 63 || (long long)B * ((long long)T + K) * C > (1LL << 40))
+    return fail(GDN_ERR_INVALID, "tensor too large (T > 2^31 - 64 or B*T*C > 2^40)");
   if (!weight || !aligned16(weight))
     return fail(GDN_ERR_INVALID, "weight must be non-NULL and 16-byte aligned");
   if (!aligned16(bias)) return fail(GDN_ERR_INVALID, "bias must be 16-byte aligned");
@@ -785,6 +786,8 @@ int gdn_short_conv_fwd_bias(const void* x, const float* weight, const float* bia
   if (rc || B == 0 || C == 0) return rc;
   if (T > 0 && (!x || !y || !aligned16(x) || !aligned16(y)))
     return fail(GDN_ERR_INVALID, "x and y must be non-NULL and 16-byte aligned");
+  if (T > (1 << 30) && state_in && state_in == state_out)
+    return fail(GDN_ERR_INVALID, "a state in place takes T up to 2^30 (one walk over all tokens)");
   if (T == 0) {
     // nothing to convolve; the state still carries through
     if (!state_out || state_out == state_in || K == 1) return GDN_OK;

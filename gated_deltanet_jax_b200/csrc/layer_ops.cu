@@ -130,7 +130,7 @@ short_conv_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
   if (c >= C) return;
   const int b = blockIdx.y;
   const int t0 = blockIdx.z * TT;
-  const int t1 = min(T, t0 + TT);
+  const int t1 = T - t0 > TT ? t0 + TT : T;
   float2 wk[K][N / 2], bs[N / 2];
 #pragma unroll
   for (int j = 0; j < K; ++j) {
@@ -262,7 +262,7 @@ template <typename Tin>
 cudaError_t conv_dispatch(const void* x, const float* w, const float* bias, const void* si,
                           void* so, void* y, int B, int T, int C, int K, int TT, int act, cudaStream_t st) {
   constexpr int N = Vec4<Tin>::N;
-  const dim3 grid((C / N + kConvThreads - 1) / kConvThreads, B, (T + TT - 1) / TT);
+  const dim3 grid((C / N + kConvThreads - 1) / kConvThreads, B, (T - 1) / TT + 1);
   const Tin* xi = static_cast<const Tin*>(x);
   const Tin* s_in = static_cast<const Tin*>(si);
   Tin* sout = static_cast<Tin*>(so);
@@ -304,9 +304,9 @@ cudaError_t launch_short_conv(const void* x, const float* w, const float* bias,
   // by the first tile and written by the last, so it takes one tile over all T.
   int TT = 64;
   const long long per = (long long)((C / 4 + kConvThreads - 1) / kConvThreads) * B;
-  while (TT > 16 && per * ((T + TT - 1) / TT) < 8LL * device_sm_count()) TT /= 2;
+  while (TT > 16 && per * ((T - 1) / TT + 1) < 8LL * device_sm_count()) TT /= 2;
   if (state_in && state_in == state_out) TT = T;
-  if ((T + TT - 1) / TT > 65535) TT = (T + 65534) / 65535;
+  if ((T - 1) / TT + 1 > 65535) TT = (T - 1) / 65535 + 1;
   return dtype == kBF16
              ? conv_dispatch<__nv_bfloat16>(x, w, bias, state_in, state_out, y, B, T, C, K, TT, act,
                                             st)

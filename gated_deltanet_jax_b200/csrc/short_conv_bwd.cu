@@ -88,7 +88,7 @@ short_conv_bwd_kernel(const Tin* __restrict__ x, const float* __restrict__ w,
   if (c >= C) return;
   const int b = blockIdx.z;
   const int t0 = blockIdx.y * TT;
-  const int t1 = min(T, t0 + TT);
+  const int t1 = T - t0 > TT ? t0 + TT : T;
   constexpr int W = K > 1 ? K - 1 : 1;
   const float2 zero = make_float2(0.f, 0.f), one = make_float2(1.f, 1.f);
   float2 wk[K], win[W], dwin[W], dw[K], db = zero, bs = zero;
@@ -254,13 +254,13 @@ int conv_bwd_tile(int B, int T, int C, int K, int dtype) {
 size_t short_conv_bwd_workspace_bytes(int B, int T, int C, int K, int dtype) {
   if (B <= 0 || T <= 0 || C <= 0) return 0;
   const int TT = conv_bwd_tile(B, T, C, K, dtype);
-  return (size_t)B * ((T + TT - 1) / TT) * (K + 1) * C * sizeof(float);
+  return (size_t)B * ((T - 1) / TT + 1) * (K + 1) * C * sizeof(float);
 }
 
 cudaError_t launch_short_conv_bwd(const ShortConvBwdArgs& a, cudaStream_t st) {
   if (!short_conv_supported(a.C, a.K, a.dtype) || a.B > 65535) return cudaErrorInvalidValue;
   const int TT = conv_bwd_tile(a.B, a.T, a.C, a.K, a.dtype);
-  const int tiles = (a.T + TT - 1) / TT;
+  const int tiles = (a.T - 1) / TT + 1;
   cudaError_t e = a.dtype == kBF16 ? bwd_dispatch<__nv_bfloat16>(a, TT, tiles, st)
                                    : bwd_dispatch<float>(a, TT, tiles, st);
   if (e != cudaSuccess) return e;

@@ -111,6 +111,7 @@ class ShortConvolution(nn.Module):
             return y
         K, C = self.weight.shape
         if (grad and K <= 8 and C % (8 if x.dtype == torch.bfloat16 else 4) == 0
+                and x.dim() == 3 and x.shape[0] <= 65535 and x.shape[1] <= 0x7fffffff - 63
                 and _kernel_call_ok(x, self.weight)):
             y, _ = ops.short_convolution(x, self.weight, bias=self.bias,
                                          activation="silu" if act else None)

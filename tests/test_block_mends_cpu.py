@@ -181,3 +181,18 @@ def test_tangents_are_refused():
         return v
     with pytest.raises(NotImplementedError, match="forward"):
         torch.func.jvp(fn, (x,), (torch.ones(3),))
+
+
+def test_conv_lengths(lib):
+    """T up to 2^31 - 64, and 2^30 where the state is updated in place."""
+    def fwd(T, si=None, so=None, dtype=BF16):
+        return lib.gdn_short_conv_fwd_bias(_at(1), _at(2), None, si, so, None, 1, T, 8, 4, 1, dtype,
+                                           None)
+    assert fwd((1 << 31) - 63) == INVALID and b"too large" in lib.gdn_last_error()
+    assert fwd((1 << 31) - 64) == INVALID and b"non-NULL" in lib.gdn_last_error()    # y is
+    assert lib.gdn_short_conv_fwd_bias(_at(1), _at(2), None, _at(3), _at(3), _at(4), 1,
+                                       (1 << 30) + 1, 8, 4, 1, BF16, None) == INVALID
+    assert b"in place" in lib.gdn_last_error()
+    # the backward's partial rows: a tile for each of 65535 blocks at most
+    rows = lib.gdn_short_conv_bwd_workspace_bytes(1, (1 << 31) - 64, 8, 4) // (5 * 8 * 4)
+    assert 1000 < rows <= 65535

@@ -355,3 +355,47 @@ def test_conv_decodes_in_place_over_parameters(cuda, T):
                 dict(x=x[0], conv_state=start.clone().requires_grad_(True))):
         with pytest.raises(NotImplementedError, match="final_state_out"):
             short_convolution(bad.pop("x"), w, bias=bias, final_state_out=S, **bad)
+
+
+# ---------------------------------------------------------------------------
+# short convolution: many rows, long rows
+# ---------------------------------------------------------------------------
+
+def test_short_convolution_module_trains_on_many_rows(cuda):
+    """More rows than the kernels' grid takes keep torch's convolution."""
+    torch.manual_seed(0)
+    conv = ShortConvolution(8, 4).to(cuda)
+    x = torch.randn(65537, 3, 8, device=cuda, requires_grad=True)
+    y = conv(x)
+    y.sum().backward()
+    few = x.detach()[-2:].clone().requires_grad_(True)
+    z = conv(few)
+    (g,) = torch.autograd.grad(z.sum(), few)
+    assert torch.allclose(y[-2:], z, atol=1e-5) and torch.allclose(x.grad[-2:], g, atol=1e-5)
+
+
+def _room(gb):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gb << 30:
+        pytest.skip(f"needs {gb} GB of device memory")
+
+
+@pytest.mark.parametrize("T,grad,gb", [((1 << 30) + 77, True, 90), ((1 << 31) - 64, False, 90)])
+def test_conv_rows_past_2_30_tokens(cuda, T, grad, gb):
+    """The last tokens of a row as long as the kernels take, against those on their own."""
+    _room(gb)
+    tail = 100
+    x = torch.randn(1, T, 8, device=cuda, dtype=torch.bfloat16).requires_grad_(grad)
+    w = torch.randn(4, 8, device=cuda) * 0.5
+    y, s = short_convolution(x, w, output_final_state=True)
+    cut = x.detach()[:, -tail:].clone().requires_grad_(grad)
+    yt, st = short_convolution(cut, w, conv_state=x.detach()[:, -tail - 3:-tail].clone(),
+                               output_final_state=True)
+    assert torch.equal(y[:, -tail:], yt) and torch.equal(s, st)
+    if grad:
+        dy = torch.randn_like(y)
+        (dx,) = torch.autograd.grad(y, x, dy)
+        (dt,) = torch.autograd.grad(yt, cut, dy[:, -tail:].clone())
+        assert torch.equal(dx[:, -tail:], dt)
+    del x, y
+    torch.cuda.empty_cache()
