@@ -45,6 +45,7 @@ from torch import nn
 from torch.autograd import forward_ad
 from torch.nn.modules import module
 import torch.nn.functional as F
+from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import dispatch, ops
 from .configuration import GatedDeltaNetConfig
@@ -66,14 +67,21 @@ def _linear(d_in: int, d_out: int) -> nn.Linear:
     return lin
 
 
+def _eager() -> bool:
+    """Outside torch's tracing (compiled or torch.jit.trace, which would record the
+    questions below too) and dispatch modes (which count, record or replace operations)."""
+    return (torch._C._get_tracing_state() is None and not torch.compiler.is_compiling()
+            and not is_in_torch_dispatch_mode())
+
+
 def _kernel_call_ok(*ts) -> bool:
     """Whether the kernels may stand in for torch operations on these tensors: plain
-    CUDA tensors of one dtype that the kernels take, outside torch's tracing,
-    function transforms, forward-mode differentiation and autocast."""
+    CUDA tensors of one dtype that the kernels take, outside torch's function
+    transforms, forward-mode differentiation and autocast (asked after _eager)."""
     x = ts[0]
     return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32)
             and all(type(t) in (torch.Tensor, nn.Parameter) and t.device == x.device for t in ts)
-            and not torch.compiler.is_compiling() and not torch.is_autocast_enabled("cuda")
+            and not torch.is_autocast_enabled("cuda")
             and not torch._C._are_functorch_transforms_active()
             and forward_ad._current_level < 0)
 
@@ -105,12 +113,12 @@ class ShortConvolution(nn.Module):
         act = self.activation in ("silu", "swish")
         grad = torch.is_grad_enabled() and (
             x.requires_grad or any(p.requires_grad for p in self.parameters()))
-        if not grad and self.bias is None:
+        if not grad and self.bias is None and torch._C._get_tracing_state() is None:
             y, _ = ops.short_convolution(x.contiguous(), self.weight.detach().float(),
                                          activation="silu" if act else None)
             return y
         K, C = self.weight.shape
-        if (grad and K <= 8 and C % (8 if x.dtype == torch.bfloat16 else 4) == 0
+        if (grad and _eager() and K <= 8 and C % (8 if x.dtype == torch.bfloat16 else 4) == 0
                 and x.dim() == 3 and x.shape[0] <= 65535 and x.shape[1] <= 0x7fffffff - 63
                 and _kernel_call_ok(x, self.weight)):
             y, _ = ops.short_convolution(x, self.weight, bias=self.bias,
@@ -255,7 +263,7 @@ class GatedDeltaNetMLP(nn.Module):
         gate, up = self.gate_proj, self.up_proj
         grad = torch.is_grad_enabled() and (
             x.requires_grad or any(p.requires_grad for p in self.parameters()))
-        if ((grad or self.fused_inference) and x.dtype == torch.bfloat16
+        if ((grad or self.fused_inference) and _eager() and x.dtype == torch.bfloat16
                 and _plain_linear(gate, x.dtype) and _plain_linear(up, x.dtype)
                 and gate.weight.shape == up.weight.shape
                 and x.shape[-1] % 8 == 0 and gate.out_features % 8 == 0

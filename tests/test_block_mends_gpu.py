@@ -399,3 +399,26 @@ def test_conv_rows_past_2_30_tokens(cuda, T, grad, gb):
         assert torch.equal(dx[:, -tail:], dt)
     del x, y
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------
+# the modules under torch's tracing and dispatch modes
+# ---------------------------------------------------------------------------
+
+def test_modules_trace_to_torch_operations(cuda):
+    """A traced module is a graph of torch's operations that another input, and another
+    program, can run."""
+    from torch.utils.flop_counter import FlopCounterMode
+    torch.manual_seed(0)
+    mlp = GatedDeltaNetMLP(GatedDeltaNetConfig(hidden_size=64)).to(cuda, torch.bfloat16)
+    conv = ShortConvolution(64, 4).to(cuda)
+    for m, x, shape in ((mlp, torch.randn(5, 64, device=cuda).bfloat16(), (9, 64)),
+                        (conv, torch.randn(2, 9, 64, device=cuda), (2, 9, 64))):
+        traced = torch.jit.trace(m, x)
+        assert "PythonOp" not in str(traced.inlined_graph)
+        v = torch.randn(*shape, device=cuda).to(x.dtype)
+        with torch.no_grad():
+            assert torch.allclose(traced(v).float(), m(v).float(), rtol=3e-2, atol=3e-2)
+        with FlopCounterMode(display=False) as counted:
+            m(x)
+        assert counted.get_total_flops() > 0
