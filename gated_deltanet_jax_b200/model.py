@@ -267,6 +267,7 @@ class GatedDeltaNetMLP(nn.Module):
                 and _plain_linear(gate, x.dtype) and _plain_linear(up, x.dtype)
                 and gate.weight.shape == up.weight.shape
                 and x.shape[-1] % 8 == 0 and gate.out_features % 8 == 0
+                and x.shape[-1] <= 131072 and x.shape[:-1].numel() <= 1 << 30
                 and _kernel_call_ok(x, gate.weight, up.weight)):
             return self.down_proj(ops.gated_linear_unit(x, gate.weight, up.weight))
         return self.down_proj(F.silu(gate(x)) * up(x))

@@ -540,6 +540,12 @@ def _cuda_input(name, t):
         raise TypeError(f"{name} must be bfloat16 or float32; got {t.dtype}")
 
 
+def _check_sizes(name, sizes):
+    """The library's sizes are 32-bit; a larger one would arrive as its low half."""
+    if sizes and max(sizes) > 0x7fffffff:
+        raise ValueError(f"{name} is too large: {tuple(sizes)} has a size past 2^31 - 1")
+
+
 def _conv_state(t, name, shape, dtype, dev):
     if t is None:
         return None
@@ -711,6 +717,7 @@ def short_convolution(x, weight, *, bias=None, activation: Optional[str] = "silu
     _cuda_input("x", x)
     if x.dim() != 3:
         raise ValueError(f"x must be [B,T,C]; got {tuple(x.shape)}")
+    _check_sizes("x", x.shape)
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be 'silu', 'swish' or None; got {activation!r}")
@@ -846,6 +853,8 @@ def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") ->
         raise ValueError(f"gate_weight and up_weight must both be [I,{D}]; got "
                          f"{tuple(gate_weight.shape)}, {tuple(up_weight.shape)}")
     x2 = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), D)
+    _check_sizes("x", x2.shape)
+    _check_sizes("gate_weight", gate_weight.shape)
     if _wants_grad(x, gate_weight, up_weight):
         h = _GluFn.apply(_aligned(x2), _aligned(gate_weight), _aligned(up_weight))
     else:
@@ -966,6 +975,7 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
     _check_input("C", C, dev, dtype)
     if z is not None:
         _check_input("z", z, dev, dtype)
+    _check_sizes("x", shape_x)
     b, T, ch = shape_x
     if dt.shape != shape_x or (z is not None and z.shape != shape_x):
         raise ValueError(f"dt and z must have x's shape {tuple(shape_x)}")
@@ -981,6 +991,7 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
     if B.shape != (b, T, G, N) or C.shape != B.shape:
         raise ValueError(f"B and C must be [{b},{T},{N}] or [{b},{T},G,{N}]; got "
                          f"{tuple(B.shape)}, {tuple(C.shape)}")
+    _check_sizes("B", B.shape)
     if G < 1 or ch % G:
         raise ValueError(f"x's {ch} channels must be a multiple of the {G} groups of B and C")
     if D is not None:

@@ -196,3 +196,10 @@ def test_conv_lengths(lib):
     # the backward's partial rows: a tile for each of 65535 blocks at most
     rows = lib.gdn_short_conv_bwd_workspace_bytes(1, (1 << 31) - 64, 8, 4) // (5 * 8 * 4)
     assert 1000 < rows <= 65535
+
+
+def test_sizes_past_32_bits_are_refused():
+    ops._check_sizes("x", (3, (1 << 31) - 1))
+    ops._check_sizes("x", ())
+    with pytest.raises(ValueError, match="x is too large"):
+        ops._check_sizes("x", (0, 1 << 31))

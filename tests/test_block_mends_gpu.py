@@ -422,3 +422,29 @@ def test_modules_trace_to_torch_operations(cuda):
         with FlopCounterMode(display=False) as counted:
             m(x)
         assert counted.get_total_flops() > 0
+
+
+# ---------------------------------------------------------------------------
+# sizes past 32 bits
+# ---------------------------------------------------------------------------
+
+def test_sizes_past_32_bits_are_refused(cuda):
+    """They once arrived as their low halves, and outputs came back unwritten."""
+    _room(80)
+    big = (1 << 32) + 5
+    w = torch.ones(8, 8, device=cuda, dtype=torch.bfloat16)
+    x = torch.empty(big, 8, device=cuda, dtype=torch.bfloat16)
+    for call in (lambda: gated_linear_unit(x, w, w),
+                 lambda: gated_linear_unit(x.view(1, big, 8), w, w),
+                 lambda: gated_linear_unit(x[:2], x, x),
+                 lambda: short_convolution(x[None], w[:4]),
+                 lambda: short_convolution(x[:, None], w[:4]),
+                 lambda: short_convolution(x[:, None, :0], w[:4, :0])):
+        with pytest.raises(ValueError, match="too large"):
+            call()
+    A = torch.ones(1, 1, device=cuda)
+    v = x.view(-1)[:big].view(1, big, 1)
+    with pytest.raises(ValueError, match="too large"):
+        selective_scan(v, v, A, v, v)
+    del x, v
+    torch.cuda.empty_cache()
