@@ -922,6 +922,9 @@ int gdn_selective_scan_fwd(const void* x, const void* dt, const float* A, const 
   if (rc || B == 0 || C == 0) return rc;
   if ((T > 0 && !y) || !aligned16(y) || !aligned16(hT) || !aligned16(checkpoints))
     return fail(GDN_ERR_INVALID, "y must be non-NULL; y, hT and checkpoints 16-byte aligned");
+  const uintptr_t in = reinterpret_cast<uintptr_t>(h0), out = reinterpret_cast<uintptr_t>(hT);
+  if (h0 && hT && h0 != hT && (in > out ? in - out : out - in) < sizeof(float) * (size_t)B * C * N)
+    return fail(GDN_ERR_INVALID, "hT is h0 or apart from it: other blocks read what it overlaps");
   if (T == 0) {
     if (!hT || hT == h0) return GDN_OK;
     return carry(hT, h0, sizeof(float) * (size_t)B * C * N, stream,

@@ -960,7 +960,8 @@ def selective_scan(x, dt, A, B, C, *, D=None, z=None, dt_bias=None, dt_softplus:
     to float32; None: zero; z None: no gate); N up to 64.  Returns ``(y,
     state)`` like the recurrent op: state float32 ``[B,Ch,N]`` when
     ``output_final_state`` or ``final_state_out`` is given (decode:
-    ``initial_state=S, final_state_out=S`` updates S in place), else None.
+    ``initial_state=S, final_state_out=S`` updates S in place; else they do not
+    overlap), else None.
     Differentiable in every tensor, through y and the returned state (without
     ``final_state_out``; gdn_selective_scan_bwd), once: second derivatives raise
     NotImplementedError.  Its layer feeds x through

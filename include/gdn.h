@@ -446,7 +446,8 @@ int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void*
  * x, dt, z, y [B, T, C] and Bm, Cm [B, T, G, N] in `dtype` (z NULL: no gate);
  * channel c uses group c / (C / G).  A [C, N], D, dt_bias [C] fp32 (D, dt_bias
  * NULL: zero).  h0, hT [B, C, N] fp32: NULL h0 starts from zeros, NULL hT drops
- * the final state, h0 == hT updates in place (decode: T = 1).  N <= 64.
+ * the final state, h0 == hT updates in place (decode: T = 1); otherwise they do
+ * not overlap.  N <= 64.
  * `checkpoints` (NULL: not wanted; gdn_selective_scan_checkpoint_bytes())
  * receives the states that gdn_selective_scan_bwd restarts from.  `workspace`:
  * gdn_selective_scan_workspace_bytes() bytes (0 where the rows are not cut:

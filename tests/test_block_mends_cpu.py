@@ -203,3 +203,18 @@ def test_sizes_past_32_bits_are_refused():
     ops._check_sizes("x", ())
     with pytest.raises(ValueError, match="x is too large"):
         ops._check_sizes("x", (0, 1 << 31))
+
+
+def test_scan_states_overlap_wholly_or_not_at_all(lib):
+    b, T, ch, N = 2, 5000, 8, 16
+    n = b * ch * N * 4
+
+    def fwd(h0, hT):
+        return lib.gdn_selective_scan_fwd(_at(1), _at(2), _at(3), _at(4), _at(5), None, None, None,
+                                          ctypes.c_void_p(h0), _at(6), ctypes.c_void_p(hT), None,
+                                          b, T, ch, N, 1, 1, BF16, None, 0, None)
+    at = 64 << 20
+    for off in (16, n - 16, -16, 16 - n):
+        assert fwd(at, at + off) == INVALID and b"apart" in lib.gdn_last_error(), off
+    for off in (0, n, -n):                # refused for the workspace that is missing
+        assert fwd(at, at + off) == INVALID and b"workspace" in lib.gdn_last_error(), off
