@@ -33,6 +33,7 @@
 
 #include "gdn_common.cuh"
 #include "gdn_internal.h"
+#include "glu_few_plan.h"
 #include "ptx.cuh"
 
 namespace gdn {
@@ -349,12 +350,7 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
 // then sums the S partial accumulators of its share of the tokens, sent through
 // distributed shared memory in a fixed order, and writes their silu(g) u.
 constexpr int kFewThreads = 192;
-constexpr int kFewRows = 64;                         // output columns of a cluster
-constexpr int kFewTokens = 128;                      // the most this form takes
-constexpr int kFewA = 2 * kFewRows * 128;            // bytes of a stage's weights
-constexpr int kFewMaxStages = 11;
-constexpr int kFewMaxSplit = 8;
-constexpr int kFewMaxShare = 2;                      // CTAs of an SM
+static_assert(kFewBK == kBK, "the operands' boxes are shared");
 
 struct FewShape {
   int M, I, kblocks, n, stages, cols, split;   // n: tokens rounded up to 16
@@ -573,30 +569,9 @@ int tc_dw_parts(int M, int* steps) {
 
 cudaError_t launch_few(const GluArgs& a, cudaStream_t st) {
   FewMaps m;
-  FewShape sh;
-  sh.M = a.M;
-  sh.I = a.I;
-  const int tiles = ceil_div(a.I, kFewRows), sms = device_sm_count();
-  sh.kblocks = ceil_div(a.D, kBK);
-  sh.n = ceil_div(a.M, 16) * 16;
-  sh.cols = sh.n <= 32 ? 32 : sh.n <= 64 ? 64 : 128;
-  // The split whose busiest SM has the least work (tiles / S each), the smallest
-  // such, with at most two CTAs sharing an SM and four steps left to each (the
-  // exchange costs 1 to 2 us).
-  sh.split = 1;
-  double best = ceil_div(tiles, sms);
-  for (int S = 2; S <= kFewMaxSplit && 4 * S <= sh.kblocks; ++S) {
-    const int c = ceil_div(tiles * S, sms);
-    if (c <= kFewMaxShare && (double)c / S < 0.95 * best) {
-      best = (double)c / S;
-      sh.split = S;
-    }
-  }
-  const int smem = (ceil_div(tiles * sh.split, sms) == 1 ? 226 : 112) * 1024;   // and 1 KB static
-  sh.share = ceil_div(ceil_div(a.M, sh.split), 4) * 4;
-  sh.stages = (smem - 1024) / (kFewA + sh.n * 128);
-  if (sh.stages > kFewMaxStages) sh.stages = kFewMaxStages;
-  if (sh.split * sh.share * 512 > smem - 1024) return cudaErrorInvalidValue;
+  const FewPlan p = few_plan(a.M, a.D, a.I, device_sm_count());
+  if (!p.fits()) return cudaErrorInvalidValue;
+  const FewShape sh{a.M, a.I, p.kblocks, p.n, p.stages, p.cols, p.split, p.share};
   // (a box of n rows past the M there are is filled with zeros)
   if (!make_map(&m.x, a.x, a.M, a.D, sh.n) || !make_map(&m.wg, a.wg, a.I, a.D, kFewRows) ||
       !make_map(&m.wu, a.wu, a.I, a.D, kFewRows))
@@ -605,9 +580,9 @@ cudaError_t launch_few(const GluArgs& a, cudaStream_t st) {
   const cudaError_t e = ensure_smem(glu_few_kernel, 226 * 1024, slot);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * sh.split);
+  cfg.gridDim = dim3(p.tiles * p.split);
   cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = p.smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -218,3 +218,43 @@ def test_scan_states_overlap_wholly_or_not_at_all(lib):
         assert fwd(at, at + off) == INVALID and b"apart" in lib.gdn_last_error(), off
     for off in (0, n, -n):                # refused for the workspace that is missing
         assert fwd(at, at + off) == INVALID and b"workspace" in lib.gdn_last_error(), off
+
+
+PLAN_CHECK = r"""
+#include <cstdio>
+#include "glu_few_plan.h"
+int main() {
+  long long bad = 0, seen = 0;
+  const int sms[] = {148, 132, 1};
+  const int widths[] = {8, 64, 72, 256, 264, 1000, 2048, 4096, 5632, 11008, 28672, 131072, 1 << 20,
+                        1 << 30};
+  for (int s : sms)
+    for (int M = 1; M <= gdn::kFewTokens; ++M)
+      for (int D : widths)
+        for (int I : widths) {
+          if (D > 131072) continue;
+          const gdn::FewPlan p = gdn::few_plan(M, D, I, s);
+          bool ok = p.fits() && p.stages <= gdn::kFewMaxStages;
+          ok = ok && p.n >= M && p.n <= 128 && p.cols >= p.n && p.split * p.share >= M;
+          ok = ok && p.split <= gdn::kFewMaxSplit && p.kblocks >= p.split && p.share % 4 == 0;
+          // static shared memory below 1 KB, 1 KB kept by the system, 228 KB an SM
+          ok = ok && (p.smem + 2048) * (p.smem > 113 * 1024 ? 1 : 2) <= 228 * 1024;
+          ok = ok && p.stage_bytes() % 1024 == 0 && (long long)p.tiles * 64 >= I;
+          ++seen;
+          if (!ok && ++bad < 5) std::printf("M=%d D=%d I=%d sms=%d\n", M, D, I, s);
+        }
+  std::printf("%lld of %lld\n", bad, seen);
+  return bad != 0;
+}
+"""
+
+
+def test_glu_few_token_layout_stays_in_its_memory(tmp_path):
+    """Stages, exchange and TMEM columns of the kernel for few tokens, over its sizes."""
+    import subprocess
+    src, exe = tmp_path / "plan.cpp", tmp_path / "plan"
+    src.write_text(PLAN_CHECK)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", _build.CSRC, str(src), "-o", str(exe)],
+                   check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.startswith("0 of 64512"), r.stdout
