@@ -238,13 +238,14 @@ long long simt_tiles(int mode, int tile, int M, int N) {
 // on 128 x 128).  In parts: dx of 64 tokens of 296 x 11000 47 us, in one 0.95 ms.
 SimtPlan simt_plan(int mode, int M, int N, int K, bool parts_ok) {
   static const double kStep[3] = {35., 58., 94.}, kLone[3] = {8., 15., 18.};
+  const int sms = device_sm_count();
   const double depth = (mode == kDx ? 2. : 1.) * K / 1024.;
   SimtPlan best{0, 1, 1e300};
   for (int parts = 1; parts <= (parts_ok ? 64 : 1); parts *= 2) {
     if (parts > 1 && depth * 1024. / parts < 128.) break;
     for (int tile = 0; tile < 3; ++tile) {
       const long long n = simt_tiles(mode, tile, M, N) * parts;
-      const long long per_sm = (n + 147) / 148;
+      const long long per_sm = (n + sms - 1) / sms;
       double t = (kStep[tile] * per_sm + (per_sm == 1 ? kLone[tile] : 0.)) * depth / parts;
       if (parts > 1) t += 4. + (mode == kDw ? 2. : 1.) * M * N * parts * 8. / 3e6;
       if (t < best.us * 0.98) best = SimtPlan{tile, parts, t};

@@ -551,11 +551,11 @@ cudaError_t sum_parts(const float* part, int parts, long long n, long long strid
 // half the pairs of SMs (a tile walks 2 I / 64 steps alone) up to 16 of 8 steps or more.  The
 // whole backward of 2048 x 5632: 16 tokens 74 -> 40 us, 256 81 -> 46, 1000 105 -> 88.
 int tc_dx_parts(int M, int D, int I, int* steps) {
-  const int ksteps = 2 * ceil_div(I, kBK), pairs = 74;
+  const int ksteps = 2 * ceil_div(I, kBK), pairs = device_sm_count() / 2;
   const long long tiles = (long long)ceil_div(M, kTile) * ceil_div(D, kTile);
   int parts = ceil_div(ksteps, kMaxSteps);
   if (tiles > 0 && 2 * tiles <= pairs)
-    parts = std::max(parts, (int)std::min(std::min(pairs / tiles, 16LL), ksteps / 8LL));
+    parts = std::max(parts, (int)std::min({pairs / tiles, 16LL, ksteps / 8LL}));
   *steps = parts > 1 ? ceil_div(ksteps, parts) : ksteps;
   return parts > 1 ? ceil_div(ksteps, *steps) : 1;
 }

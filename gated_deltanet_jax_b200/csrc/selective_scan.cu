@@ -460,7 +460,7 @@ ScanSplit scan_split(int B, int T, int C, int G, bool backward) {
   const long long blocks = (long long)((C / G + kScanCh - 1) / kScanCh) * G * B;
   ScanSplit s{1, T};
   if (T <= 0 || blocks <= 0 || blocks > (backward ? 512 : 384)) return s;
-  const long long want = (148LL * (backward ? 16 : 14) + blocks - 1) / blocks;
+  const long long want = ((long long)device_sm_count() * (backward ? 16 : 14) + blocks - 1) / blocks;
   long long tokens = (T + want - 1) / want;
   if (tokens < 128) tokens = 128;   // a chunk's launch and chaining against its walk
   tokens = (tokens + 31) / 32 * 32;

@@ -237,7 +237,7 @@ cudaError_t bwd_dispatch(const ShortConvBwdArgs& a, int TT, int tiles, cudaStrea
 // 8 x 2048 x 4096: 256 tokens, one wave, 101 us; 208 tokens 105, 352 tokens 118.
 int conv_bwd_tile(int B, int T, int C, int K, int dtype) {
   const long long per = (long long)((C / kVec + kThreads - 1) / kThreads) * B;
-  const long long slots = 148LL * bwd_blocks(K, dtype == kBF16 ? 2 : 4);
+  const long long slots = (long long)device_sm_count() * bwd_blocks(K, dtype == kBF16 ? 2 : 4);
   long long tt = T;
   for (int n = 1; per > 0 && n <= 8; ++n) {
     const long long tiles = n * slots / per;
