@@ -52,7 +52,9 @@ EXPORTED_SYMBOLS = (
     "gdn_short_conv_bwd",
     "gdn_short_conv_bwd_workspace_bytes",
     "gdn_glu_fwd",
+    "gdn_glu_fwd_kept",
     "gdn_glu_bwd",
+    "gdn_glu_bwd_kept",
     "gdn_glu_bwd_workspace_bytes",
     "gdn_selective_scan_fwd",
     "gdn_selective_scan_bwd",
@@ -143,6 +145,10 @@ def _declare(lib):
     lib.gdn_glu_fwd.restype = _i
     lib.gdn_glu_bwd.argtypes = [_vp] * 9 + [_i] * 4 + [_vp, _sz, _vp]
     lib.gdn_glu_bwd.restype = _i
+    lib.gdn_glu_fwd_kept.argtypes = [_vp] * 6 + [_i] * 5 + [_vp]
+    lib.gdn_glu_fwd_kept.restype = _i
+    lib.gdn_glu_bwd_kept.argtypes = [_vp] * 9 + [_i] * 5 + [_vp, _sz, _vp]
+    lib.gdn_glu_bwd_kept.restype = _i
     lib.gdn_glu_bwd_workspace_bytes.argtypes = [_i] * 4
     lib.gdn_glu_bwd_workspace_bytes.restype = _sz
     lib.gdn_selective_scan_fwd.argtypes = [_vp] * 12 + [_i] * 7 + [_vp, _sz, _vp]

@@ -175,10 +175,13 @@ size_t glu_half_bytes(int M, int I, int dtype) {
   return ((size_t)M * I * e + 255) / 256 * 256;
 }
 
-int check_glu(const void* x, const void* wg, const void* wu, int M, int D, int I, int dtype) {
+int check_glu(const void* x, const void* wg, const void* wu, int M, int D, int I, int dtype,
+              int kept) {
   g_err[0] = '\0';
   if (M < 0 || D < 0 || I < 0) return fail(GDN_ERR_INVALID, "negative size M=%d D=%d I=%d", M, D, I);
   if (int rc = check_dtype(dtype)) return rc;
+  if (kept != dtype && kept != GDN_DTYPE_FP32)
+    return fail(GDN_ERR_INVALID, "g and u are kept in the inputs' dtype or in fp32 (got %d)", kept);
   // (the CUDA-core form's grid: 65535 row tiles of 64; the tensor-core form's row indexes)
   const int most = gdn::glu_tc_widths(D, I, dtype) ? 1 << 30 : 65535 * 64;
   if (M > most || I > most || D > most)
@@ -768,7 +771,7 @@ int gdn_device_error(int clear) {
   return a ? a : (b ? b : (c ? c : (d ? d : (e ? e : f))));
 }
 
-int gdn_abi_version(void) { return (1 << 16) | 11; }
+int gdn_abi_version(void) { return (1 << 16) | 12; }
 
 int gdn_binary_version(void) { return gdn::chunk_scan_binary_version(); }
 
@@ -851,7 +854,12 @@ int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
 
 int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, void* g, void* u,
                 int M, int D, int I, int dtype, void* stream) {
-  int rc = check_glu(x, w_gate, w_up, M, D, I, dtype);
+  return gdn_glu_fwd_kept(x, w_gate, w_up, h, g, u, M, D, I, dtype, dtype, stream);
+}
+
+int gdn_glu_fwd_kept(const void* x, const void* w_gate, const void* w_up, void* h, void* g,
+                     void* u, int M, int D, int I, int dtype, int kept_dtype, void* stream) {
+  int rc = check_glu(x, w_gate, w_up, M, D, I, dtype, kept_dtype);
   if (rc) return rc;
   if (M == 0 || I == 0) return GDN_OK;
   if (!h || !aligned16(h)) return fail(GDN_ERR_INVALID, "h must be non-NULL and 16-byte aligned");
@@ -859,7 +867,7 @@ int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, vo
     return fail(GDN_ERR_INVALID, "g and u are kept together: both or neither");
   if (g && (!aligned16(g) || !aligned16(u)))
     return fail(GDN_ERR_INVALID, "g and u must be 16-byte aligned");
-  gdn::GluArgs a{x, w_gate, w_up, h, g, u, M, D, I, dtype};
+  gdn::GluArgs a{x, w_gate, w_up, h, g, u, M, D, I, dtype, kept_dtype};
   return cuda_status(gdn::launch_glu_fwd(a, (cudaStream_t)stream), "gdn_glu_fwd");
 }
 
@@ -871,7 +879,15 @@ size_t gdn_glu_bwd_workspace_bytes(int M, int D, int I, int dtype) {
 int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void* g, const void* u,
                 const void* dh, void* dx, void* dw_gate, void* dw_up, int M, int D, int I,
                 int dtype, void* workspace, size_t ws_bytes, void* stream) {
-  int rc = check_glu(x, w_gate, w_up, M, D, I, dtype);
+  return gdn_glu_bwd_kept(x, w_gate, w_up, g, u, dh, dx, dw_gate, dw_up, M, D, I, dtype, dtype,
+                          workspace, ws_bytes, stream);
+}
+
+int gdn_glu_bwd_kept(const void* x, const void* w_gate, const void* w_up, const void* g,
+                     const void* u, const void* dh, void* dx, void* dw_gate, void* dw_up, int M,
+                     int D, int I, int dtype, int kept_dtype, void* workspace, size_t ws_bytes,
+                     void* stream) {
+  int rc = check_glu(x, w_gate, w_up, M, D, I, dtype, kept_dtype);
   if (rc) return rc;
   if ((dw_gate == nullptr) != (dw_up == nullptr))
     return fail(GDN_ERR_INVALID, "dw_gate and dw_up are formed together: both or neither");
@@ -899,7 +915,7 @@ int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void*
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const size_t half = glu_half_bytes(M, I, dtype);
   gdn::GluBwdArgs a{x, w_gate, w_up, g, u, dh, ws, ws + half, dx, dw_gate, dw_up,
-                    reinterpret_cast<float*>(ws + 2 * half), M, D, I, dtype};
+                    reinterpret_cast<float*>(ws + 2 * half), M, D, I, dtype, kept_dtype};
   return cuda_status(gdn::launch_glu_bwd(a, (cudaStream_t)stream), "gdn_glu_bwd");
 }
 

@@ -321,7 +321,7 @@ cudaError_t launch_gated_norm(const void* o, const void* gate, const float* w, v
 
 // The gated linear unit h = silu(x Wg^T) * (x Wu^T) (glu.cu): x [M,D], wg, wu
 // [I,D], h [M,I], all in one dtype; g, u [M,I] (the two projections, kept for
-// the backward) or both NULL.
+// the backward) in `kept`, that dtype or fp32, or both NULL.
 struct GluArgs {
   const void* x;
   const void* wg;
@@ -329,7 +329,7 @@ struct GluArgs {
   void* h;
   void* g;
   void* u;
-  int M, D, I, dtype;
+  int M, D, I, dtype, kept;
 };
 cudaError_t launch_glu_fwd(const GluArgs& a, cudaStream_t st);
 // Its gradients from g, u and dh [M,I]; dg, du [M,I] and part (glu_part_floats()
@@ -348,7 +348,7 @@ struct GluBwdArgs {
   void* dwg;
   void* dwu;
   float* part;
-  int M, D, I, dtype;
+  int M, D, I, dtype, kept;
 };
 cudaError_t launch_glu_bwd(const GluBwdArgs& a, cudaStream_t st);
 // Their products on tcgen05 (glu_tc.cu): bf16, D and I multiples of 8 (a row's

@@ -36,6 +36,13 @@ __device__ __forceinline__ void load_vec(const T* p, int n, bool vec, float (&v)
   }
 }
 
+// A projection kept for the backward, in T or (keep32) in fp32.
+template <typename T>
+__device__ __forceinline__ void keep(T* p, long long i, float v, bool keep32) {
+  if (sizeof(T) < 4 && keep32) reinterpret_cast<float*>(p)[i] = v;
+  else p[i] = from_f32<T>(v);
+}
+
 enum GluMode : int {
   kFwd = 0,    // [g | u] = x [Wg | Wu]^T, h out (g, u out when asked for)
   kDx = 1,     // dx = dg Wg + du Wu
@@ -54,7 +61,7 @@ template <typename T, int MODE, int TR, int TC>
 __global__ void __launch_bounds__(kThreads, TR * TC >= 64 ? 2 : TR * TC >= 32 ? 3 : 4)
 glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __restrict__ B0,
                 const T* __restrict__ B1, T* __restrict__ O0, T* __restrict__ O1,
-                T* __restrict__ O2, int M, int N, int K, int kpart, bool vec) {
+                T* __restrict__ O2, int M, int N, int K, int kpart, bool vec, bool keep32) {
   constexpr int BM = 16 * TR, BN = 16 * TC, H = TC / 2;
   constexpr int BNH = MODE == kFwd ? BN / 2 : BN;   // output columns of a tile
   constexpr int LA = BM * kBK / 4 / kThreads;        // vectors of A's tile per thread
@@ -199,8 +206,8 @@ glu_simt_kernel(const T* __restrict__ A0, const T* __restrict__ A1, const T* __r
         const float sg = 1.f / (1.f + expf(-g));
         O0[m * N + n] = from_f32<T>(g * sg * u);
         if (O1) {
-          O1[m * N + n] = from_f32<T>(g);
-          O2[m * N + n] = from_f32<T>(u);
+          keep(O1, m * N + n, g, keep32);
+          keep(O2, m * N + n, u, keep32);
         }
       } else {
         T* O = MODE == kDw && blockIdx.z % 2 ? O1 : O0;
@@ -256,7 +263,8 @@ SimtPlan simt_plan(int mode, int M, int N, int K, bool parts_ok) {
 
 template <typename T, int MODE>
 cudaError_t launch_simt(const T* A0, const T* A1, const T* B0, const T* B1, T* O0, T* O1, T* O2,
-                        int M, int N, int K, const SimtPlan& p, cudaStream_t st) {
+                        int M, int N, int K, const SimtPlan& p, cudaStream_t st,
+                        bool keep32 = false) {
   // 16-byte (fp32) or 8-byte (bf16) vectors need rows that are a multiple of four elements
   const bool vec = MODE == kDw ? (M % 4 == 0 && N % 4 == 0)
                                : (K % 4 == 0 && (MODE == kFwd || N % 4 == 0));
@@ -266,7 +274,7 @@ cudaError_t launch_simt(const T* A0, const T* A1, const T* B0, const T* B1, T* O
   const dim3 grid((unsigned)((N + cols - 1) / cols), (unsigned)((M + rows - 1) / rows),
                   (MODE == kDw ? 2 : 1) * p.parts);
   auto go = [&](auto kernel) {
-    kernel<<<grid, kThreads, 0, st>>>(A0, A1, B0, B1, O0, O1, O2, M, N, K, kpart, vec);
+    kernel<<<grid, kThreads, 0, st>>>(A0, A1, B0, B1, O0, O1, O2, M, N, K, kpart, vec, keep32);
     return cudaGetLastError();
   };
   switch (p.tile) {
@@ -315,10 +323,10 @@ cudaError_t sum_parts(const float* part, int parts, long long n, long long split
 
 // dg, du from g, u, dh (n elements each): HBM-bound, three arrays read and two
 // written (8200 x 5632 in bf16: 77 us, 6.0 TB/s).
-template <typename T, bool kVec>
+template <typename T, typename Kept, bool kVec>
 __global__ void __launch_bounds__(256)
-glu_act_bwd_kernel(const T* __restrict__ g, const T* __restrict__ u, const T* __restrict__ dh,
-                   T* __restrict__ dg, T* __restrict__ du, long long n) {
+glu_act_bwd_kernel(const Kept* __restrict__ g, const Kept* __restrict__ u,
+                   const T* __restrict__ dh, T* __restrict__ dg, T* __restrict__ du, long long n) {
   constexpr int E = kVec ? 4 : 1;
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * E;
   if (i >= n) return;
@@ -390,7 +398,8 @@ __device__ __forceinline__ void lane_sums(float2* v, int lane) {
 template <typename T, int MB, bool kVec>
 __global__ void __launch_bounds__(128)
 glu_rows_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu,
-                T* __restrict__ h, T* __restrict__ go, T* __restrict__ uo, int M, int I, int K) {
+                T* __restrict__ h, T* __restrict__ go, T* __restrict__ uo, int M, int I, int K,
+                bool keep32) {
   const int lane = threadIdx.x % 32;
   const long long n0 = ((long long)blockIdx.x * 4 + threadIdx.x / 32) * 2;
   if (n0 >= I) return;
@@ -467,8 +476,8 @@ glu_rows_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* __re
     const float sg = 1.f / (1.f + expf(-g));
     h[m * I + c] = from_f32<T>(g * sg * u);
     if (go) {
-      go[m * I + c] = from_f32<T>(g);
-      uo[m * I + c] = from_f32<T>(u);
+      keep(go, m * I + c, g, keep32);
+      keep(uo, m * I + c, u, keep32);
     }
   }
 }
@@ -480,9 +489,11 @@ cudaError_t launch_rows(const GluArgs& a, cudaStream_t st) {
           *wu = static_cast<const T*>(a.wu);
   T *h = static_cast<T*>(a.h), *g = static_cast<T*>(a.g), *u = static_cast<T*>(a.u);
   if (a.D % 4 == 0)
-    glu_rows_kernel<T, MB, true><<<grid, 128, 0, st>>>(x, wg, wu, h, g, u, a.M, a.I, a.D);
+    glu_rows_kernel<T, MB, true><<<grid, 128, 0, st>>>(x, wg, wu, h, g, u, a.M, a.I, a.D,
+                                                       a.kept == kFP32);
   else
-    glu_rows_kernel<T, MB, false><<<grid, 128, 0, st>>>(x, wg, wu, h, g, u, a.M, a.I, a.D);
+    glu_rows_kernel<T, MB, false><<<grid, 128, 0, st>>>(x, wg, wu, h, g, u, a.M, a.I, a.D,
+                                                        a.kept == kFP32);
   return cudaGetLastError();
 }
 
@@ -501,20 +512,20 @@ cudaError_t fwd_simt(const GluArgs& a, cudaStream_t st) {
   return launch_simt<T, kFwd>(static_cast<const T*>(a.x), nullptr, static_cast<const T*>(a.wg),
                               static_cast<const T*>(a.wu), static_cast<T*>(a.h),
                               static_cast<T*>(a.g), static_cast<T*>(a.u), a.M, a.I, a.D,
-                              p, st);
+                              p, st, a.kept == kFP32);
 }
 
-template <typename T>
+template <typename T, typename Kept>
 cudaError_t act_bwd(const GluBwdArgs& a, cudaStream_t st) {
   const long long n = (long long)a.M * a.I;
   const bool vec = n % 4 == 0;
   const long long blocks = (n / (vec ? 4 : 1) + 255) / 256;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const T *g = static_cast<const T*>(a.g), *u = static_cast<const T*>(a.u),
-          *dh = static_cast<const T*>(a.dh);
+  const Kept *g = static_cast<const Kept*>(a.g), *u = static_cast<const Kept*>(a.u);
+  const T* dh = static_cast<const T*>(a.dh);
   T *dg = static_cast<T*>(a.dg), *du = static_cast<T*>(a.du);
-  if (vec) glu_act_bwd_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(g, u, dh, dg, du, n);
-  else glu_act_bwd_kernel<T, false><<<(unsigned)blocks, 256, 0, st>>>(g, u, dh, dg, du, n);
+  if (vec) glu_act_bwd_kernel<T, Kept, true><<<(unsigned)blocks, 256, 0, st>>>(g, u, dh, dg, du, n);
+  else glu_act_bwd_kernel<T, Kept, false><<<(unsigned)blocks, 256, 0, st>>>(g, u, dh, dg, du, n);
   return cudaGetLastError();
 }
 
@@ -565,7 +576,9 @@ cudaError_t launch_glu_fwd(const GluArgs& a, cudaStream_t st) {
 }
 
 cudaError_t launch_glu_bwd(const GluBwdArgs& a, cudaStream_t st) {
-  const cudaError_t e = a.dtype == kBF16 ? act_bwd<__nv_bfloat16>(a, st) : act_bwd<float>(a, st);
+  const cudaError_t e = a.dtype == kFP32   ? act_bwd<float, float>(a, st)
+                        : a.kept == kFP32 ? act_bwd<__nv_bfloat16, float>(a, st)
+                                          : act_bwd<__nv_bfloat16, __nv_bfloat16>(a, st);
   if (e != cudaSuccess) return e;
   if (glu_tc_supported(a.M, a.D, a.I, a.dtype)) return launch_glu_tc_bwd(a, st);
   return a.dtype == kBF16 ? bwd_products_simt<__nv_bfloat16>(a, st)

@@ -24,11 +24,11 @@
 // ms back to back under the power cap; 8200 tokens: 257 us storing g and u too
 // (tensor pipe 86 % busy), dx 260 and both weights' gradients 243 us (95 %).
 //
-// Roundings: accumulators are fp32.  g and u are kept in bf16 for the backward and
-// dg, du are rounded to bf16 as its products' operands, each by at most 2^-9 of the
-// value: together they take a gradient's error in the norm from 1.7e-3 (its own
-// rounding) to 3.1e-3.  Keeping g and u in fp32 would double what a training step
-// keeps of them.
+// Roundings: accumulators are fp32.  dg, du are rounded to bf16 as the backward's
+// operands, by at most 2^-8 of the value, which takes a gradient's error in the norm from
+// 1.7e-3 (its own rounding) to 2.4e-3.  g and u are kept in fp32 for it: in bf16 they
+// would halve what a training step keeps of them, and their roundings would make it 3.1e-3
+// (a caller of the library may ask for that).
 #include <algorithm>
 
 #include "gdn_common.cuh"
@@ -66,7 +66,7 @@ struct alignas(64) GluMaps {
 struct GluShape {
   int tiles_m, tiles_n;   // output tiles (kDw: of dWg; dWu has as many again)
   int kblocks;            // 64-wide steps along the contraction (kDx: of each half)
-  int keep;               // kFwd: g and u are stored
+  int keep;               // kFwd: g and u are stored (1: bf16, 2: fp32)
   int rows, cols;         // of the output
   // kDx, kDw: the contraction's parts and their steps.  With more than one, part p's sums
   // leave in fp32 for rows 256 tiles_m p .. (kDw: 512 tiles_m p, dWg's before dWu's) of out[2].
@@ -251,6 +251,12 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
         *reinterpret_cast<uint4*>(box + sw128(row, chunk + c)) = q;
       }
     };
+    auto put_fp32 = [&](unsigned char* box, const float (&v)[32]) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<float4*>(box + sw128(row, c)) =
+            make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    };
     uint32_t j = 0;
     bool ok = true;
     for (long long t = pair; ok && t < items; t += npairs, ++j) {
@@ -284,7 +290,17 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
         }
         if (!sh.keep) release();
         end_box(&maps.out[0], c0, r0, box);
-        if (sh.keep) {
+        if (sh.keep == 2) {
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {   // g, then u, 32 columns a box
+            box = begin_box();
+            float v[32];
+            tmem_ld32(acc + (w >> 1) * 128 + half * 64 + (w & 1) * 32, v);
+            put_fp32(box, v);
+            if (w == 3) release();
+            end_box(&maps.out[1 + (w >> 1)], c0 + (w & 1) * 32, r0, box);
+          }
+        } else if (sh.keep) {
 #pragma unroll 1
           for (int w = 0; w < 2; ++w) {   // g, then u
             box = begin_box();
@@ -304,10 +320,7 @@ glu_tc_kernel(const __grid_constant__ GluMaps maps, const GluShape sh) {
           unsigned char* box = begin_box();
           float v[32];
           tmem_ld32(acc + half * 128 + w * 32, v);
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<float4*>(box + sw128(row, c)) =
-                make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+          put_fp32(box, v);
           if (w == 3) release();
           end_box(&maps.out[2], n * kTile + half * 128 + w * 32,
                   (KIND == kDw ? 2 * part + second : part) * sh.tiles_m * kTile + r0, box);
@@ -355,6 +368,7 @@ static_assert(kFewBK == kBK, "the operands' boxes are shared");
 struct FewShape {
   int M, I, kblocks, n, stages, cols, split;   // n: tokens rounded up to 16
   int share;                                   // tokens a CTA finishes (a multiple of 4)
+  bool keep32;                                 // g and u are kept in fp32
 };
 struct alignas(64) FewMaps {
   CUtensorMap x, wg, wu;
@@ -362,8 +376,7 @@ struct alignas(64) FewMaps {
 
 __global__ void __launch_bounds__(kFewThreads)
 glu_few_kernel(const __grid_constant__ FewMaps maps, const FewShape sh,
-               __nv_bfloat16* __restrict__ h, __nv_bfloat16* __restrict__ gk,
-               __nv_bfloat16* __restrict__ uk) {
+               __nv_bfloat16* __restrict__ h, void* __restrict__ gk, void* __restrict__ uk) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = smem_raw + (1024u - (smem_u32(smem_raw) & 1023u)) % 1024u;
   __shared__ __align__(8) uint64_t full[kFewMaxStages], empty[kFewMaxStages], done;
@@ -483,9 +496,12 @@ glu_few_kernel(const __grid_constant__ FewMaps maps, const FewShape sh,
       if (tl + e >= mine) break;
       const size_t o = (size_t)(first + tl + e) * sh.I + col;
       h[o] = __float2bfloat16_rn(gv[e] * fast_sigmoid(gv[e]) * uv[e]);
-      if (gk) {
-        gk[o] = __float2bfloat16_rn(gv[e]);
-        uk[o] = __float2bfloat16_rn(uv[e]);
+      if (gk && sh.keep32) {
+        static_cast<float*>(gk)[o] = gv[e];
+        static_cast<float*>(uk)[o] = uv[e];
+      } else if (gk) {
+        static_cast<__nv_bfloat16*>(gk)[o] = __float2bfloat16_rn(gv[e]);
+        static_cast<__nv_bfloat16*>(uk)[o] = __float2bfloat16_rn(uv[e]);
       }
     }
   }
@@ -571,7 +587,8 @@ cudaError_t launch_few(const GluArgs& a, cudaStream_t st) {
   FewMaps m;
   const FewPlan p = few_plan(a.M, a.D, a.I, device_sm_count());
   if (!p.fits()) return cudaErrorInvalidValue;
-  const FewShape sh{a.M, a.I, p.kblocks, p.n, p.stages, p.cols, p.split, p.share};
+  const FewShape sh{a.M, a.I, p.kblocks, p.n, p.stages, p.cols, p.split, p.share,
+                    a.kept == kFP32};
   // (a box of n rows past the M there are is filled with zeros)
   if (!make_map(&m.x, a.x, a.M, a.D, sh.n) || !make_map(&m.wg, a.wg, a.I, a.D, kFewRows) ||
       !make_map(&m.wu, a.wu, a.I, a.D, kFewRows))
@@ -592,8 +609,8 @@ cudaError_t launch_few(const GluArgs& a, cudaStream_t st) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = sh.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, glu_few_kernel, m, sh, static_cast<__nv_bfloat16*>(a.h),
-                            static_cast<__nv_bfloat16*>(a.g), static_cast<__nv_bfloat16*>(a.u));
+  return cudaLaunchKernelEx(&cfg, glu_few_kernel, m, sh, static_cast<__nv_bfloat16*>(a.h), a.g,
+                            a.u);
 }
 
 }  // namespace
@@ -617,13 +634,13 @@ cudaError_t launch_glu_tc_fwd(const GluArgs& a, cudaStream_t st) {
   GluMaps m;
   if (!make_map(&m.a[0], a.x, a.M, a.D, 128) || !make_map(&m.b[0], a.wg, a.I, a.D, 128) ||
       !make_map(&m.b[1], a.wu, a.I, a.D, 128) || !make_map(&m.out[0], a.h, a.M, a.I, 128) ||
-      (a.g && (!make_map(&m.out[1], a.g, a.M, a.I, 128) ||
-               !make_map(&m.out[2], a.u, a.M, a.I, 128))))
+      (a.g && (!make_map(&m.out[1], a.g, a.M, a.I, 128, a.kept == kFP32) ||
+               !make_map(&m.out[2], a.u, a.M, a.I, 128, a.kept == kFP32))))
     return cudaErrorInvalidValue;
   m.a[1] = m.a[0];
   if (!a.g) m.out[1] = m.out[2] = m.out[0];
   const GluShape sh{ceil_div(a.M, kTile), ceil_div(a.I, 128), ceil_div(a.D, kBK),
-                    a.g != nullptr, a.M, a.I};
+                    a.g == nullptr ? 0 : a.kept == kFP32 ? 2 : 1, a.M, a.I};
   return launch_kind<kFwd>(m, sh, st);
 }
 

@@ -758,19 +758,22 @@ def _glu_fwd(x, wg, wu, keep):
     the two projections."""
     (M, D), I = x.shape, wg.shape[0]
     h = x.new_empty((M, I))
-    g, u = (x.new_empty((M, I)), x.new_empty((M, I))) if keep else (None, None)
+    # (in fp32 whatever x's type: rounded to bf16, they would be most of the gradients' error)
+    g = u = None
+    if keep:
+        g, u = h.new_empty((M, I), dtype=torch.float32), h.new_empty((M, I), dtype=torch.float32)
     lib = _lib.load()
     dev = x.get_device()
     with _on_device(dev):
-        rc = lib.gdn_glu_fwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(h), _ptr(g), _ptr(u), M, D, I,
-                             _DTYPES[x.dtype], _stream(dev))
+        rc = lib.gdn_glu_fwd_kept(_ptr(x), _ptr(wg), _ptr(wu), _ptr(h), _ptr(g), _ptr(u), M, D, I,
+                                  _DTYPES[x.dtype], _lib.GDN_DTYPE_FP32, _stream(dev))
     _lib.check(rc, "gdn_glu_fwd")
     return h, g, u
 
 
 def _glu_formula(x, wg, wu):
     """The gated linear unit in torch's operations: products in the inputs' type, the
-    activation in fp32, as the kernels round."""
+    activation in fp32."""
     lin = torch.nn.functional.linear
     g, u = lin(x, wg), lin(x, wu)
     if x.dtype == torch.bfloat16:
@@ -789,9 +792,9 @@ def _glu_bwd(dh, x, wg, wu, g, u, need_x, need_w):
     with _on_device(dev):
         n = lib.gdn_glu_bwd_workspace_bytes(M, D, I, _DTYPES[x.dtype])
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=x.device)
-        rc = lib.gdn_glu_bwd(_ptr(x), _ptr(wg), _ptr(wu), _ptr(g), _ptr(u), _ptr(dh),
-                             _ptr(dx), _ptr(dwg), _ptr(dwu), M, D, I, _DTYPES[x.dtype],
-                             _ptr(ws), n, _stream(dev))
+        rc = lib.gdn_glu_bwd_kept(_ptr(x), _ptr(wg), _ptr(wu), _ptr(g), _ptr(u), _ptr(dh),
+                                  _ptr(dx), _ptr(dwg), _ptr(dwu), M, D, I, _DTYPES[x.dtype],
+                                  _lib.GDN_DTYPE_FP32, _ptr(ws), n, _stream(dev))
     _lib.check(rc, "gdn_glu_bwd")
     return dx, dwg, dwu
 
@@ -836,7 +839,7 @@ def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") ->
     x ``[...,D]``, gate_weight and up_weight ``[I,D]`` (torch's Linear layout)
     in one dtype, bfloat16 or float32, on a CUDA device; returns ``[...,I]``.
     ``activation``: ``'silu'`` / ``'swish'``.  Differentiable in all three
-    (gdn_glu_bwd, from the two projections kept in x's dtype), twice too (second
+    (gdn_glu_bwd, from the two projections kept in float32), twice too (second
     derivatives run on torch's operations).  bfloat16 widths D and I that are multiples of
     8 run on the tensor cores, others on CUDA cores.
     """

@@ -423,6 +423,11 @@ int gdn_short_conv_bwd(const void* x, const float* weight, const float* bias,
  */
 int gdn_glu_fwd(const void* x, const void* w_gate, const void* w_up, void* h, void* g, void* u,
                 int M, int D, int I, int dtype, void* stream);
+/* The same with g and u in `kept_dtype`, the inputs' dtype or fp32 (bf16
+ * gradients from fp32 projections are off by 1.4 roundings in the norm, from
+ * bf16 ones by 1.9). */
+int gdn_glu_fwd_kept(const void* x, const void* w_gate, const void* w_up, void* h, void* g,
+                     void* u, int M, int D, int I, int dtype, int kept_dtype, void* stream);
 
 /*
  * Its gradients from dh [M, I] and the forward's g and u: dx [M, D] (NULL: not
@@ -436,6 +441,11 @@ size_t gdn_glu_bwd_workspace_bytes(int M, int D, int I, int dtype);
 int gdn_glu_bwd(const void* x, const void* w_gate, const void* w_up, const void* g, const void* u,
                 const void* dh, void* dx, void* dw_gate, void* dw_up, int M, int D, int I,
                 int dtype, void* workspace, size_t ws_bytes, void* stream);
+/* From g and u as gdn_glu_fwd_kept wrote them. */
+int gdn_glu_bwd_kept(const void* x, const void* w_gate, const void* w_up, const void* g,
+                     const void* u, const void* dh, void* dx, void* dw_gate, void* dw_up, int M,
+                     int D, int I, int dtype, int kept_dtype, void* workspace, size_t ws_bytes,
+                     void* stream);
 
 /*
  * Selective state-space scan (no counterpart in the reference).  Per row b,
@@ -489,7 +499,7 @@ int gdn_selective_scan_bwd(const void* x, const void* dt, const float* A, const 
  * the other tensor-core shapes and the general recurrent shapes,
  * gdn_short_conv_fwd, gdn_gated_rmsnorm_fwd; 1.10: gdn_chunk_bwd_workspace_bytes_for;
  * 1.11: the gated linear unit, the selective scan, the short convolution's bias
- * and gradients). */
+ * and gradients; 1.12: the gated linear unit's projections kept in fp32). */
 int gdn_abi_version(void);
 
 /*

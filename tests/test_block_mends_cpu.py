@@ -258,3 +258,16 @@ def test_glu_few_token_layout_stays_in_its_memory(tmp_path):
                    check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout.startswith("0 of 64512"), r.stdout
+
+
+def test_glu_kept_types(lib):
+    """g and u in the inputs' type or fp32."""
+    def fwd(dtype, kept):
+        return lib.gdn_glu_fwd_kept(_at(1), _at(2), _at(3), None, _at(5), _at(6), 4, 64, 32, dtype,
+                                    kept, None)
+    for dtype, kept in ((FP32, BF16), (BF16, 7)):
+        assert fwd(dtype, kept) == INVALID and b"kept" in lib.gdn_last_error()
+    for dtype, kept in ((FP32, FP32), (BF16, FP32), (BF16, BF16)):
+        assert fwd(dtype, kept) == INVALID and b"h must be" in lib.gdn_last_error()
+    assert lib.gdn_glu_bwd_kept(_at(1), _at(2), _at(3), _at(4), _at(5), _at(6), _at(7), _at(8),
+                                _at(9), 4, 64, 32, FP32, BF16, _at(10), 1 << 20, None) == INVALID

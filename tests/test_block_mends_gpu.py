@@ -78,6 +78,67 @@ def test_glu_inputs_wider_than_the_tensor_core_form(cuda):
     _sum_error(h, g * torch.sigmoid(g) * u, "h")
 
 
+FORMS = [(5, 256, 328), (64, 512, 136), (300, 256, 328), (1100, 72, 264), (300, 130, 66),
+         (7, 250, 66)]   # few tokens, tiles of CTA pairs, CUDA cores
+
+
+@pytest.mark.parametrize("M,D,I", FORMS)
+def test_glu_bf16_gradients_carry_two_roundings(cuda, M, D, I):
+    """A gradient is rounded once itself and once through dg or du, the products' bf16
+    operands.  Roundings of one spread (relative, between 0.39 and 0.43 of 2^-8 in the
+    mean square for values of such distributions) make 1.42 of one at most 1.5."""
+    gen = _gen(cuda, M + I)
+    rn = lambda *s: torch.randn(*s, device=cuda, generator=gen)   # noqa: E731
+    x, dh = rn(M, D).bfloat16(), rn(M, I).bfloat16()
+    wg, wu = ((rn(I, D) * D ** -0.5).bfloat16() for _ in range(2))
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu)]
+    got = torch.autograd.grad(gated_linear_unit(*leaves), leaves, dh)
+    xd, gd, ud = (t.detach().double() for t in leaves)
+    a, b = _silu_grads(xd @ gd.T, xd @ ud.T, dh.double())
+    for out, ref in zip(got, (a @ gd + b @ ud, a.T @ xd, b.T @ xd)):
+        once = (ref.bfloat16().double() - ref).norm()
+        assert float((out.double() - ref).norm() / once) <= 1.5
+
+
+@pytest.mark.parametrize("M,D,I", FORMS)
+def test_glu_projections_kept_in_either_type(cuda, M, D, I):
+    """The library's two forms: g and u in fp32 are the fp32 sums, in bf16 those rounded
+    once; h is the same, and the gradients are the same but for their roundings."""
+    lib = _lib.load()
+    gen = _gen(cuda, M)
+    rn = lambda *s: torch.randn(*s, device=cuda, generator=gen)   # noqa: E731
+    x, dh = rn(M, D).bfloat16(), rn(M, I).bfloat16()
+    wg, wu = ((rn(I, D) * D ** -0.5).bfloat16() for _ in range(2))
+    st = torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(lib.gdn_glu_bwd_workspace_bytes(M, D, I, _lib.GDN_DTYPE_BF16),
+                     dtype=torch.uint8, device=cuda)
+    p = lambda *ts: [t.data_ptr() for t in ts]   # noqa: E731
+    out = {}
+    for kept, dt in ((_lib.GDN_DTYPE_FP32, torch.float32), (_lib.GDN_DTYPE_BF16, torch.bfloat16)):
+        h = torch.empty(M, I, device=cuda, dtype=torch.bfloat16)
+        flat = torch.full((2, (M * I + 64) // 64 * 64), 3.0, device=cuda, dtype=dt)
+        g, u = flat[0, :M * I].view(M, I), flat[1, :M * I].view(M, I)
+        grads = [torch.empty_like(t) for t in (x, wg, wu)]
+        assert lib.gdn_glu_fwd_kept(*p(x, wg, wu, h, g, u), M, D, I, 1, kept, st) == 0
+        assert lib.gdn_glu_bwd_kept(*p(x, wg, wu, g, u, dh, *grads), M, D, I, 1, kept, *p(ws),
+                                    ws.numel(), st) == 0
+        assert bool((flat[:, M * I:] == 3.0).all())
+        out[dt] = [h, g, u] + grads
+    a, b = out[torch.float32], out[torch.bfloat16]
+    assert torch.equal(a[0], b[0])
+    assert torch.equal(a[1].bfloat16(), b[1]) and torch.equal(a[2].bfloat16(), b[2])
+    # (an accumulator's step of 16 terms drops a last place, 2^-23, of it at most)
+    assert _rel(a[1], x.double() @ wg.double().T) <= (D / 16 + 8) * 2.0 ** -23
+    for s, t in zip(a[3:], b[3:]):
+        assert _rel(t, s) <= 5 * 2.0 ** -8
+    # the calls without a type keep x's
+    h, g, u = (torch.empty_like(t) for t in b[:3])
+    assert lib.gdn_glu_fwd(*p(x, wg, wu, h, g, u), M, D, I, 1, st) == 0
+    grads = [torch.empty_like(t) for t in (x, wg, wu)]
+    assert lib.gdn_glu_bwd(*p(x, wg, wu, g, u, dh, *grads), M, D, I, 1, *p(ws), ws.numel(), st) == 0
+    assert all(torch.equal(s, t) for s, t in zip([h, g, u] + grads, b))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("M,D,I", [(0, 64, 40), (5, 64, 0), (0, 64, 0), (5, 0, 40), (0, 33, 7),
                                    (5, 33, 0), (0, 64, 5_000_000)])
