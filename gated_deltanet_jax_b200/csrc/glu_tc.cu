@@ -21,8 +21,8 @@
 // warps run the epilogue through 128-byte-swizzled staging and TMA stores, which
 // clip ragged edges (loads fill them with zeros).  16384 tokens of 2048 x 5632:
 // 478 us in short runs, 1582 TFLOP/s (0.96 of the measured bf16 rate), 0.54 to 0.56
-// ms back to back under the power cap; 8200 tokens: 257 us storing g and u too
-// (tensor pipe 86 % busy), dx 260 and both weights' gradients 243 us (95 %).
+// ms back to back under the power cap; 8200 tokens: 280 us storing g and u in fp32 too
+// (257 in bf16), dx 260 and both weights' gradients 244 us (tensor pipe 95 % busy).
 //
 // Roundings: accumulators are fp32.  dg, du are rounded to bf16 as the backward's
 // operands, by at most 2^-8 of the value, which takes a gradient's error in the norm from

@@ -34,7 +34,8 @@ constexpr float kDecayBias = 0x1p-25f;
 
 // softplus(v) = max(v, 0) + log(1 + e), e = exp(-|v|) <= 1, the logarithm as
 // 2 atanh(s) with s = e / (2 + e) <= 1/3: the series s + s^3 / 3 + ... + s^13 / 13
-// leaves less than s^15 / 15 / (1 - s^2) < 2^-27 of it out.  No cancellation at small
+// leaves less than 2 s^15 / 15 / (1 - s^2) out, 1.1e-8 at s = 1/3 and there 2^-26 of the
+// logarithm, less of it at smaller s.  No cancellation at small
 // e, where step sizes lie.  A NaN stays one (through e).
 __device__ __forceinline__ float softplus_e(float v, float e) {
   const float s = e * fast_rcp(2.f + e);
@@ -167,7 +168,8 @@ __device__ __forceinline__ void store_pairs(float* p, const float2 (&v)[scan_pai
 __device__ __forceinline__ float& pair_at(float2& v, int i) { return i ? v.y : v.x; }
 
 // Tokens of the backward's tile (and the distance of the forward's checkpoints)
-// for NL states a lane: 64 decay factors a lane stay in registers.
+// for NL states a lane: half a tile's states of the lane's two channels, 64 of them at
+// most, stay in registers.
 template <int NL>
 constexpr int scan_tile() { return NL <= 4 ? 16 : 64 / NL; }
 

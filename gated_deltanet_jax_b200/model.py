@@ -98,7 +98,7 @@ class ShortConvolution(nn.Module):
     ``weight`` [K, C] (the Flax depthwise kernel [K, 1, C] squeezed), optional bias.
     On the GPU kernel (gdn_short_conv_fwd) for inference without a bias, and with its
     backward (gdn_short_conv_bwd) for training at the shapes they take; torch's
-    conv1d elsewhere."""
+    conv1d elsewhere, and under torch's tracing, modes and transforms."""
 
     def __init__(self, hidden_size: int, kernel_size: int, activation: Optional[str] = "silu",
                  use_bias: bool = False):
@@ -243,7 +243,8 @@ class GatedDeltaNetMLP(nn.Module):
     (``ops.gated_linear_unit``).  Inference keeps torch's separate operations, and
     with them the bits it gave before, unless ``fused_inference`` is set (on the
     class or an instance): the kernel rounds once where they round four times, and
-    takes 0.49 ms against 0.65 for 16384 tokens of 2048 x 5632."""
+    takes 0.51 ms against 0.77 back to back for 16384 tokens of 2048 x 5632 (0.48
+    against 0.65 in short runs)."""
 
     fused_inference = False
 

@@ -841,7 +841,7 @@ def gated_linear_unit(x, gate_weight, up_weight, *, activation: str = "silu") ->
     ``activation``: ``'silu'`` / ``'swish'``.  Differentiable in all three
     (gdn_glu_bwd, from the two projections kept in float32), twice too (second
     derivatives run on torch's operations).  bfloat16 widths D and I that are multiples of
-    8 run on the tensor cores, others on CUDA cores.
+    8 (D up to 131072) run on the tensor cores, others on CUDA cores.
     """
     _cuda_input("x", x)
     if activation not in ("silu", "swish"):
